@@ -563,20 +563,27 @@ def _own_sparse(s):
     return ops.kv8_sparse_attn(s["q"], cache, idx=s["idx"], sel_lens=s["picks"], **tail)
 
 
-def _own_fork(s):
+def _buffers(s):
+    """The list of the layers' arrays, made once by a program."""
     from omnikv_amd import ops
 
+    if "handle" not in s:
+        s["handle"] = ops.PageBuffers(s["buffers"])
+    return ops, s["handle"]
+
+
+def _own_fork(s):
+    ops, buffers = _buffers(s)
     page, state = s["case"]["page"], (s["page_table"], s["seq_lens"], s["refs"])
     ops.pages_free(*state, s["to"], page)
-    ops.pages_fork(*state, s["from"], s["to"], page, s["buffers"])
+    ops.pages_fork(*state, s["from"], s["to"], page, buffers)
     ops.pages_extend(*state, s["to"], s["grow"], page)
     return [s["page_table"], s["refs"], s["seq_lens"]] + [s[n] for n in ("k", "v", "k_scale", "v_scale")]
 
 
 def _own_compact(s):
-    from omnikv_amd import ops
-
-    table, refs, _ = ops.pages_compact(s["page_table"], s["refs"], s["buffers"])
+    ops, buffers = _buffers(s)
+    table, refs, _ = ops.pages_compact(s["page_table"], s["refs"], buffers)
     return [table, refs] + [s[n] for n in ("k", "v", "k_scale", "v_scale")]
 
 
