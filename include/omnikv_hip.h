@@ -54,7 +54,9 @@ enum okv_status {
   OKV_ERR_HIP = -4          /* a HIP runtime call failed */
 };
 
-enum okv_dtype { OKV_F32 = 0, OKV_BF16 = 1, OKV_F16 = 2 };
+/* OKV_E4M3 (OCP fp8: 4 exponent, 3 mantissa bits, largest value 448) and OKV_I8 are code formats of
+ * okv_kv8_cache_t; no other argument takes them. */
+enum okv_dtype { OKV_F32 = 0, OKV_BF16 = 1, OKV_F16 = 2, OKV_E4M3 = 3, OKV_I8 = 4 };
 
 /* How the per-head logits of a token become one score. */
 enum okv_head_reduce { OKV_REDUCE_MAX = 0, OKV_REDUCE_SUM = 1 };
@@ -372,6 +374,169 @@ int okv_offload_plan(const int32_t* idx_new, int32_t k, int32_t* slot_tok, int32
 int okv_offload_fetch(const void* src, int64_t row_bytes, const int32_t* fetch_tok,
                       const int32_t* fetch_slot, const int32_t* fetch_count, int32_t max_rows,
                       void* dev_dst, okv_stream_t stream);
+
+/*
+ * K/V cache in 8 bits.  A (token, kv head) row is head_dim = 128 codes of one byte; block_tokens
+ * consecutive tokens (16, 32, 64 or 128; blocks start at multiples of it) of one kv head share one fp32 scale, K and V
+ * one each:
+ *   scale = max(fl32(amax / qmax), 2^-126), qmax = 448 (OKV_E4M3) or 127 (OKV_I8)
+ *   code  = the format's value nearest to fl32(x * fl32(1 / scale)), ties to even;  value = code * scale
+ * A block that holds a NaN or an infinity gets the scale NaN (and codes 0), so that whatever attends to it
+ * shows it, as 16-bit K/V would.  Each element is rounded once: the rows of a sequence's last, not yet full block wait
+ * in 16 bits in the request's open buffer (block_tokens rows per kv head, row t of the sequence in
+ * slot t % block_tokens) and are quantised together when the block fills.  A cache without open
+ * buffers is closed: all its rows are codes, the last block possibly a short one, and it takes no
+ * further rows.  No counterpart in the reference, whose cache is 16-bit.
+ *   element (b, t, g, d): contiguous  codes + b*batch_stride + t*token_stride + g*head_stride + d
+ *                         paged       codes + page_table[b*page_table_stride + t/page_size]*page_stride
+ *                                           + (t%page_size)*token_stride + g*head_stride + d
+ *   its scale:            contiguous  scale + b*scale_batch_stride + (t/block)*scale_block_stride + g*scale_head_stride
+ *                         paged       scale + page*scale_page_stride + (t%page_size/block)*scale_block_stride + g*scale_head_stride
+ * Code strides are in bytes and multiples of 16, scale strides in floats; block_tokens divides
+ * page_size and capacity.  A page number outside [0, num_pages) is never followed: reading, its tokens take no part in
+ * the softmax (their raw score is -inf); writing, its rows are dropped.
+ */
+typedef struct okv_kv8_cache {
+  void* k_codes; /* 16-byte aligned */
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  int32_t format; /* OKV_E4M3 or OKV_I8 */
+  int32_t dtype;  /* OKV_BF16 or OKV_F16: queries, new rows, open rows, tails, outputs */
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t block_tokens;
+  int32_t capacity; /* tokens a request has room for; paged: ignored (page_table_stride pages) */
+  int64_t token_stride, head_stride, batch_stride;
+  int64_t scale_block_stride, scale_head_stride, scale_batch_stride;
+  const int32_t* page_table; /* device; NULL selects contiguous mode */
+  int32_t page_size;
+  int32_t page_table_stride; /* entries per request */
+  int32_t num_pages;         /* pages of the pool */
+  int64_t page_stride, scale_page_stride;
+  void* open_k; /* element (b, slot, g, d) at open_k + b*open_batch_stride + slot*open_token_stride + g*open_head_stride + d; */
+  void* open_v; /* both NULL for a closed cache; 16-byte aligned, strides in elements, multiples of 8 */
+  int64_t open_token_stride, open_head_stride, open_batch_stride;
+} okv_kv8_cache_t;
+
+/*
+ * Appends new_len rows of K and V per request behind its first `start` rows: the blocks they
+ * complete become codes, the rest waits in the open buffers.  New element (b, r, g, d) at
+ * new_k + b*new_batch_stride + r*new_token_stride + g*new_head_stride + d (strides in elements,
+ * multiples of 8, 16-byte aligned).  starts (device int32[batch]) or start for every request;
+ * new_lens (device int32[batch]) or max_new for every request.  close = 1 quantises a short last
+ * block too (over its own rows; the rows behind it are left as they were): with close, or without
+ * open buffers, starts must be NULL and start a multiple of block_tokens, and without open buffers
+ * close must be 1 or every request must end at a block's border (max_new a multiple, new_lens NULL).
+ * A request whose rows would not fit (start < 0, or start + new_len beyond its room) is left as it was.
+ */
+int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, const void* new_v,
+                   int64_t new_token_stride, int64_t new_head_stride, int64_t new_batch_stride,
+                   const int32_t* starts, int32_t start, const int32_t* new_lens, int32_t max_new,
+                   int32_t close, int32_t batch, okv_stream_t stream);
+
+/* Scratch of the two attention calls: `max_rows` is max_seq_len, or max_sel_len + max_tail_len;
+ * max_score_len 0 without scores. */
+int okv_kv8_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t max_rows,
+                            int32_t max_score_len, size_t* out_bytes);
+
+/*
+ * okv_dense_attn over an 8-bit cache: the rows [0, seq_len) of each request, those behind the last
+ * full block from its open buffer, with optional filter-layer scores of the first score_len rows
+ * (as okv_score defines them).  num_q_heads is num_kv_heads times a group of 1 to 8.  Lengths read
+ * from the device count as clamped to [0, max_seq_len] and [0, min(max_score_len, seq_len)]; a request without rows gets
+ * zeros.
+ */
+int okv_kv8_dense_attn(const void* q, int32_t num_q_heads, const okv_kv8_cache_t* cache,
+                       const int32_t* seq_lens, int32_t max_seq_len, int32_t batch, float scale, void* out,
+                       const int32_t* score_lens, int32_t max_score_len, int32_t head_reduce,
+                       int32_t normalise, float* scores, int64_t score_stride, void* ws, size_t ws_bytes,
+                       okv_stream_t stream);
+
+/*
+ * okv_sparse_attn over an 8-bit cache: rows idx[b][0 .. sel_len_b) of the codes (idx NULL: rows
+ * 0 .. sel_len_b-1) followed by tail_len_b 16-bit tail rows, one softmax.  An index outside the request's
+ * room takes no part.  slots = 1: idx holds rows of a paged pool seen as one array of token slots
+ * (page * page_size + slot; needs page_stride = page_size*token_stride and the scales likewise), so
+ * that the page table is looked up once per selection instead of once per layer.  The open buffers are
+ * not read: the rows an index may name are those that are codes.
+ */
+int okv_kv8_sparse_attn(const void* q, int32_t num_q_heads, const okv_kv8_cache_t* cache, const int32_t* idx,
+                        int64_t idx_stride, int32_t slots, const int32_t* sel_lens, int32_t max_sel_len,
+                        const void* tail_k, const void* tail_v, int64_t tail_token_stride,
+                        int64_t tail_head_stride, int64_t tail_batch_stride, const int32_t* tail_lens,
+                        int32_t max_tail_len, int32_t batch, float scale, void* out, void* ws,
+                        size_t ws_bytes, okv_stream_t stream);
+
+/* out[b][j][g][:] = codes * scale of row idx[b][j] (idx NULL: row j), in `dtype` (cache->dtype); rows behind
+ * the last full block come from the open buffers when seq_lens / max_seq_len name the requests'
+ * lengths, as in okv_kv8_dense_attn; rows outside a request are written as zeros.  Strides in elements, multiples of 8.
+ * What a caller that wants 16-bit K/V tensors gets (the values update() returns). */
+int okv_kv8_read(const okv_kv8_cache_t* cache, const int32_t* idx, int64_t idx_stride, int32_t max_rows,
+                 const int32_t* seq_lens, int32_t max_seq_len, int32_t batch, void* k_out, void* v_out,
+                 int64_t out_token_stride, int64_t out_head_stride, int64_t out_batch_stride,
+                 okv_stream_t stream);
+
+/*
+ * Pages of a cache.  Sequence s of a pool holds ceil(lens[s] / page_size) pages, named in row s of
+ * `table` (entries behind them are -1); refs[p] counts the rows that name page p, and a page with
+ * refs[p] = 0 is free.  All of it lives in device memory and every call below is one or two launches
+ * on `stream`, so a step of page operations can be captured in a HIP graph.  The pool's data are
+ * `buffers`: for every layer's K, V and scales one array of num_pages pages, page p at base +
+ * p*page_bytes (base and page_bytes multiples of 4; of 16 for speed), listed in HOST memory.  Pages
+ * are handed out lowest first, in the order of the call's entries, so results are reproducible.
+ *
+ * status (device int32[2], may be NULL): [0] pages the pool was short of -- then the call changed
+ * nothing --, [1] entries that were refused and skipped.  Entries refused: sequence numbers
+ * outside [0, num_seqs); a number that an earlier entry of the call named (children in fork,
+ * sequences in free and extend); a fork into a row that is not empty or is its own parent; growth
+ * beyond max_pages.
+ * No counterpart in the reference's path, which keeps one request (its serving stack's token
+ * slots are managed on the host, common/mem_manager.py).
+ */
+typedef struct okv_page_pool {
+  int32_t* table; /* (num_seqs, max_pages), rows table_stride entries apart */
+  int32_t* lens;  /* (num_seqs) tokens */
+  int32_t* refs;  /* (num_pages) */
+  int64_t table_stride;
+  int32_t num_seqs, max_pages, num_pages, page_size;
+} okv_page_pool_t;
+
+typedef struct okv_page_buffer {
+  void* base;
+  int64_t page_bytes;
+} okv_page_buffer_t;
+
+/* Sequences seqs[0..n) give their pages back: counts drop by one, rows become -1, lengths 0. */
+int okv_pages_free(const okv_page_pool_t* pool, const int32_t* seqs, int32_t n, int32_t* status,
+                   okv_stream_t stream);
+
+/* Sequence children[i] becomes a continuation of parents[i]: it names the parent's full pages
+ * (counted once more) and gets a copy of a partly filled last one, so both may grow on their own.
+ * All parents are read as they were before the call.  ws: okv_pages_workspace_bytes(pool, n). */
+int okv_pages_fork(const okv_page_pool_t* pool, const int32_t* parents, const int32_t* children, int32_t n,
+                   const okv_page_buffer_t* host_buffers, int32_t num_buffers, int32_t* status, void* ws,
+                   size_t ws_bytes, okv_stream_t stream);
+
+/* Room for more[i] more tokens (negative: none) in sequence seqs[i]: its length grows by it and the pages it
+ * lacks are taken from the free ones. */
+int okv_pages_extend(const okv_page_pool_t* pool, const int32_t* seqs, const int32_t* more, int32_t n,
+                     int32_t* status, void* ws, size_t ws_bytes, okv_stream_t stream);
+
+/* Pages dst[i] = pages src[i] of every buffer, i < count[0] (device) or n when count is NULL.
+ * No page may be both a source and a destination, and the destinations are distinct; page numbers
+ * outside [0, num_pages) are skipped. */
+int okv_pages_copy(const okv_page_buffer_t* host_buffers, int32_t num_buffers, int32_t num_pages,
+                   const int32_t* src, const int32_t* dst, const int32_t* count, int32_t n,
+                   okv_stream_t stream);
+
+/* The pool's U used pages become pages 0 .. U-1: those at or above U move, in order, to the free
+ * ones below.  table_out / refs_out may be the pool's own arrays; used_out (device int32, may be
+ * NULL) receives U. */
+int okv_pages_compact(const okv_page_pool_t* pool, int32_t* table_out, int64_t table_out_stride,
+                      int32_t* refs_out, int32_t* used_out, const okv_page_buffer_t* host_buffers,
+                      int32_t num_buffers, void* ws, size_t ws_bytes, okv_stream_t stream);
+int okv_pages_workspace_bytes(const okv_page_pool_t* pool, int32_t n, size_t* out_bytes);
 
 #ifdef __cplusplus
 }

@@ -15,6 +15,7 @@ DIAG_LIB_PATH = os.path.join(_PKG, "libomnikv_hip_diag.so")  # measurement build
 STAMPS_LIB_PATH = os.path.join(_PKG, "libomnikv_hip_stamps.so")  # timeline build (csrc/build.py --stamps): + device timestamps
 
 OKV_F32, OKV_BF16, OKV_F16 = 0, 1, 2
+OKV_E4M3, OKV_I8 = 3, 4  # code formats of an 8-bit cache
 OKV_REDUCE_MAX, OKV_REDUCE_SUM = 0, 1
 OKV_NORM_RAW, OKV_NORM_SOFTMAX = 0, 1
 OKV_OP_SCORE, OKV_OP_TOPK, OKV_OP_DENSE_ATTN, OKV_OP_SPARSE_ATTN, OKV_OP_SCORE_WINDOW = 0, 1, 2, 3, 4
@@ -43,6 +44,17 @@ EXPORTS = (
     "okv_rope",
     "okv_rope_append",
     "okv_silu_mul",
+    "okv_kv8_append",
+    "okv_kv8_read",
+    "okv_kv8_workspace_bytes",
+    "okv_kv8_dense_attn",
+    "okv_kv8_sparse_attn",
+    "okv_pages_free",
+    "okv_pages_fork",
+    "okv_pages_extend",
+    "okv_pages_copy",
+    "okv_pages_compact",
+    "okv_pages_workspace_bytes",
 )
 
 
@@ -76,6 +88,55 @@ class Shape(C.Structure):
         ("max_tail_len", C.c_int32),
         ("with_scores", C.c_int32),
     ]
+
+
+class KV8Cache(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p),
+        ("v_codes", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("format", C.c_int32),
+        ("dtype", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("block_tokens", C.c_int32),
+        ("capacity", C.c_int32),
+        ("token_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("batch_stride", C.c_int64),
+        ("scale_block_stride", C.c_int64),
+        ("scale_head_stride", C.c_int64),
+        ("scale_batch_stride", C.c_int64),
+        ("page_table", C.c_void_p),
+        ("page_size", C.c_int32),
+        ("page_table_stride", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("page_stride", C.c_int64),
+        ("scale_page_stride", C.c_int64),
+        ("open_k", C.c_void_p),
+        ("open_v", C.c_void_p),
+        ("open_token_stride", C.c_int64),
+        ("open_head_stride", C.c_int64),
+        ("open_batch_stride", C.c_int64),
+    ]
+
+
+class PagePool(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("refs", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("num_seqs", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("page_size", C.c_int32),
+    ]
+
+
+class PageBuffer(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("page_bytes", C.c_int64)]
 
 
 _lib = None
@@ -140,6 +201,23 @@ def _declare(l):
                                   vp, i64, vp]
     l.okv_silu_mul.restype = C.c_int
     l.okv_silu_mul.argtypes = [vp, vp, i64, i32, vp, vp]
+    cache, pool, bufs = C.POINTER(KV8Cache), C.POINTER(PagePool), C.POINTER(PageBuffer)
+    for name, args in (
+        ("okv_kv8_append", [cache, vp, vp, i64, i64, i64, vp, i32, vp, i32, i32, i32, vp]),
+        ("okv_kv8_read", [cache, vp, i64, i32, vp, i32, i32, vp, vp, i64, i64, i64, vp]),
+        ("okv_kv8_workspace_bytes", [i32, i32, i32, i32, i32, C.POINTER(sz)]),
+        ("okv_kv8_dense_attn", [vp, i32, cache, vp, i32, i32, f32, vp, vp, i32, i32, i32, vp, i64, vp, sz, vp]),
+        ("okv_kv8_sparse_attn", [vp, i32, cache, vp, i64, i32, vp, i32, vp, vp, i64, i64, i64, vp, i32, i32, f32, vp, vp, sz,
+                                 vp]),
+        ("okv_pages_free", [pool, vp, i32, vp, vp]),
+        ("okv_pages_fork", [pool, vp, vp, i32, bufs, i32, vp, vp, sz, vp]),
+        ("okv_pages_extend", [pool, vp, vp, i32, vp, vp, sz, vp]),
+        ("okv_pages_copy", [bufs, i32, i32, vp, vp, vp, i32, vp]),
+        ("okv_pages_compact", [pool, vp, i64, vp, vp, bufs, i32, vp, sz, vp]),
+        ("okv_pages_workspace_bytes", [pool, i32, C.POINTER(sz)]),
+    ):
+        getattr(l, name).restype = C.c_int
+        getattr(l, name).argtypes = args
     l.okv_offload_stage.restype = C.c_int
     l.okv_offload_stage.argtypes = [vp, i64, vp, i32, vp, i32, vp, vp, vp]
 

@@ -14,6 +14,7 @@ Usage: python omnikv_amd/csrc/build.py [--no-diag] [--stamps]
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -21,23 +22,20 @@ OUT = os.path.join(PKG, "libomnikv_hip.so")
 OUT_DIAG = os.path.join(PKG, "libomnikv_hip_diag.so")
 OUT_STAMPS = os.path.join(PKG, "libomnikv_hip_stamps.so")
 SOURCES = ["okv_api.hip", "okv_attn.hip", "okv_attn_mfma.hip", "okv_topk.hip", "okv_topk_mb.hip", "okv_gather.hip",
-           "okv_window.hip", "okv_layer.hip"]
+           "okv_window.hip", "okv_layer.hip", "okv_kv8_append.hip", "okv_kv8_attn.hip", "okv_pages.hip"]
 DIAG_SOURCES = SOURCES + ["okv_diag.hip"]
 FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wno-unused-command-line-argument",
     "-pthread",
 ]
 
 
-def _compile(sources, out, extra, verbose):
-    srcs = [os.path.join(HERE, s) for s in sources]
-    cmd = ["hipcc"] + FLAGS + extra + srcs + ["-o", out]
+def _run(cmd, verbose):
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
@@ -47,6 +45,19 @@ def _compile(sources, out, extra, verbose):
         print(text)
     if res.returncode != 0:
         raise RuntimeError("hipcc failed:\n" + text)
+
+
+def _compile(sources, out, extra, verbose):
+    """One object per source, side by side, then one link."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, s + ".o") for s in sources]
+        with ThreadPoolExecutor(max_workers=4) as pool:
+            for f in [pool.submit(_run, ["hipcc"] + FLAGS + extra + ["-c", os.path.join(HERE, s), "-o", o], verbose)
+                      for s, o in zip(sources, objs)]:
+                f.result()
+        _run(["hipcc"] + FLAGS + ["-shared"] + objs + ["-o", out], verbose)
     return out
 
 
@@ -64,7 +75,7 @@ def build(force: bool = True, verbose: bool = True, diag: bool = True) -> str:
     if diag:
         jobs.append((DIAG_SOURCES, OUT_DIAG, ["-DOKV_DIAG"]))
     if not force:
-        headers = [os.path.join(HERE, h) for h in ("okv_internal.h", "okv_device.h")]
+        headers = [os.path.join(HERE, h) for h in ("okv_internal.h", "okv_device.h", "okv_kv8.h")]
         jobs = [j for j in jobs if not os.path.exists(j[1]) or os.path.getmtime(j[1]) < max(
             os.path.getmtime(p) for p in [os.path.join(HERE, s) for s in j[0]] + headers)]
     with ThreadPoolExecutor(max_workers=2) as pool:

@@ -1,0 +1,253 @@
+// Writing (okv_kv8_append) and reading back (okv_kv8_read) rows of the 8-bit K/V cache.
+#include <math.h>
+
+#include "okv_kv8.h"
+
+namespace okv {
+
+int kv8_validate(const okv_kv8_cache_t* c, const char* what) {
+  OKV_REQUIRE(c != nullptr, OKV_ERR_INVALID, "%s: cache is NULL", what);
+  OKV_REQUIRE(c->k_codes && c->v_codes && c->k_scale && c->v_scale, OKV_ERR_INVALID, "%s: NULL codes or scales", what);
+  OKV_REQUIRE(c->format == OKV_E4M3 || c->format == OKV_I8, OKV_ERR_UNSUPPORTED,
+              "%s: code format %d (OKV_E4M3 and OKV_I8 are)", what, c->format);
+  OKV_REQUIRE(c->dtype == OKV_BF16 || c->dtype == OKV_F16, OKV_ERR_UNSUPPORTED,
+              "%s: dtype %d next to an 8-bit cache (OKV_BF16 and OKV_F16 are)", what, c->dtype);
+  OKV_REQUIRE(c->head_dim == kD, OKV_ERR_UNSUPPORTED, "%s: head_dim %d not supported (kernels are built for 128)", what,
+              c->head_dim);
+  OKV_REQUIRE(c->num_kv_heads >= 1, OKV_ERR_INVALID, "%s: num_kv_heads %d", what, c->num_kv_heads);
+  const int bt = c->block_tokens;
+  OKV_REQUIRE(bt == 16 || bt == 32 || bt == 64 || bt == 128, OKV_ERR_UNSUPPORTED, "%s: block_tokens %d (16, 32, 64, 128)",
+              what, bt);
+  OKV_REQUIRE(((uintptr_t)c->k_codes & 15) == 0 && ((uintptr_t)c->v_codes & 15) == 0, OKV_ERR_INVALID,
+              "%s: code pointers must be 16-byte aligned", what);
+  OKV_REQUIRE(((uintptr_t)c->k_scale & 3) == 0 && ((uintptr_t)c->v_scale & 3) == 0, OKV_ERR_INVALID,
+              "%s: scale pointers must be 4-byte aligned", what);
+  OKV_REQUIRE(c->token_stride % 16 == 0 && c->head_stride % 16 == 0 && c->batch_stride % 16 == 0 && c->page_stride % 16 == 0,
+              OKV_ERR_INVALID, "%s: code strides must be multiples of 16 bytes", what);
+  OKV_REQUIRE(c->token_stride >= 0 && c->token_stride < (1ll << 31), OKV_ERR_UNSUPPORTED, "%s: token stride %lld", what,
+              (long long)c->token_stride);
+  if (c->page_table) {
+    OKV_REQUIRE(c->page_size >= bt && c->page_size % bt == 0, OKV_ERR_INVALID,
+                "%s: page_size %d is not a multiple of block_tokens %d", what, c->page_size, bt);
+    OKV_REQUIRE(c->page_table_stride >= 1 && c->num_pages >= 1, OKV_ERR_INVALID, "%s: page_table_stride %d, num_pages %d",
+                what, c->page_table_stride, c->num_pages);
+  } else {
+    OKV_REQUIRE(c->capacity >= bt && c->capacity % bt == 0, OKV_ERR_INVALID,
+                "%s: capacity %d is not a multiple of block_tokens %d", what, c->capacity, bt);
+  }
+  OKV_REQUIRE((c->open_k == nullptr) == (c->open_v == nullptr), OKV_ERR_INVALID, "%s: one of open_k / open_v is NULL", what);
+  if (c->open_k)
+    OKV_REQUIRE(((uintptr_t)c->open_k & 15) == 0 && ((uintptr_t)c->open_v & 15) == 0 && c->open_token_stride % 8 == 0 &&
+                    c->open_head_stride % 8 == 0 && c->open_batch_stride % 8 == 0,
+                OKV_ERR_INVALID, "%s: open buffers: 16-byte aligned, strides multiples of 8 elements", what);
+  return OKV_OK;
+}
+
+struct AppendArgs {
+  okv_kv8_cache_t c;
+  const void* rows[2];  // new K, new V
+  int64_t token_stride, head_stride, batch_stride;
+  const int32_t* starts;
+  const int32_t* new_lens;
+  int32_t start, max_new, close;
+};
+
+// One workgroup per (touched block, kv head, request, K or V): 16 lanes hold a row (eight elements each), sixteen
+// rows per trip, the whole block in registers between the two passes (maximum, then codes).
+// The workgroup of the first touched block also moves the rows of the block that stays open: it has read the old
+// open rows by then, and nobody else touches the request's open buffer.
+template <typename T, typename F>
+__global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
+  __shared__ float s_max[4];
+  const okv_kv8_cache_t& c = a.c;
+  const int B = c.block_tokens;
+  const int g = blockIdx.y, b = blockIdx.z >> 1, is_v = blockIdx.z & 1;
+  const int start = a.starts ? a.starts[b] : a.start;
+  int n = a.new_lens ? a.new_lens[b] : a.max_new;
+  n = n < 0 ? 0 : n > a.max_new ? a.max_new : n;
+  if (n == 0 || start < 0 || (int64_t)start + n > kv8_room(c)) return;
+  const int end = start + n;
+  const int first = start / B, blk = first + blockIdx.x;
+  if (blk * B >= end) return;
+  const T* src = reinterpret_cast<const T*>(a.rows[is_v]) + (int64_t)b * a.batch_stride + (int64_t)g * a.head_stride;
+  T* open = reinterpret_cast<T*>(is_v ? c.open_v : c.open_k);
+  if (open) open += (int64_t)b * c.open_batch_stride + (int64_t)g * c.open_head_stride;
+  const int tid = threadIdx.x, col = tid & 15, row = tid >> 4;
+  const bool whole = (blk + 1) * B <= end || a.close;  // this block becomes codes
+  if (whole) {
+    constexpr int P = kMaxBlockTokens / 16;
+    uint4 x[P];
+    float amax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int r = 16 * p + row, t = blk * B + r;
+      x[p] = make_uint4(0, 0, 0, 0);
+      if (r < B && t < end) {
+        const T* q = t >= start ? src + (int64_t)(t - start) * a.token_stride : open + (int64_t)r * c.open_token_stride;
+        x[p] = *reinterpret_cast<const uint4*>(q + 8 * col);
+      }
+      float v[8];
+      cvt8((const T*)nullptr, x[p], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        amax = fmaxf(amax, fabsf(v[i]));
+        bad = bad || !(fabsf(v[i]) < INFINITY);
+      }
+    }
+    if (bad) amax = INFINITY;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    if ((tid & 63) == 0) s_max[tid >> 6] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const bool poison = amax == INFINITY;
+    const float scale = poison ? NAN : fmaxf(amax / qmax_of(F{}), kMinScale);
+    const float inv = poison ? 0.f : 1.f / scale;
+    int64_t ro, so;
+    if (kv8_locate(c, b, blk * B, &ro, &so)) {
+      uint8_t* dst = reinterpret_cast<uint8_t*>(is_v ? c.v_codes : c.k_codes) + ro + (int64_t)g * c.head_stride;
+      if (tid == 0) (is_v ? c.v_scale : c.k_scale)[so + (int64_t)g * c.scale_head_stride] = scale;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int r = 16 * p + row;
+        if (r >= B || blk * B + r >= end) continue;
+        float v[8];
+        cvt8((const T*)nullptr, x[p], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] *= inv;
+          v[i] = poison ? 0.f : fminf(fmaxf(v[i], -qmax_of(F{})), qmax_of(F{}));
+        }
+        *reinterpret_cast<uint2*>(dst + (int64_t)r * c.token_stride + 8 * col) =
+            make_uint2(encode4(F{}, v), encode4(F{}, v + 4));
+      }
+    }
+  }
+  if (blockIdx.x != 0 || a.close || end % B == 0) return;
+  // rows of the last block, which stays open; the old open rows have been read
+  __syncthreads();
+  const int lo = max(start, end / B * B);
+  for (int t = lo + row; t < end; t += 16)
+    *reinterpret_cast<uint4*>(open + (int64_t)(t % B) * c.open_token_stride + 8 * col) =
+        *reinterpret_cast<const uint4*>(src + (int64_t)(t - start) * a.token_stride + 8 * col);
+}
+
+struct ReadArgs {
+  okv_kv8_cache_t c;
+  const int32_t* idx;
+  int64_t idx_stride;
+  const int32_t* seq_lens;
+  int32_t max_seq_len, max_rows;
+  void* out[2];
+  int64_t token_stride, head_stride, batch_stride;
+};
+
+template <typename T, typename F>
+__global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
+  const okv_kv8_cache_t& c = a.c;
+  const int g = blockIdx.y, b = blockIdx.z >> 1, is_v = blockIdx.z & 1;
+  const int col = threadIdx.x & 15, j = blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (j >= a.max_rows) return;
+  const int64_t room = kv8_room(c);
+  int64_t len = a.seq_lens ? a.seq_lens[b] : a.max_seq_len;
+  len = len < 0 ? 0 : len > a.max_seq_len ? a.max_seq_len : len;
+  const int64_t closed = c.open_k ? len / c.block_tokens * c.block_tokens : len;
+  const int t = a.idx ? a.idx[(int64_t)b * a.idx_stride + j] : j;
+  T* dst = reinterpret_cast<T*>(a.out[is_v]) + (int64_t)b * a.batch_stride + (int64_t)j * a.token_stride +
+           (int64_t)g * a.head_stride + 8 * col;
+  if (t >= closed && t < len) {
+    const T* open = reinterpret_cast<const T*>(is_v ? c.open_v : c.open_k) + (int64_t)b * c.open_batch_stride +
+                    (int64_t)g * c.open_head_stride + (int64_t)(t % c.block_tokens) * c.open_token_stride;
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(open + 8 * col);
+    return;
+  }
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  int64_t ro, so;
+  if (t >= 0 && t < len && t < room && kv8_locate(c, b, t, &ro, &so)) {
+    const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(is_v ? c.v_codes : c.k_codes) + ro +
+                                                    (int64_t)g * c.head_stride + 8 * col);
+    const float s = (is_v ? c.v_scale : c.k_scale)[so + (int64_t)g * c.scale_head_stride];
+    decode4(F{}, x.x, v);
+    decode4(F{}, x.y, v + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= s;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) store1(dst + i, v[i]);
+}
+
+template <typename A>
+static bool wide_rows(const A& a) {
+  return a.token_stride % 8 == 0 && a.head_stride % 8 == 0 && a.batch_stride % 8 == 0;
+}
+
+}  // namespace okv
+
+using namespace okv;
+
+#define OKV_KV8_DISPATCH(c, KERNEL, grid, args)                                                               \
+  do {                                                                                                        \
+    if ((c)->dtype == OKV_BF16) {                                                                             \
+      if ((c)->format == OKV_E4M3) hipLaunchKernelGGL((KERNEL<BF16, E4M3>), grid, dim3(256), 0, (hipStream_t)stream, args); \
+      else hipLaunchKernelGGL((KERNEL<BF16, I8>), grid, dim3(256), 0, (hipStream_t)stream, args);             \
+    } else {                                                                                                  \
+      if ((c)->format == OKV_E4M3) hipLaunchKernelGGL((KERNEL<F16, E4M3>), grid, dim3(256), 0, (hipStream_t)stream, args); \
+      else hipLaunchKernelGGL((KERNEL<F16, I8>), grid, dim3(256), 0, (hipStream_t)stream, args);              \
+    }                                                                                                         \
+  } while (0)
+
+extern "C" {
+
+int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, const void* new_v, int64_t new_token_stride,
+                   int64_t new_head_stride, int64_t new_batch_stride, const int32_t* starts, int32_t start,
+                   const int32_t* new_lens, int32_t max_new, int32_t close, int32_t batch, okv_stream_t stream) {
+  int rc = kv8_validate(cache, "okv_kv8_append");
+  if (rc) return rc;
+  const int B = cache->block_tokens;
+  OKV_REQUIRE(new_k && new_v, OKV_ERR_INVALID, "new_k or new_v is NULL");
+  OKV_REQUIRE(batch >= 1 && max_new >= 0, OKV_ERR_INVALID, "bad batch or length");
+  AppendArgs a{*cache, {new_k, new_v}, new_token_stride, new_head_stride, new_batch_stride, starts, new_lens, start, max_new,
+               close ? 1 : 0};
+  OKV_REQUIRE(((uintptr_t)new_k & 15) == 0 && ((uintptr_t)new_v & 15) == 0 && wide_rows(a), OKV_ERR_INVALID,
+              "new rows: 16-byte aligned, strides multiples of 8 elements");
+  if (!starts)
+    OKV_REQUIRE(start >= 0 && (new_lens || (int64_t)start + max_new <= kv8_room(*cache)), OKV_ERR_INVALID,
+                "rows [%d, %lld) do not fit the cache's %lld tokens", start, (long long)start + max_new,
+                (long long)kv8_room(*cache));
+  if (close || !cache->open_k)
+    OKV_REQUIRE(!starts && start % B == 0, OKV_ERR_INVALID,
+                "closing the last block, and a cache without open buffers, need a start at a block's border, known to the host");
+  if (!cache->open_k && !close)
+    OKV_REQUIRE(!new_lens && max_new % B == 0, OKV_ERR_INVALID,
+                "without open buffers an append ends at a block's border or closes the last block");
+  if (max_new == 0) return OKV_OK;
+  // a start the device knows may lie anywhere in its block
+  const int64_t blocks = starts ? ((int64_t)max_new + 2 * B - 2) / B : ((int64_t)start % B + max_new + B - 1) / B;
+  OKV_REQUIRE(cache->num_kv_heads <= 65535 && batch <= 32767, OKV_ERR_UNSUPPORTED, "too many heads or requests");
+  OKV_KV8_DISPATCH(cache, kv8_append_kernel, dim3((uint32_t)blocks, cache->num_kv_heads, 2 * batch), a);
+  OKV_HIP_CHECK(hipGetLastError());
+  return OKV_OK;
+}
+
+int okv_kv8_read(const okv_kv8_cache_t* cache, const int32_t* idx, int64_t idx_stride, int32_t max_rows,
+                 const int32_t* seq_lens, int32_t max_seq_len, int32_t batch, void* k_out, void* v_out,
+                 int64_t out_token_stride, int64_t out_head_stride, int64_t out_batch_stride, okv_stream_t stream) {
+  int rc = kv8_validate(cache, "okv_kv8_read");
+  if (rc) return rc;
+  OKV_REQUIRE(k_out && v_out, OKV_ERR_INVALID, "k_out or v_out is NULL");
+  OKV_REQUIRE(batch >= 1 && max_rows >= 0 && max_seq_len >= 0 && max_seq_len <= kv8_room(*cache), OKV_ERR_INVALID,
+              "bad batch or length");
+  if (idx) OKV_REQUIRE(idx_stride >= max_rows, OKV_ERR_INVALID, "idx_stride < max_rows");
+  ReadArgs a{*cache, idx, idx_stride, seq_lens, max_seq_len, max_rows, {k_out, v_out}, out_token_stride, out_head_stride,
+             out_batch_stride};
+  OKV_REQUIRE(((uintptr_t)k_out & 15) == 0 && ((uintptr_t)v_out & 15) == 0 && wide_rows(a), OKV_ERR_INVALID,
+              "outputs: 16-byte aligned, strides multiples of 8 elements");
+  if (max_rows == 0) return OKV_OK;
+  OKV_REQUIRE(cache->num_kv_heads <= 65535 && batch <= 32767, OKV_ERR_UNSUPPORTED, "too many heads or requests");
+  OKV_KV8_DISPATCH(cache, kv8_read_kernel, dim3((max_rows + 15) / 16, cache->num_kv_heads, 2 * batch), a);
+  OKV_HIP_CHECK(hipGetLastError());
+  return OKV_OK;
+}
+
+}  // extern "C"

@@ -8,10 +8,12 @@ token-major store are read in place.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import functools
 import math
 from dataclasses import dataclass
-from typing import Dict, Optional, Tuple
+from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -499,3 +501,413 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     out = torch.empty_like(gate)
     check(lib().okv_silu_mul(gate.data_ptr(), up.data_ptr(), gate.numel(), dt, out.data_ptr(), _stream_ptr(gate.device)))
     return out
+
+
+# ---------------------------------------------------------------- 8-bit K/V cache
+KV8_FORMATS = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+_KV8_CODES = {torch.float8_e4m3fn: _lib.OKV_E4M3, torch.int8: _lib.OKV_I8}
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device's context when it is not the current one: a launch goes to the current device."""
+    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _scratch(device, nbytes: int) -> torch.Tensor:
+    """Scratch of one call, from torch's allocator: it may be reused by what the same stream runs next, and a
+    captured graph keeps a piece of its own pool, so two graphs never share one."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _dev_i32(t: Optional[torch.Tensor], n: int, device, name: str):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.device != device or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on {device}")
+    return t.data_ptr()
+
+
+class KV8:
+    """An 8-bit K/V cache: codes (torch.float8_e4m3fn or torch.int8) with one fp32 scale per `block` tokens and kv
+    head (include/omnikv_hip.h, okv_kv8_cache_t, has the format).
+
+    contiguous: k, v (bsz, Hkv, capacity, 128), scales (bsz, Hkv, capacity / block)
+    paged:      k, v (pages, page_size, Hkv, 128), scales (pages, page_size / block, Hkv), page_table (bsz, max_pages) int32
+    open_k, open_v (bsz, Hkv, block, 128), bfloat16 or float16: the rows of each request's last, not yet full block; without them the
+    cache is closed (it takes no more rows).  K and V share strides, and so do the two scales.  The
+    handle keeps the tensors; the lengths are the caller's."""
+
+    def __init__(self, k, v, k_scale, v_scale, block: int, open_k=None, open_v=None,
+                 page_table: Optional[torch.Tensor] = None):
+        paged = page_table is not None
+        if k.dtype not in _KV8_CODES or v.dtype != k.dtype:
+            raise ValueError("codes must be torch.float8_e4m3fn or torch.int8, K and V alike")
+        if k.dim() != 4 or k.shape[-1] != 128 or k.stride(-1) != 1 or v.shape != k.shape or v.stride() != k.stride():
+            raise ValueError("K and V codes must be 4-d with 128 contiguous elements last, same shape and strides")
+        if any(s % 16 for s in k.stride()[:3]):
+            raise ValueError("code strides must be multiples of 16")
+        if block not in (16, 32, 64, 128):
+            raise ValueError("block must be 16, 32, 64 or 128 tokens")
+        tokens = k.shape[1] if paged else k.shape[2]
+        hkv = k.shape[2] if paged else k.shape[1]
+        if tokens < block or tokens % block:
+            raise ValueError(f"{'page_size' if paged else 'capacity'} must be a multiple of block")
+        want = (k.shape[0], tokens // block, hkv) if paged else (k.shape[0], hkv, tokens // block)
+        for s in (k_scale, v_scale):
+            if tuple(s.shape) != want or s.dtype != torch.float32 or s.stride() != k_scale.stride():
+                raise ValueError(f"scales must be float32 {want}, same strides for K and V")
+        devices = {t.device for t in (k, v, k_scale, v_scale, open_k, open_v, page_table) if t is not None}
+        if len(devices) != 1 or not k.is_cuda:
+            raise ValueError("every tensor of the cache must be on one GPU (the HIP path has no CPU fallback)")
+        self.bsz = page_table.shape[0] if paged else k.shape[0]
+        if paged and (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1):
+            raise ValueError("page_table must be (bsz, max_pages) int32, rows contiguous")
+        if (open_k is None) != (open_v is None):
+            raise ValueError("open_k and open_v go together")
+        if open_k is not None:
+            if (tuple(open_k.shape) != (self.bsz, hkv, block, 128) or open_k.dtype not in (torch.bfloat16, torch.float16)
+                    or open_v.shape != open_k.shape or open_v.dtype != open_k.dtype or open_v.stride() != open_k.stride()
+                    or open_k.stride(-1) != 1 or any(s % 8 for s in open_k.stride()[:3])):
+                raise ValueError(f"open_k / open_v must be ({self.bsz}, {hkv}, {block}, 128) in bfloat16 or float16, "
+                                 "same strides (multiples of 8), contiguous last dimension")
+        self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
+        self.open_k, self.open_v, self.page_table = open_k, open_v, page_table
+        self.device, self.num_kv_heads = k.device, hkv
+        self.page_size = tokens if paged else 0
+        self.capacity = page_table.shape[1] * tokens if paged else tokens  # tokens a request has room for
+        self.dtype = open_k.dtype if open_k is not None else None
+        st, ss = k.stride(), k_scale.stride()
+        self._c = {}
+        for dt in (torch.bfloat16, torch.float16):
+            if self.dtype not in (None, dt):
+                continue
+            c = _lib.KV8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _KV8_CODES[k.dtype],
+                              _DTYPES[dt], hkv, 128, block, 0 if paged else tokens)
+            if paged:
+                c.token_stride, c.head_stride, c.page_stride = st[1], st[2], st[0]
+                c.scale_block_stride, c.scale_head_stride, c.scale_page_stride = ss[1], ss[2], ss[0]
+                c.page_table, c.page_size = page_table.data_ptr(), tokens
+                c.page_table_stride, c.num_pages = page_table.shape[1], k.shape[0]
+                if self.bsz > 1 and page_table.stride(0) != page_table.shape[1]:
+                    raise ValueError("page_table rows must lie back to back")
+            else:
+                c.batch_stride, c.head_stride, c.token_stride = st[:3]
+                c.scale_batch_stride, c.scale_head_stride, c.scale_block_stride = ss
+            if open_k is not None:
+                c.open_k, c.open_v = open_k.data_ptr(), open_v.data_ptr()
+                c.open_batch_stride, c.open_head_stride, c.open_token_stride = open_k.stride()[:3]
+            self._c[dt] = c
+
+    @classmethod
+    def empty(cls, bsz: int, num_kv_heads: int, capacity: int, fmt: str = "e4m3", block: int = 64,
+              dtype: Optional[torch.dtype] = torch.bfloat16, device="cuda") -> "KV8":
+        """A contiguous cache with room for `capacity` tokens per request (rounded up to whole blocks); dtype None: closed."""
+        cap = -(-capacity // block) * block
+        k, v = (torch.zeros((bsz, num_kv_heads, cap, 128), dtype=torch.uint8, device=device).view(KV8_FORMATS[fmt])
+                for _ in "kv")
+        s = torch.zeros((2, bsz, num_kv_heads, cap // block), dtype=torch.float32, device=device)
+        o = [None, None] if dtype is None else torch.zeros((2, bsz, num_kv_heads, block, 128), dtype=dtype, device=device)
+        return cls(k, v, s[0], s[1], block, o[0], o[1])
+
+    @classmethod
+    def empty_paged(cls, page_table: torch.Tensor, num_pages: int, page_size: int, num_kv_heads: int, fmt: str = "e4m3",
+                    block: int = 16, dtype: Optional[torch.dtype] = torch.bfloat16) -> "KV8":
+        """A pool of `num_pages` pages read and written through `page_table` (bsz, max_pages); dtype None: closed."""
+        dev = page_table.device
+        k, v = (torch.zeros((num_pages, page_size, num_kv_heads, 128), dtype=torch.uint8, device=dev).view(KV8_FORMATS[fmt])
+                for _ in "kv")
+        s = torch.zeros((2, num_pages, page_size // block, num_kv_heads), dtype=torch.float32, device=dev)
+        o = [None, None] if dtype is None else torch.zeros((2, page_table.shape[0], num_kv_heads, block, 128), dtype=dtype,
+                                                           device=dev)
+        return cls(k, v, s[0], s[1], block, o[0], o[1], page_table)
+
+    def slot_index(self, idx: torch.Tensor) -> torch.Tensor:
+        """Token positions (bsz, k) int32 -> rows of the pool seen as one array of token slots, as
+        PagedKV.slot_index; positions and pages outside the request's table stay out (-1)."""
+        if self.page_table is None:
+            raise ValueError("slots address a paged pool")
+        t = idx.clamp(min=0, max=self.capacity - 1).to(torch.int64)
+        page = self.page_table.gather(1, t // self.page_size).to(torch.int64)
+        slots = page * self.page_size + t % self.page_size
+        ok = (idx >= 0) & (idx < self.capacity) & (page >= 0) & (page < self.k.shape[0])
+        return torch.where(ok, slots.to(torch.int32), -1)
+
+    def _struct(self, dtype: torch.dtype):
+        c = self._c.get(dtype)
+        if c is None:
+            raise ValueError(f"{dtype} next to this cache: it takes " + " and ".join(str(d) for d in self._c))
+        return c
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv8_workspace_bytes(device_index: int, batch: int, hq: int, hkv: int, rows: int, score_len: int) -> int:
+    out = C.c_size_t(0)
+    check(lib().okv_kv8_workspace_bytes(batch, hq, hkv, rows, score_len, C.byref(out)))
+    return out.value
+
+
+def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor] = 0,
+               new_lens: Optional[torch.Tensor] = None, close: bool = False) -> None:
+    """Appends k, v (bsz, Hkv, n, 128; any strides, contiguous last dimension) behind the first `start` rows of each
+    request: an int, or an int32 GPU tensor (bsz,) of the requests' lengths.  new_lens (bsz,) int32: rows per request,
+    at most n.  Blocks that fill become codes, the other rows wait in the open buffers; close=True quantises a
+    short last block as well (start then an int at a block's border).  A request whose rows would not
+    fit is left as it was.  okv_kv8_append."""
+    c = cache._struct(k.dtype)
+    if k.dim() != 4 or k.shape[0] != cache.bsz or k.shape[1] != cache.num_kv_heads or k.shape[3] != 128:
+        raise ValueError(f"new rows must be ({cache.bsz}, {cache.num_kv_heads}, n, 128)")
+    if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype or k.stride(3) != 1:
+        raise ValueError("new K and V must share shape, strides and dtype, with a contiguous last dimension")
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError("new rows and cache must be on one GPU")
+    n, (sb, sg, st, _) = k.shape[2], k.stride()
+    if n == 0:
+        return
+    on_dev = isinstance(start, torch.Tensor)
+    starts = _dev_i32(start, cache.bsz, cache.device, "start") if on_dev else None
+    with _on(cache.device):
+        check(lib().okv_kv8_append(C.byref(c), k.data_ptr(), v.data_ptr(), st, sg, sb, starts, 0 if on_dev else int(start),
+                                   _dev_i32(new_lens, cache.bsz, cache.device, "new_lens"), n, int(close), cache.bsz,
+                                   _stream_ptr(cache.device)))
+
+
+def _kv8_query(q: torch.Tensor, cache: KV8):
+    q = _q3(q)
+    if q.dim() != 3 or q.shape[0] != cache.bsz or q.shape[2] != 128:
+        raise ValueError(f"q must be ({cache.bsz}, Hq, 128) or ({cache.bsz}, Hq, 1, 128)")
+    if q.device != cache.device:
+        raise ValueError("q and cache must be on one GPU")
+    return q, cache._struct(q.dtype)
+
+
+def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, seq_lens: Optional[torch.Tensor] = None,
+                   scale: Optional[float] = None, selector: Optional[str] = None, score_len: Optional[int] = None,
+                   score_lens: Optional[torch.Tensor] = None, scores_out: Optional[torch.Tensor] = None,
+                   select_k: Optional[int] = None, k_per_seg: Optional[torch.Tensor] = None,
+                   idx_out: Optional[torch.Tensor] = None):
+    """dense_attn over an 8-bit cache: q (bsz, Hq, 128) attends to the first seq_len rows (seq_lens: per request, on
+    the GPU) -> (bsz, Hq, 128); with `selector` also the filter layer's scores of the first score_len rows, from the same
+    pass, and with `select_k` the ascending indices of the largest ones, as topk gives them.  A request
+    without rows gets zeros.  okv_kv8_dense_attn."""
+    q, c = _kv8_query(q, cache)
+    hq, hkv, dev, bsz = q.shape[1], cache.num_kv_heads, cache.device, cache.bsz
+    if seq_len is None:
+        seq_len = cache.capacity
+    if select_k is not None and selector is None:
+        raise ValueError("select_k needs a selector")
+    out = torch.empty_like(q)
+    scores, sp, ss, red, norm, slen, sl = None, None, 0, 0, 0, 0, None
+    if selector is not None:
+        norm_s, red_s = SELECTOR_MODES[selector]
+        red, norm = _REDUCE[red_s], _NORM[norm_s]
+        slen = seq_len if score_len is None else score_len
+        scores = scores_out
+        if scores is None:
+            scores = torch.empty((bsz, slen), dtype=torch.float32, device=dev)
+        elif scores.shape != (bsz, slen) or scores.dtype != torch.float32 or scores.stride(1) != 1 or scores.device != dev:
+            raise ValueError("scores_out must be (bsz, score_len) float32 with contiguous rows, on the cache's GPU")
+        sp, ss, sl = scores.data_ptr(), scores.stride(0), _dev_i32(score_lens, bsz, dev, "score_lens")
+    ws = _scratch(dev, _kv8_workspace_bytes(dev.index, bsz, hq, hkv, seq_len, slen))
+    with _on(dev):
+        check(lib().okv_kv8_dense_attn(q.data_ptr(), hq, C.byref(c), _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz,
+                                       scale if scale is not None else 1.0 / math.sqrt(128), out.data_ptr(), sl, slen, red,
+                                       norm, sp, ss, ws.data_ptr(), ws.numel(), _stream_ptr(dev)))
+        if selector is None:
+            return out
+        if select_k is None:
+            return out, scores
+        return out, scores, topk(scores, select_k, score_lens, k_per_seg, out=idx_out)
+
+
+def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = None, sel_len: Optional[int] = None,
+                    sel_lens: Optional[torch.Tensor] = None, tail_k: Optional[torch.Tensor] = None,
+                    tail_v: Optional[torch.Tensor] = None, tail_len: Optional[int] = None,
+                    tail_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """sparse_attn over an 8-bit cache: rows idx (bsz, k) int32 of the codes (None: rows [0, sel_len)) followed by
+    16-bit tail rows (bsz, Hkv, T, 128) in q's dtype; slots: KV8.slot_index(idx) instead of idx.  Entries outside the
+    request's room (padding, -1) take no part; open rows are not reached.  okv_kv8_sparse_attn."""
+    q, c = _kv8_query(q, cache)
+    hq, hkv, dev, bsz = q.shape[1], cache.num_kv_heads, cache.device, cache.bsz
+    if slots is not None:
+        if cache.page_table is None or idx is not None:
+            raise ValueError("slots go with a paged cache and replace idx")
+        idx = slots
+    ip, istride = None, 0
+    if idx is not None:
+        if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != bsz or idx.stride(1) != 1 or idx.device != dev:
+            raise ValueError(f"idx must be a ({bsz}, k) int32 tensor with contiguous rows on the cache's GPU")
+        if sel_len is None:
+            sel_len = idx.shape[1]
+        elif sel_len > idx.shape[1]:
+            raise ValueError("sel_len exceeds idx")
+        ip, istride = idx.data_ptr(), max(idx.stride(0), idx.shape[1])
+        if bsz > 1 and idx.stride(0) < idx.shape[1]:
+            raise ValueError("idx rows must not overlap")
+    elif sel_len is None:
+        sel_len = cache.capacity
+    tkp = tvp = None
+    tts = ths = tbs = 0
+    if tail_k is not None:
+        if (tail_k.dim() != 4 or tail_v is None or tail_k.shape != tail_v.shape or tail_k.stride() != tail_v.stride()
+                or tail_k.stride(-1) != 1 or tail_k.shape[0] != bsz or tail_k.shape[1] != hkv or tail_k.shape[3] != 128):
+            raise ValueError("tail_k / tail_v must be (bsz, Hkv, T, 128), same strides, contiguous last dimension")
+        if tail_k.dtype != q.dtype or tail_v.dtype != q.dtype or tail_k.device != dev or tail_v.device != dev:
+            raise ValueError("tail and q differ in dtype or GPU")
+        if tail_len is None:
+            tail_len = tail_k.shape[2]
+        elif tail_len > tail_k.shape[2]:
+            raise ValueError("tail_len exceeds the tail")
+        tkp, tvp = tail_k.data_ptr(), tail_v.data_ptr()
+        tts, ths, tbs = tail_k.stride(2), tail_k.stride(1), tail_k.stride(0)
+    elif tail_len:
+        raise ValueError("tail_len without a tail")
+    tail_len = tail_len or 0
+    out = torch.empty_like(q)
+    ws = _scratch(dev, _kv8_workspace_bytes(dev.index, bsz, hq, hkv, sel_len + tail_len, 0))
+    with _on(dev):
+        check(lib().okv_kv8_sparse_attn(q.data_ptr(), hq, C.byref(c), ip, istride, int(slots is not None),
+                                        _dev_i32(sel_lens, bsz, dev, "sel_lens"), sel_len, tkp, tvp, tts, ths, tbs,
+                                        _dev_i32(tail_lens, bsz, dev, "tail_lens"), tail_len, bsz,
+                                        scale if scale is not None else 1.0 / math.sqrt(128), out.data_ptr(), ws.data_ptr(),
+                                        ws.numel(), _stream_ptr(dev)))
+    return out
+
+
+def kv8_read(cache: KV8, dtype: torch.dtype, idx: Optional[torch.Tensor] = None, seq_len: Optional[int] = None,
+             seq_lens: Optional[torch.Tensor] = None):
+    """The cached values as 16-bit tensors (bsz, Hkv, n, 128): rows idx (bsz, n) int32, or the first seq_len; rows outside a
+    request (seq_lens, seq_len; default: the whole room) are zeros.  okv_kv8_read."""
+    c, dev, bsz = cache._struct(dtype), cache.device, cache.bsz
+    if seq_len is None:
+        seq_len = cache.capacity
+    n = seq_len
+    if idx is not None:
+        if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != bsz or not idx.is_contiguous() or idx.device != dev:
+            raise ValueError(f"idx must be a contiguous ({bsz}, n) int32 tensor on the cache's GPU")
+        n = idx.shape[1]
+    k, v = (torch.empty((bsz, cache.num_kv_heads, n, 128), dtype=dtype, device=dev) for _ in "kv")
+    sb, sg, st, _ = k.stride()
+    with _on(dev):
+        check(lib().okv_kv8_read(C.byref(c), idx.data_ptr() if idx is not None else None, n, n,
+                                 _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz, k.data_ptr(), v.data_ptr(), st, sg,
+                                 sb, _stream_ptr(dev)))
+    return k, v
+
+
+# ---------------------------------------------------------------- pages of a cache
+class PageBuffers:
+    """The arrays whose pages move together (every layer's K, V and scales): contiguous tensors
+    (num_pages, ...) on one GPU, their page a multiple of 4 bytes.  Listed once, used by every call."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise ValueError("no buffers")
+        self.device, self.num_pages = self.tensors[0].device, self.tensors[0].shape[0]
+        self._c = (_lib.PageBuffer * len(self.tensors))()
+        for t, b in zip(self.tensors, self._c):
+            if not t.is_cuda or t.device != self.device or not t.is_contiguous() or t.shape[0] != self.num_pages:
+                raise ValueError("buffers must be contiguous (num_pages, ...) tensors on one GPU")
+            b.base, b.page_bytes = t.data_ptr(), t.numel() // max(1, self.num_pages) * t.element_size()
+
+    def __len__(self):
+        return len(self.tensors)
+
+
+def _buffers(buffers) -> PageBuffers:
+    return buffers if isinstance(buffers, PageBuffers) else PageBuffers(buffers)
+
+
+def _page_pool(table, lens, refs, page_size):
+    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or not table.is_cuda:
+        raise ValueError("table must be a (num_seqs, max_pages) int32 GPU tensor with contiguous rows")
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError("table rows must not overlap")
+    lp = _dev_i32(lens, table.shape[0], table.device, "lens")
+    rp = _dev_i32(refs, refs.numel(), table.device, "refs")
+    return _lib.PagePool(table.data_ptr(), lp, rp, max(table.stride(0), table.shape[1]), table.shape[0], table.shape[1],
+                         refs.numel(), page_size)
+
+
+def _entries(t, n, device, name):
+    if t.dim() != 1 or t.numel() < 1:
+        raise ValueError(f"{name} must be a list of at least one entry")
+    return _dev_i32(t, t.numel() if n is None else n, device, name)
+
+
+def _pages_scratch(pool, n, device):
+    out = C.c_size_t(0)
+    check(lib().okv_pages_workspace_bytes(C.byref(pool), n, C.byref(out)))
+    return _scratch(device, out.value)
+
+
+def pages_free(table, lens, refs, seqs, page_size: int, status: Optional[torch.Tensor] = None) -> None:
+    """Sequences `seqs` give their pages back, in place: reference counts drop, table rows become -1, lengths 0.  table
+    (num_seqs, max_pages), lens (num_seqs,), refs (num_pages,), seqs (n,): int32 on the GPU; status (2,) int32
+    receives [0, entries outside the table].  okv_pages_free."""
+    dev, pool = table.device, _page_pool(table, lens, refs, page_size)
+    with _on(dev):
+        check(lib().okv_pages_free(C.byref(pool), _entries(seqs, None, dev, "seqs"), seqs.numel(),
+                                   _dev_i32(status, 2, dev, "status"), _stream_ptr(dev)))
+
+
+def pages_fork(table, lens, refs, parents, children, page_size: int, buffers, status: Optional[torch.Tensor] = None) -> None:
+    """Sequence children[i] (empty) becomes a continuation of parents[i], in place: it shares the full pages and gets a copy
+    of a partly filled last one in every buffer (a PageBuffers or a list of tensors; the lowest free pages).  status
+    (2,) int32 receives [pages short, pairs refused]; short of pages, nothing changes.  okv_pages_fork."""
+    dev, pool, bufs = table.device, _page_pool(table, lens, refs, page_size), _buffers(buffers)
+    if bufs.device != dev or bufs.num_pages != refs.numel():
+        raise ValueError("buffers must hold refs.numel() pages on the table's GPU")
+    n = parents.numel()
+    ws = _pages_scratch(pool, n, dev)
+    with _on(dev):
+        check(lib().okv_pages_fork(C.byref(pool), _entries(parents, None, dev, "parents"), _entries(children, n, dev, "children"),
+                                   n, bufs._c, len(bufs), _dev_i32(status, 2, dev, "status"), ws.data_ptr(), ws.numel(),
+                                   _stream_ptr(dev)))
+
+
+def pages_extend(table, lens, refs, seqs, more, page_size: int, status: Optional[torch.Tensor] = None) -> None:
+    """Sequence seqs[i] grows by more[i] tokens, in place: it takes the pages it lacks from the lowest free ones.  status as in
+    pages_fork.  okv_pages_extend."""
+    dev, pool, n = table.device, _page_pool(table, lens, refs, page_size), seqs.numel()
+    ws = _pages_scratch(pool, n, dev)
+    with _on(dev):
+        check(lib().okv_pages_extend(C.byref(pool), _entries(seqs, None, dev, "seqs"), _entries(more, n, dev, "more"), n,
+                                     _dev_i32(status, 2, dev, "status"), ws.data_ptr(), ws.numel(), _stream_ptr(dev)))
+
+
+def pages_copy(buffers, src: torch.Tensor, dst: torch.Tensor, count: Optional[torch.Tensor] = None) -> None:
+    """Pages dst[i] = pages src[i] of every buffer; count (1,) int32 on the GPU: only the first count.  No page may be
+    both a source and a destination, and the destinations are distinct.  okv_pages_copy."""
+    bufs, n = _buffers(buffers), src.numel()
+    dev = bufs.device
+    if n == 0:
+        return
+    with _on(dev):
+        check(lib().okv_pages_copy(bufs._c, len(bufs), bufs.num_pages, _entries(src, None, dev, "src"),
+                                   _entries(dst, n, dev, "dst"), _dev_i32(count, 1, dev, "count"), n, _stream_ptr(dev)))
+
+
+def pages_compact(table, refs, buffers, table_out: Optional[torch.Tensor] = None, refs_out: Optional[torch.Tensor] = None):
+    """Moves the pool's U used pages to pages 0 .. U-1 (those at or above U go to the free ones below, in order) and returns
+    (table, refs, used): the renamed table and counts (new tensors, or table_out / refs_out, which may be the inputs) and
+    U as a (1,) int32 GPU tensor.  okv_pages_compact."""
+    dev, bufs = table.device, _buffers(buffers)
+    pool = _page_pool(table, None, refs, 1)
+    if bufs.device != dev or bufs.num_pages != refs.numel():
+        raise ValueError("buffers must hold refs.numel() pages on the table's GPU")
+    if table_out is None:
+        table_out = torch.empty(table.shape, dtype=torch.int32, device=dev)
+    elif table_out.shape != table.shape or table_out.dtype != torch.int32 or table_out.stride(1) != 1 or table_out.device != dev:
+        raise ValueError("table_out must look like table")
+    if refs_out is None:
+        refs_out = torch.empty_like(refs)
+    used = torch.empty(1, dtype=torch.int32, device=dev)
+    ws = _pages_scratch(pool, 0, dev)
+    with _on(dev):
+        check(lib().okv_pages_compact(C.byref(pool), table_out.data_ptr(), max(table_out.stride(0), table_out.shape[1]),
+                                      _dev_i32(refs_out, refs.numel(), dev, "refs_out"), used.data_ptr(), bufs._c, len(bufs),
+                                      ws.data_ptr(), ws.numel(), _stream_ptr(dev)))
+    return table_out, refs_out, used

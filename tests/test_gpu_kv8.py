@@ -1,0 +1,455 @@
+"""The 8-bit K/V cache on the GPU against plain 64-bit restatements (tests/kv8_reference.py).
+
+Written rows are compared bit for bit: every rounding of the format is fixed.  Attention outputs and scores are held to
+bounds that kv8_reference derives from the inputs (logit_error, output_bound)."""
+import pytest
+import torch
+
+import kv8_reference as ref
+from omnikv_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF = torch.bfloat16, torch.float16
+
+
+def rows(g, *shape, dtype=BF, gain=1.0):
+    x = torch.randn(*shape, 128, generator=g) * gain
+    x[..., ::31] *= 5.0
+    return x.to(dtype)
+
+
+def make(g, fmt, dtype, block, page, lens, hkv, open_rows=True, spare=1):
+    """A cache holding requests of the given lengths, filled by one append, and its exact contents: (cache, [k], [v])
+    with k, v (hkv, len, 128) float64 per request."""
+    bsz, n = len(lens), max(max(lens), 1)
+    k, v = (rows(g, bsz, hkv, n, dtype=dtype) for _ in "kv")
+    cap = (-(-n // block) + spare) * block
+    if page:
+        per = -(-cap // page)
+        table = torch.randperm(bsz * per + 3, generator=g)[: bsz * per].to(torch.int32).view(bsz, per).to(DEV)
+        cache = ops.KV8.empty_paged(table, bsz * per + 3, page, hkv, fmt, block, dtype if open_rows else None)
+    else:
+        cache = ops.KV8.empty(bsz, hkv, cap, fmt, block, dtype if open_rows else None, DEV)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ops.kv8_append(cache, k.to(DEV), v.to(DEV), 0, lens_t, close=not open_rows)
+    return cache, [held(x[:, :m], fmt, block, open_rows) for x, m in zip(k, lens)], \
+        [held(x[:, :m], fmt, block, open_rows) for x, m in zip(v, lens)]
+
+
+def held(x, fmt, block, open_rows):
+    """What the cache holds of rows x (hkv, n, 128): float64 values."""
+    n = x.shape[1]
+    full = n if not open_rows else n // block * block
+    parts = []
+    for lo in range(0, full, block):
+        c, s = ref.quantise(x[:, lo: min(lo + block, full)], fmt)
+        parts.append(c * s.double()[:, None, None])
+    parts.append(x[:, full:].double())
+    return torch.cat(parts, 1)
+
+
+def read_back(cache, request, n, hkv):
+    """codes * scale of the first n rows of a request, straight from its tensors."""
+    out = []
+    for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        codes, scale = codes.cpu().double(), scale.cpu().double()
+        if cache.page_table is not None:
+            pages = cache.page_table[request].cpu().long()
+            c = codes[pages].flatten(0, 1).transpose(0, 1)
+            s = scale[pages].flatten(0, 1).transpose(0, 1)
+        else:
+            c, s = codes[request], scale[request]
+        out.append((c * s.repeat_interleave(cache.block, 1)[..., None])[:, :n])
+    return out
+
+
+# ------------------------------------------------------------------------------------------ append, read
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("block, page", [(16, 0), (64, 0), (128, 0), (16, 48), (32, 32), (64, 128)])
+def test_append_in_pieces_equals_one_append(fmt, dtype, block, page):
+    """A prompt, chunks that end inside blocks, single tokens, an empty append: the codes are those of one quantisation."""
+    g = torch.Generator().manual_seed(1)
+    bsz, hkv = 3, 2
+    pieces = [5, block + 7, 1, 1, 2 * block - 14, 0, 3 * block + 1, 1]
+    total = sum(pieces)
+    k, v = rows(g, bsz, hkv, total, dtype=dtype), rows(g, bsz, hkv, total, dtype=dtype, gain=3e-3)
+    cache, _, _ = make(g, fmt, dtype, block, page, [total + 2 * block] * bsz, hkv)
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).fill_(0x55)
+    lens = torch.zeros(bsz, dtype=torch.int32, device=DEV)
+    at = 0
+    for n in pieces:
+        ops.kv8_append(cache, k[:, :, at: at + n].to(DEV), v[:, :, at: at + n].to(DEV), lens)
+        lens += n
+        at += n
+    full = total // block * block
+    for b in range(bsz):
+        for got, x in zip(read_back(cache, b, full, hkv), (k, v)):
+            assert torch.equal(got, held(x[b, :, :full], fmt, block, True))
+    for got, x in ((cache.open_k, k), (cache.open_v, v)):
+        assert torch.equal(got[:, :, : total - full].cpu(), x[:, :, full:])
+    # rows behind the last full block: left as they were
+    codes = cache.k if page == 0 else cache.k[cache.page_table.long()].flatten(1, 2).transpose(1, 2)
+    assert bool((codes.contiguous().view(torch.uint8)[:, :, full: full + block] == 0x55).all())
+    rk, rv = ops.kv8_read(cache, dtype, seq_len=total + 1, seq_lens=lens)
+    for got, x in ((rk, k), (rv, v)):
+        for b in range(bsz):
+            assert torch.equal(got[b, :, :total].cpu(), held(x[b], fmt, block, True).float().to(dtype))
+        assert not got[:, :, total:].any()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("n", [1, 15, 64, 65, 200])
+def test_append_closing_the_last_block(fmt, n):
+    g = torch.Generator().manual_seed(2)
+    cache, k, v = make(g, fmt, BF, 64, 0, [n], 3, open_rows=False)
+    cache.k.view(torch.uint8)[:, :, n:].fill_(7)
+    for got, want in zip(read_back(cache, 0, n, 3), (k[0], v[0])):
+        assert torch.equal(got, want)
+    x = rows(g, 1, 3, n)
+    ops.kv8_append(cache, x.to(DEV), x.to(DEV), 0, close=True)
+    assert torch.equal(read_back(cache, 0, n, 3)[0], held(x[0], fmt, 64, False))
+    assert bool((cache.k.view(torch.uint8)[:, :, n:] == 7).all())
+
+
+def test_append_strides_ragged_lengths_and_what_does_not_fit():
+    g = torch.Generator().manual_seed(3)
+    cache = ops.KV8.empty(4, 2, 96, "int8", 32, BF, DEV)
+    x = rows(g, 4, 40, 2).transpose(1, 2)  # (b, heads, n, 128), token-major storage
+    y = rows(g, 4, 40, 2).transpose(1, 2)
+    starts = torch.tensor([0, 60, -1, 57], dtype=torch.int32, device=DEV)  # 60 + 40 and -1 do not fit
+    lens = torch.tensor([33, 40, 40, 7], dtype=torch.int32, device=DEV)
+    ops.kv8_append(cache, x.to(DEV), y.to(DEV), starts, lens)
+    assert torch.equal(read_back(cache, 0, 32, 2)[0], held(x[0, :, :32], "int8", 32, True))
+    assert torch.equal(cache.open_v[0, :, :1].cpu(), y[0, :, 32:33])
+    for b in (1, 2):
+        assert not cache.k_scale[b].any() and not cache.open_k[b].any()
+    want = torch.zeros(2, 32, 128, dtype=BF)  # request 3: its rows 57 .. 64 complete block 1 behind open rows of zeros
+    want[:, 25:32] = x[3, :, :7]
+    c, s = ref.quantise(want, "int8")
+    assert torch.equal(read_back(cache, 3, 64, 2)[0][:, 32:], c * s.double()[:, None, None])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_at_the_borders_of_the_format(fmt, dtype):
+    """Zeros, the type's extremes, subnormals, exact ties, and NaN / infinity poisoning their block only."""
+    g = torch.Generator().manual_seed(4)
+    big = torch.finfo(dtype).max
+    x = torch.zeros(1, 1, 16 * 8, 128, dtype=dtype)
+    x[..., 16:32, :] = torch.linspace(-1, 1, 128).to(dtype) * big
+    x[..., 32:48, :] = torch.finfo(dtype).smallest_normal * torch.arange(128).to(dtype) / 256
+    x[..., 48:64, :] = (torch.arange(128) - 64).to(dtype)  # amax / 2, the tie of the integer format, among them
+    x[..., 64:80, :] = (torch.arange(2048).view(16, 128) % 897 - 448).to(dtype)  # e4m3: every integer up to qmax, scale 1
+    x[..., 80:96, :] = rows(g, 16, dtype=dtype)
+    x[..., 85, 3] = float("inf")
+    x[..., 96:112, :] = rows(g, 16, dtype=dtype)
+    x[..., 100, 90] = float("nan")
+    x[..., 112:, :] = rows(g, 16, dtype=dtype)
+    cache = ops.KV8.empty(1, 1, 128, fmt, 16, dtype, DEV)
+    ops.kv8_append(cache, x.to(DEV), x.to(DEV), 0)
+    for lo in range(0, 128, 16):
+        c, s = ref.quantise(x[0, :, lo: lo + 16], fmt)
+        assert torch.equal(cache.k[0, :, lo: lo + 16].cpu().double(), c), lo
+        assert torch.equal(cache.v_scale[0, :, lo // 16].cpu().nan_to_num(-1), s.nan_to_num(-1)), lo
+    q = rows(g, 1, 2, dtype=dtype).to(DEV)
+    assert bool(ops.kv8_dense_attn(q, cache, seq_len=96).isnan().all())
+    # rows of the finite blocks; without the block of bfloat16's largest numbers (3.4e38), whose logits, sums of
+    # 128 products with queries of order 1 to 5, are beyond fp32 in any arithmetic that forms them there
+    at = torch.cat([torch.arange(0, 16), torch.arange(32, 80), torch.arange(112, 128)]).to(torch.int32).to(DEV)[None]
+    assert bool(ops.kv8_sparse_attn(q, cache, idx=at).isfinite().all())
+
+
+# ------------------------------------------------------------------------------------------ attention
+def check_attention(got, q, ks, vs, scale, dtype):
+    for b, (k, v) in enumerate(zip(ks, vs)):
+        out, _, _, spread, mass = ref.attention(q[b], k, v, scale)
+        bound = ref.output_bound(out, spread, mass, dtype)
+        diff = (got[b].cpu().double() - out).abs()
+        assert bool((diff <= bound).all()), (b, float((diff / bound).max()))
+
+
+DENSE = [
+    # fmt, dtype, block, page, hkv, group, lengths
+    ("e4m3", BF, 64, 0, 2, 4, [1]),
+    ("int8", BF, 16, 0, 1, 1, [17, 16, 15, 1, 0, 33]),
+    ("e4m3", HF, 32, 0, 3, 7, [31, 32, 64, 95, 0]),
+    ("int8", HF, 64, 0, 8, 8, [700]),
+    ("e4m3", BF, 128, 0, 2, 2, [127, 128, 129, 515]),
+    ("int8", BF, 16, 16, 8, 4, [1, 100, 257, 0, 512]),
+    ("e4m3", HF, 16, 48, 5, 3, [1000, 47, 48, 49]),
+    ("int8", HF, 32, 96, 2, 5, [95, 96, 97, 64]),
+    ("e4m3", BF, 64, 64, 8, 4, [3001]),
+    ("int8", BF, 64, 0, 4, 6, [5000, 1, 4097]),
+]
+
+
+@pytest.mark.parametrize("fmt, dtype, block, page, hkv, group, lens", DENSE)
+def test_dense(fmt, dtype, block, page, hkv, group, lens):
+    g = torch.Generator().manual_seed(11)
+    cache, ks, vs = make(g, fmt, dtype, block, page, lens, hkv)
+    q = rows(g, len(lens), hkv * group, dtype=dtype)
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=max(lens))
+    check_attention(out, q, ks, vs, 128 ** -0.5, dtype)
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert not out[b].any()
+    # a longer bound on the lengths splits the rows otherwise
+    more = ops.kv8_dense_attn(q.to(DEV)[:, :, None], cache, seq_lens=t, scale=0.3)
+    check_attention(more, q, ks, vs, 0.3, dtype)
+
+
+@pytest.mark.parametrize("fmt, dtype, block, page, hkv, group, lens", DENSE[1:])
+@pytest.mark.parametrize("selector", ["last", "softmax_before_last", "softmax_sum_last"])
+def test_dense_scores(fmt, dtype, block, page, hkv, group, lens, selector):
+    """Scored lengths that end inside a block, at and behind the open rows, and beyond a request's own length."""
+    g = torch.Generator().manual_seed(12)
+    cache, ks, vs = make(g, fmt, dtype, block, page, lens, hkv)
+    q = rows(g, len(lens), hkv * group, dtype=dtype)
+    most = max(lens)
+    want_len = [max(0, n - (0, 1, 13)[b % 3]) for b, n in enumerate(lens)]
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    tl = torch.tensor(want_len, dtype=torch.int32, device=DEV)
+    buf = torch.full((len(lens), most + 5), 77.0, device=DEV)[:, :most]
+    out, scores = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=most, selector=selector, score_len=most,
+                                     score_lens=tl, scores_out=buf)
+    assert scores.data_ptr() == buf.data_ptr()
+    check_attention(out, q, ks, vs, 128 ** -0.5, dtype)
+    for b, n in enumerate(want_len):
+        assert bool((scores[b, n:] == 77).all())
+        if n == 0:
+            continue
+        _, x, p, _, mass = ref.attention(q[b], ks[b][:, :n], vs[b][:, :n], 128 ** -0.5)
+        dl = ref.logit_error(mass)
+        if selector == "last":
+            y, bound = x.amax(0), dl.amax(0)
+        else:
+            # the logit's own error and the normaliser's; 2^-18 for exponentials and sums in fp32
+            rel = torch.expm1(dl + dl.amax(1, keepdim=True)) * 2 + 2.0 ** -18
+            y, bound = (p.amax(0), (p * rel).amax(0)) if selector == "softmax_before_last" else (p.sum(0), (p * rel).sum(0))
+            bound = bound + 2.0 ** -120
+        diff = (scores[b, :n].cpu().double() - y).abs()
+        assert bool((diff <= bound).all()), (b, float((diff / bound).max()))
+
+
+def test_dense_select_equals_topk_of_its_scores():
+    g = torch.Generator().manual_seed(13)
+    cache, _, _ = make(g, "e4m3", BF, 64, 0, [900, 500], 2)
+    q = rows(g, 2, 8).to(DEV)
+    t = torch.tensor([900, 500], dtype=torch.int32, device=DEV)
+    out, scores, idx = ops.kv8_dense_attn(q, cache, seq_lens=t, seq_len=900, selector="softmax_before_last", score_len=900,
+                                          score_lens=t, select_k=60)
+    assert torch.equal(idx, ops.topk(scores, 60, t))
+    assert torch.equal(out, ops.kv8_dense_attn(q, cache, seq_lens=t, seq_len=900, selector="last")[0])
+
+
+SPARSE = [
+    # fmt, dtype, block, page, hkv, group, lengths, selected rows, tails
+    ("e4m3", BF, 64, 0, 2, 4, [300], [1], [0]),
+    ("int8", BF, 16, 0, 8, 4, [500, 40, 7], [100, 40, 0], [5, 0, 3]),
+    ("e4m3", HF, 32, 0, 3, 7, [1000, 1000], [333, 0], [0, 0]),
+    ("int8", HF, 16, 16, 5, 2, [2000, 100, 33, 17], [1500, 99, 33, 1], [129, 0, 31, 16]),
+    ("e4m3", BF, 16, 48, 8, 8, [700, 3], [70, 3], [1, 40]),
+    ("int8", BF, 64, 0, 1, 1, [6000], [5999], [700]),
+]
+
+
+@pytest.mark.parametrize("fmt, dtype, block, page, hkv, group, lens, picks, tails", SPARSE)
+def test_sparse(fmt, dtype, block, page, hkv, group, lens, picks, tails):
+    g = torch.Generator().manual_seed(21)
+    bsz = len(lens)
+    cache, ks, vs = make(g, fmt, dtype, block, page, lens, hkv, open_rows=False)
+    q = rows(g, bsz, hkv * group, dtype=dtype)
+    idx = torch.full((bsz, max(picks) + 3), -1, dtype=torch.int32)
+    tk, tv = (rows(g, bsz, max(tails) + 1, hkv, dtype=dtype).transpose(1, 2) for _ in "kv")
+    wk, wv = [], []
+    for b in range(bsz):
+        at = torch.randperm(lens[b], generator=g)[: picks[b]].sort()[0]
+        idx[b, : picks[b]] = at.to(torch.int32)
+        wk.append(torch.cat([ks[b][:, at], tk[b, :, : tails[b]].double()], 1))
+        wv.append(torch.cat([vs[b][:, at], tv[b, :, : tails[b]].double()], 1))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    kw = dict(tail_k=tk.to(DEV), tail_v=tv.to(DEV), tail_lens=i32(tails))
+    di = idx.to(DEV)
+    out = ops.kv8_sparse_attn(q.to(DEV), cache, idx=di, sel_lens=i32(picks), **kw)
+    check_attention(out, q, wk, wv, 128 ** -0.5, dtype)
+    padded = ops.kv8_sparse_attn(q.to(DEV), cache, idx=di, **kw)  # padding (-1) takes no part
+    check_attention(padded, q, wk, wv, 128 ** -0.5, dtype)
+    stray = torch.where(di < 0, 1 << 30, di)
+    assert torch.equal(ops.kv8_sparse_attn(q.to(DEV), cache, idx=stray, **kw), padded)
+    if page:
+        slots = cache.slot_index(di)
+        assert torch.equal(ops.kv8_sparse_attn(q.to(DEV), cache, slots=slots, sel_lens=i32(picks), **kw), out)
+    if max(tails) == 0:
+        none = ops.kv8_sparse_attn(q.to(DEV), cache, idx=di, sel_lens=i32(picks))
+        check_attention(none, q, wk, wv, 128 ** -0.5, dtype)
+
+
+def test_sparse_without_an_index_and_with_a_tail_alone():
+    g = torch.Generator().manual_seed(22)
+    cache, ks, vs = make(g, "int8", BF, 32, 0, [130, 77], 2, open_rows=False)
+    q = rows(g, 2, 8)
+    tk, tv = rows(g, 2, 2, 9), rows(g, 2, 2, 9)
+    n = torch.tensor([130, 77], dtype=torch.int32, device=DEV)
+    out = ops.kv8_sparse_attn(q.to(DEV), cache, sel_len=130, sel_lens=n, tail_k=tk.to(DEV), tail_v=tv.to(DEV))
+    check_attention(out, q, [torch.cat([k, t.double()], 1) for k, t in zip(ks, tk)],
+                    [torch.cat([v, t.double()], 1) for v, t in zip(vs, tv)], 128 ** -0.5, BF)
+    out = ops.kv8_sparse_attn(q.to(DEV), cache, sel_len=0, tail_k=tk.to(DEV), tail_v=tv.to(DEV), tail_len=4)
+    check_attention(out, q, tk[:, :, :4].double(), tv[:, :, :4].double(), 128 ** -0.5, BF)
+
+
+def test_pages_outside_the_pool_take_no_part():
+    g = torch.Generator().manual_seed(23)
+    cache, ks, vs = make(g, "e4m3", BF, 16, 32, [200, 90], 2)
+    q = rows(g, 2, 8)
+    t = torch.tensor([200, 90], dtype=torch.int32, device=DEV)
+    cache.page_table[0, 2], cache.page_table[0, 5] = -1, 1 << 30
+    cache.page_table[1, :2] = -7
+    keep = [[r for r in range(200) if r // 32 not in (2, 5)], [r for r in range(90) if r // 32 not in (0, 1)]]
+    out, scores = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=200, selector="softmax_sum_last", score_len=200,
+                                     score_lens=t)
+    check_attention(out, q, [k[:, i] for k, i in zip(ks, keep)], [v[:, i] for v, i in zip(vs, keep)], 128 ** -0.5, BF)
+    assert not scores[0, 64:96].any() and not scores[0, 160:192].any() and bool(scores[0, :64].all())
+    raw = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=200, selector="last", score_len=200, score_lens=t)[1]
+    assert bool((raw[0, 64:96] == float("-inf")).all()) and bool(raw[1, 64:90].isfinite().all())
+    cache.page_table[:] = -1  # closed rows: none left
+    only_open = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=200)
+    check_attention(only_open, q, [ks[0][:, 192:], ks[1][:, 80:]], [vs[0][:, 192:], vs[1][:, 80:]], 128 ** -0.5, BF)
+    whole = torch.tensor([192, 80], dtype=torch.int32, device=DEV)
+    out, scores = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=whole, seq_len=200, selector="softmax_before_last",
+                                     score_len=192, score_lens=whole)
+    assert not out.any() and not scores[0].any()
+    x = rows(g, 2, 2, 1)
+    before = [t.clone() for t in (cache.k.view(torch.uint8), cache.k_scale)]
+    ops.kv8_append(cache, x.to(DEV), x.to(DEV), torch.tensor([207, 95], dtype=torch.int32, device=DEV))  # both fill a block
+    assert torch.equal(cache.k.view(torch.uint8), before[0]) and torch.equal(cache.k_scale, before[1])
+
+
+def test_large_values_and_a_lone_huge_logit():
+    """Logits of thousands: the running maximum moves late, everything else underflows to nothing."""
+    g = torch.Generator().manual_seed(24)
+    cache, ks, vs = make(g, "int8", BF, 16, 0, [2000], 1)
+    k = rows(g, 1, 1, 16, gain=300.0)
+    v = rows(g, 1, 1, 16)
+    ops.kv8_append(cache, k.to(DEV), v.to(DEV), 2000)
+    ks[0], vs[0] = (torch.cat([a, held(x[0], "int8", 16, True)], 1) for a, x in ((ks[0], k), (vs[0], v)))
+    q = rows(g, 1, 4, gain=8.0)
+    out = ops.kv8_dense_attn(q.to(DEV), cache, seq_len=2016)
+    # (2000 is a multiple of 16: the sixteen rows are one block)
+    want, _, p, spread, mass = ref.attention(q[0], ks[0], vs[0], 128 ** -0.5)
+    assert float(p.amax()) > 0.9
+    dl = ref.logit_error(mass.amax())
+    assert bool(((out[0].cpu().double() - want).abs() <= ref.output_bound(want, spread, mass.amax(), BF)).all()) or dl > 1
+
+
+# ------------------------------------------------------------------------------------------ use together
+def test_decode_loop_append_and_attend_in_a_replayed_graph():
+    """A captured step (append one token, attend, score and select, attend to the selection) replayed with the lengths
+    on the device, every replay against the eager step on a second cache, eager work and waits in between."""
+    g = torch.Generator().manual_seed(31)
+    lens0 = [125, 64, 1]
+    caches = [make(torch.Generator().manual_seed(5), "e4m3", BF, 16, 32, lens0, 2, spare=8)[0] for _ in range(2)]
+    steps = 40
+    ks, vs = rows(g, steps, 3, 2, 1).to(DEV), rows(g, steps, 3, 2, 1).to(DEV)
+    qs = rows(g, steps, 3, 8).to(DEV)
+    bound = max(lens0) + steps
+
+    def step(cache, q, k, v, lens):
+        ops.kv8_append(cache, k, v, lens)
+        lens += 1
+        out, scores, idx = ops.kv8_dense_attn(q, cache, seq_lens=lens, seq_len=bound, selector="softmax_before_last",
+                                              score_len=bound, score_lens=lens // 16 * 16, select_k=20)
+        return out, idx, ops.kv8_sparse_attn(q, cache, idx=idx, tail_k=k, tail_v=v)
+
+    q, k, v = qs[0].clone(), ks[0].clone(), vs[0].clone()
+    lens = [torch.tensor(lens0, dtype=torch.int32, device=DEV) for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        spare = make(torch.Generator().manual_seed(5), "e4m3", BF, 16, 32, lens0, 2, spare=8)[0]
+        step(spare, q, k, v, torch.tensor(lens0, dtype=torch.int32, device=DEV))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[0], q, k, v, lens[0])
+    lens[0].copy_(torch.tensor(lens0))
+    for i in range(steps):
+        q.copy_(qs[i]), k.copy_(ks[i]), v.copy_(vs[i])
+        graph.replay()
+        want = step(caches[1], qs[i], ks[i], vs[i], lens[1])
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), i
+        if i % 7 == 0:
+            torch.cuda.synchronize()
+    assert torch.equal(lens[0], lens[1])
+    for name in ("k", "v"):
+        assert torch.equal(getattr(caches[0], name).view(torch.uint8), getattr(caches[1], name).view(torch.uint8))
+
+
+def test_two_graphs_and_another_stream_do_not_share_scratch():
+    g = torch.Generator().manual_seed(32)
+    cache, ks, vs = make(g, "int8", HF, 64, 0, [4000], 2)
+    qa, qb = rows(g, 1, 8, dtype=HF).to(DEV), rows(g, 1, 8, dtype=HF).to(DEV)
+    want = [ops.kv8_dense_attn(x, cache, seq_len=4000) for x in (qa, qb)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in (qa, qb):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(ops.kv8_dense_attn(x, cache, seq_len=4000))
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for s, gr in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                gr.replay()
+        eager = ops.kv8_dense_attn(qa, cache, seq_len=4000)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[0])
+
+
+def test_long_cache_offsets_pass_32_bits():
+    """One request whose codes lie beyond 4 GiB from the base: every row attended through an index and densely."""
+    g = torch.Generator().manual_seed(33)
+    hkv, n = 2, 256
+    far = (1 << 32) // 128 + 4096  # tokens between the two heads' rows: the second head starts behind 4 GiB
+    base = [torch.zeros(far * 128 + n * 128, dtype=torch.uint8, device=DEV) for _ in "kv"]
+    k, v = (torch.as_strided(t, (1, hkv, n, 128), (0, far * 128, 128, 1)).view(torch.int8) for t in base)
+    s = torch.zeros((2, 1, hkv, n // 64), device=DEV)
+    cache = ops.KV8(k, v, s[0], s[1], 64)
+    x, y = rows(g, 1, hkv, n), rows(g, 1, hkv, n)
+    ops.kv8_append(cache, x.to(DEV), y.to(DEV), 0, close=True)
+    q = rows(g, 1, 8)
+    kk, vv = [held(x[0], "int8", 64, False)], [held(y[0], "int8", 64, False)]
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache), q, kk, vv, 128 ** -0.5, BF)
+    idx = torch.arange(n, dtype=torch.int32, device=DEV)[None]
+    check_attention(ops.kv8_sparse_attn(q.to(DEV), cache, idx=idx), q, kk, vv, 128 ** -0.5, BF)
+
+
+def test_front_end_refusals():
+    cache = ops.KV8.empty(2, 2, 64, "int8", 32, BF, DEV)
+    q = torch.zeros((2, 8, 128), dtype=BF, device=DEV)
+    i = torch.zeros((2, 4), dtype=torch.int32, device=DEV)
+    for bad in (lambda: ops.kv8_dense_attn(q.half(), cache), lambda: ops.kv8_dense_attn(q.float(), cache),
+                lambda: ops.kv8_dense_attn(q[:1], cache), lambda: ops.kv8_dense_attn(q.cpu(), cache),
+                lambda: ops.kv8_dense_attn(q, cache, select_k=3),
+                lambda: ops.kv8_dense_attn(q, cache, seq_lens=torch.zeros(2, dtype=torch.int64, device=DEV)),
+                lambda: ops.kv8_dense_attn(q, cache, seq_lens=torch.zeros(3, dtype=torch.int32, device=DEV)),
+                lambda: ops.kv8_sparse_attn(q, cache, idx=i.long()), lambda: ops.kv8_sparse_attn(q, cache, idx=i[:1]),
+                lambda: ops.kv8_sparse_attn(q, cache, idx=i, sel_len=5), lambda: ops.kv8_sparse_attn(q, cache, slots=i),
+                lambda: ops.kv8_sparse_attn(q, cache, idx=i, tail_len=2), lambda: cache.slot_index(i),
+                lambda: ops.kv8_append(cache, q[:, :2, None], q[:, :2, None].half(), 0),
+                lambda: ops.kv8_append(cache, q[:, :3, None], q[:, :3, None], 0),
+                lambda: ops.kv8_append(cache, q[:, :2, None], q[:, :2, None], i[:, 0].long())):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: ops.kv8_dense_attn(q, cache, seq_len=65), lambda: ops.kv8_dense_attn(q, cache, seq_len=0),
+                lambda: ops.kv8_append(cache, q[:, :2, None], q[:, :2, None], 64),
+                lambda: ops.kv8_append(cache, q[:, :2, None], q[:, :2, None], 5, close=True)):
+        with pytest.raises(Exception, match="invalid"):
+            bad()
