@@ -24,11 +24,13 @@ int kv8_validate(const okv_kv8_cache_t* c, const char* what) {
               "%s: scale pointers must be 4-byte aligned", what);
   OKV_REQUIRE(c->token_stride % 16 == 0 && c->head_stride % 16 == 0 && c->batch_stride % 16 == 0 && c->page_stride % 16 == 0,
               OKV_ERR_INVALID, "%s: code strides must be multiples of 16 bytes", what);
-  OKV_REQUIRE(c->token_stride >= 0 && c->token_stride < (1ll << 31), OKV_ERR_UNSUPPORTED, "%s: token stride %lld", what,
+  OKV_REQUIRE(c->token_stride >= 0 && c->token_stride < (1ll << 26), OKV_ERR_UNSUPPORTED, "%s: token stride %lld", what,
               (long long)c->token_stride);
   if (c->page_table) {
     OKV_REQUIRE(c->page_size >= bt && c->page_size % bt == 0, OKV_ERR_INVALID,
                 "%s: page_size %d is not a multiple of block_tokens %d", what, c->page_size, bt);
+    OKV_REQUIRE((int64_t)c->num_pages * c->page_size < (1ll << 31) && (int64_t)c->page_table_stride * c->page_size < (1ll << 31),
+                OKV_ERR_UNSUPPORTED, "%s: 2^31 token slots or more", what);
     OKV_REQUIRE(c->page_table_stride >= 1 && c->num_pages >= 1, OKV_ERR_INVALID, "%s: page_table_stride %d, num_pages %d",
                 what, c->page_table_stride, c->num_pages);
   } else {

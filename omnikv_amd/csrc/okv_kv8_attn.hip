@@ -26,8 +26,8 @@ struct Kv8Attn {
   int32_t sparse, slots;
   const int32_t* idx;
   int64_t idx_stride;
-  const void* tail[2];
-  int64_t tail_token_stride, tail_head_stride, tail_batch_stride;
+  const void* late[2];  // 16-bit rows behind the codes: the tail, or the open buffers
+  int64_t late_token_stride, late_head_stride, late_batch_stride;
   const int32_t* tail_lens;
   int32_t max_tail_len;
   const int32_t* score_lens;
@@ -38,6 +38,9 @@ struct Kv8Attn {
   float* logits;    // [batch][Hq][logits_stride], natural units
   int64_t logits_stride;
   int32_t splits, split_rows;
+  int32_t fold;         // raw scores: the q heads of a kv head are folded by the split (1 max, 2 sum): one logits row per kv head
+  int32_t logit_heads;  // rows of `logits` per request
+  int32_t lds_scales;   // floats before the scale staging of the gather mode
   // outputs
   void* out;
   float* scores;
@@ -54,139 +57,551 @@ __device__ __forceinline__ int kv8_score_len(const Kv8Attn& a, int b, int len) {
   return s < len ? s : len;
 }
 
-// grid (Hkv, splits, batch): eight lanes hold a row, 16 elements each.
-template <typename T, typename F>
-__global__ __launch_bounds__(256) void kv8_split(Kv8Attn a) {
-  __shared__ float s_q[kMaxGroup][kD];
-  __shared__ float s_m[32][kMaxGroup], s_l[32][kMaxGroup];
-  __shared__ float s_o[4][kMaxGroup][kD];
+// ---------------------------------------------------------------- matrix-core pieces
+// two fp32 -> one dword of two 16-bit elements, the first in the low half
+__device__ __forceinline__ uint32_t pack_pair(const BF16*, float a, float b) {
+  const f32x2_t x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
+}
+__device__ __forceinline__ uint32_t pack_pair(const F16*, float a, float b) {
+  const f32x2_t x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_t));
+}
+__device__ __forceinline__ f32x2_t unpack_pair(const BF16*, uint32_t x) {
+  return f32x2_t{__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)};
+}
+__device__ __forceinline__ f32x2_t unpack_pair(const F16*, uint32_t x) {
+  const f16x2_t h = __builtin_bit_cast(f16x2_t, x);
+  return f32x2_t{(float)h.x, (float)h.y};
+}
+
+// bytes 2H and 2H+1 of x -> a dword of two 16-bit elements; every code is exact in both types
+template <int H>
+__device__ __forceinline__ uint32_t decode_pair(E4M3, const BF16*, uint32_t x) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, H != 0));
+}
+template <int H>
+__device__ __forceinline__ uint32_t decode_pair(E4M3, const F16*, uint32_t x) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, H != 0));
+}
+template <int H, typename T>
+__device__ __forceinline__ uint32_t decode_pair(I8, const T*, uint32_t x) {
+  return pack_pair((const T*)nullptr, (float)(int8_t)(x >> (16 * H)), (float)(int8_t)(x >> (16 * H + 8)));
+}
+
+// lanes 8..15 (MASK 0xC) or 0..7 (MASK 0x3) of every 16-lane row take `from` of the lane eight away, the others keep `own`
+template <int MASK>
+__device__ __forceinline__ uint32_t take8(uint32_t own, uint32_t from) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)own, (int)from, 0x128, 0xf, MASK, false);
+}
+// value of lane H of the caller's 16-lane row
+template <int H>
+__device__ __forceinline__ float row_lane(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x150 + H, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+// over the four lane rows (lanes l, l^16, l^32, l^48), left in all of them
+__device__ __forceinline__ float rows_max(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+enum { kContiguous = 0, kPaged = 1, kGather = 2 };
+
+// A wave's 32 rows: K rows (m & 7) + 8x, 16-byte chunk j + 4(m >> 3), and V rows 4j + i of the upper or lower sixteen
+// (m >> 3), chunk m & 7, of lane l = 16j + m: every load covers whole 128-byte rows.
+struct Kv8Tile {
+  uint4 k[4], v[4];
+  float sc;   // dense: lane row 0..3 = K scale of rows 0-15, of 16-31, V scales likewise; gather: lanes 0..31 K, 32..63 V scale of row l % 32
+  uint32_t ok;  // dense: bit s = page of rows 16s.. lies in the pool; gather: this lane's own row (l % 32) takes part
+};
+struct Kv8Rows {
+  int page[2];         // paged
+  int k[4], v[4], s;   // gather: index entries
+};
+
+// grid (Hkv, splits, batch), four waves that take 32-row tiles in turn.
+//
+// q.K^T: the tile's codes become 16-bit elements (exact) and are the A operand of v_mfma_f32_16x16x32: lane 16j + m
+// holds row m, elements 16j .. +16 and 64 + 16j .. +16.  Loading that directly would touch 16 rows x 64 bytes per
+// instruction; the loads take whole 128-byte rows instead, and lanes m and m^8 exchange halves (one DPP move per dword).
+// The kv head's q heads are columns 0..7 of B (padded by repeating the last) and AGAIN columns 8..15.
+// P.V: the logits come out as lane (column m, rows 4j .. +4), which is the A operand's layout of P.  Columns 0..7
+// carry bf16(p), columns 8..15 the rest p - bf16(p): the spare half of the matrix instruction gives P 16 bits.  The V
+// scale of a row is folded into its p; V's codes, exact in bf16, are the B operand: a lane's eight rows x
+// eight elements, turned by byte permutes as they are decoded.
+// Scales of K are applied to the fp32 logits.  One running maximum per q head and wave; the waves meet in LDS.
+template <typename T, typename F, int MODE, bool LOGITS>
+__global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
+  extern __shared__ float lds[];
   const okv_kv8_cache_t& c = a.c;
   const int g = blockIdx.x, split = blockIdx.y, b = blockIdx.z, G = a.group;
   const int main_len = clamp_len(a.lens, b, a.max_len);
-  const int tail_len = a.max_tail_len ? clamp_len(a.tail_lens, b, a.max_tail_len) : 0;
-  const int L = main_len + tail_len, A = kv8_score_len(a, b, main_len);
+  const int L = main_len + (a.max_tail_len ? clamp_len(a.tail_lens, b, a.max_tail_len) : 0);
+  const int A = LOGITS ? kv8_score_len(a, b, main_len) : 0;
   int begin, end;
   rl_split_range(split, a.split_rows, A, L, &begin, &end);
   if (begin >= end) return;
+  // rows [0, closed) are codes, the rest 16-bit rows: the open block, or the tail
   const int closed = a.sparse || !c.open_k ? main_len : main_len / c.block_tokens * c.block_tokens;
-  for (int i = threadIdx.x; i < G * kD; i += 256) {
-    const T x = reinterpret_cast<const T*>(a.q)[(int64_t)(b * a.hq + g * G) * kD + i];
-    float v;
-    if constexpr (sizeof(T) == 2) {
-      uint4 u = make_uint4(x.v, 0, 0, 0);
-      float o[8];
-      cvt8((const T*)nullptr, u, o);
-      v = o[0];
-    }
-    s_q[i / kD][i % kD] = v;
+  const int main_end = min(end, closed);
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m16 = lane & 15, j = lane >> 4, m8 = m16 & 7, hi8 = m16 >> 3;
+
+  uint4 qf[4];
+  {
+    const int h = m8 < G ? m8 : G - 1;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(b * a.hq + g * G + h) * kD + 16 * j;
+    qf[0] = *reinterpret_cast<const uint4*>(qp);
+    qf[1] = *reinterpret_cast<const uint4*>(qp + 8);
+    qf[2] = *reinterpret_cast<const uint4*>(qp + 64);
+    qf[3] = *reinterpret_cast<const uint4*>(qp + 72);
   }
-  __syncthreads();
-  const int lane8 = threadIdx.x & 7, slot = threadIdx.x >> 3, e0 = 16 * lane8;
-  const int64_t room = a.slots ? (int64_t)c.num_pages * c.page_size : kv8_room(c);
-  float m[kMaxGroup], l[kMaxGroup], o[kMaxGroup][16];
+
+  const uint32_t ts = (uint32_t)c.token_stride;
+  const int64_t head = (int64_t)g * c.head_stride + (MODE == kPaged || c.page_table ? 0 : (int64_t)b * c.batch_stride);
+  const int64_t shead = (int64_t)g * c.scale_head_stride + (MODE == kPaged || c.page_table ? 0 : (int64_t)b * c.scale_batch_stride);
+  const uint8_t* kb = reinterpret_cast<const uint8_t*>(c.k_codes) + head;
+  const uint8_t* vb = reinterpret_cast<const uint8_t*>(c.v_codes) + head;
+  const float* ksb = c.k_scale + shead;
+  const float* vsb = c.v_scale + shead;
+  const uint32_t kcol = 16 * (j + 4 * hi8), vcol = 16 * m8;
+  const int last = main_end - 1;
+  const int32_t* table = c.page_table + (int64_t)b * c.page_table_stride;
+  const int32_t* idx = a.idx + (int64_t)b * a.idx_stride;
+  const uint32_t room = MODE != kGather ? 0 : a.slots ? (uint32_t)(c.num_pages * c.page_size) : (uint32_t)kv8_room(c);
+
+  // ---- what has to be known of a tile's rows before they can be addressed
+  auto rows_of = [&](int t, Kv8Rows& r) {
+    if (MODE == kPaged) {
 #pragma unroll
-  for (int h = 0; h < kMaxGroup; ++h) {
-    m[h] = -INFINITY;
-    l[h] = 0.f;
+      for (int s = 0; s < 2; ++s) r.page[s] = table[min(t + 16 * s, last) / c.page_size];
+    } else if (MODE == kGather) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[h][i] = 0.f;
-  }
-  for (int r0 = begin; r0 < end; r0 += 32) {
-    const int r = r0 + slot;
-    bool ok = r < end;
-    float kv[2][16];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) kv[x][i] = 0.f;
-    if (ok && r >= closed) {
-      const bool tail = r >= main_len;
-      const int t = tail ? r - main_len : r % c.block_tokens;
-      for (int x = 0; x < 2; ++x) {
-        const T* p = reinterpret_cast<const T*>(tail ? a.tail[x] : x ? c.open_v : c.open_k);
-        p += tail ? (int64_t)b * a.tail_batch_stride + (int64_t)t * a.tail_token_stride + (int64_t)g * a.tail_head_stride
-                  : (int64_t)b * c.open_batch_stride + (int64_t)t * c.open_token_stride + (int64_t)g * c.open_head_stride;
-        load8(p + e0, kv[x]);
-        load8(p + e0 + 8, kv[x] + 8);
+      for (int x = 0; x < 4; ++x) {
+        const int rk = min(t + 8 * x + m8, last), rv = min(t + 16 * hi8 + 4 * j + x, last);
+        r.k[x] = a.idx ? idx[rk] : rk;
+        r.v[x] = a.idx ? idx[rv] : rv;
       }
-    } else if (ok) {
-      const int t = a.idx ? a.idx[(int64_t)b * a.idx_stride + r] : r;
-      ok = t >= 0 && t < room;
-      if (ok) {
-        int64_t ro, so;
-        if (a.slots) {
-          ro = (int64_t)t * c.token_stride;
-          so = (int64_t)(t / c.block_tokens) * c.scale_block_stride;
+      const int rs = min(t + (lane & 31), last);
+      r.s = a.idx ? idx[rs] : rs;
+    }
+  };
+  auto load = [&](int t, const Kv8Rows& r, Kv8Tile& x) {
+    if (MODE == kContiguous) {
+      const bool whole = t + 32 <= main_end;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int rk = 8 * i + m8, rv = 16 * hi8 + 4 * j + i;
+        if (!whole) {
+          rk = min(rk, last - t);
+          rv = min(rv, last - t);
+        }
+        x.k[i] = load_stream16(kb + (int64_t)t * ts + (uint32_t)rk * ts + kcol);
+        x.v[i] = load_stream16(vb + (int64_t)t * ts + (uint32_t)rv * ts + vcol);
+      }
+      const int blk = min(t + 16 * (j & 1), last) / c.block_tokens;
+      x.sc = (j < 2 ? ksb : vsb)[(int64_t)blk * c.scale_block_stride];
+      x.ok = 3;
+    } else if (MODE == kPaged) {
+      int64_t base[2];
+      x.ok = 0;
+      int64_t sbase = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int u = min(t + 16 * s, last) & ~15;
+        const bool in = (uint32_t)r.page[s] < (uint32_t)c.num_pages;
+        const int64_t p = in ? r.page[s] : 0;
+        const int slot = u % c.page_size;
+        base[s] = p * c.page_stride + (int64_t)slot * ts;
+        const int64_t sb = p * c.scale_page_stride + (int64_t)(slot / c.block_tokens) * c.scale_block_stride;
+        if ((j & 1) == s) sbase = sb;
+        x.ok |= in ? 1u << s : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // rows past the last one: the last one again (its tile and page are those of u)
+        const int sk = i >> 1, rk = min((8 * i + m8) & 15, (last - t - 16 * sk < 0 ? last & 15 : min(15, last - t - 16 * sk)));
+        const int lv = last - t - 16 * hi8, rv = min(4 * j + i, lv < 0 ? last & 15 : min(15, lv));
+        x.k[i] = load_stream16(kb + base[sk] + (uint32_t)rk * ts + kcol);
+        x.v[i] = load_stream16(vb + (hi8 ? base[1] : base[0]) + (uint32_t)rv * ts + vcol);
+      }
+      x.sc = (j < 2 ? ksb : vsb)[sbase];
+    } else {
+      // an entry outside the request's room is read as row 0 and takes no part
+      auto at = [&](int t_, int64_t* row, int64_t* scale) -> bool {
+        bool in = (uint32_t)t_ < room;
+        const int tt = in ? t_ : 0;
+        if (c.page_table && !a.slots) {
+          const int pg = table[tt / c.page_size], slot = tt % c.page_size;
+          in = in && (uint32_t)pg < (uint32_t)c.num_pages;
+          const int64_t p = (uint32_t)pg < (uint32_t)c.num_pages ? pg : 0;
+          *row = p * c.page_stride + (int64_t)slot * ts;
+          *scale = p * c.scale_page_stride + (int64_t)(slot / c.block_tokens) * c.scale_block_stride;
         } else {
-          ok = kv8_locate(c, b, t, &ro, &so);
+          *row = (int64_t)tt * ts;
+          *scale = (int64_t)(tt / c.block_tokens) * c.scale_block_stride;
         }
-        for (int x = 0; x < 2; ++x) {
-          const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(x ? c.v_codes : c.k_codes) + ro +
-                                                          (int64_t)g * c.head_stride + e0);
-          const float s = (x ? c.v_scale : c.k_scale)[so + (int64_t)g * c.scale_head_stride];
-          decode4(F{}, u.x, kv[x]);
-          decode4(F{}, u.y, kv[x] + 4);
-          decode4(F{}, u.z, kv[x] + 8);
-          decode4(F{}, u.w, kv[x] + 12);
+        return in;
+      };
+      int64_t row, scale;
+      bool bad = false;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) kv[x][i] *= s;
+      for (int i = 0; i < 4; ++i) {
+        at(r.k[i], &row, &scale);
+        x.k[i] = load_stream16(kb + row + kcol);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bad = !at(r.v[i], &row, &scale) || bad;
+        x.v[i] = load_stream16(vb + row + vcol);
+      }
+      x.ok = at(r.s, &row, &scale);
+      x.sc = (lane < 32 ? ksb : vsb)[scale];
+    }
+  };
+
+  float m = -INFINITY;  // running maximum of head m8's logits, times log2(e), over the wave's rows
+  float l = 0.f;        // sum of exponentials over the rows of lane row j, relative to m
+  f32x4_t acc[8];       // acc[e][i]: element 16 m8 + 8 hi8 + e of head (4j + i) % 8; j < 2: from bf16(p), else the rest
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float rest = hi8 ? 1.f : 0.f;
+  const bool scored = LOGITS && begin < A;
+  float* slog = lds;  // [G, or 1 when the heads are folded][split_rows]: handed over at the end
+
+  auto raise_max = [&](float top) {
+    if (__ballot(top > m) == 0ull) return;
+    const float mn = rows_max(fmaxf(top, m));
+    const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    l *= al;
+    m = mn;
+    const float lo[4] = {row_lane<0>(al), row_lane<1>(al), row_lane<2>(al), row_lane<3>(al)};
+    const float hi[4] = {row_lane<4>(al), row_lane<5>(al), row_lane<6>(al), row_lane<7>(al)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = (j & 1) ? hi[i] : lo[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e][i] *= f;
+    }
+  };
+  auto stage_logits = [&](int row, const float (&v)[4]) {  // natural units, rows row .. +4
+    float o[4] = {v[0], v[1], v[2], v[3]};
+    if (a.fold) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = a.fold == 2 && m8 >= G ? 0.f : o[i];
+        const float x1 = dpp_f<0xB1>(x);  // lane ^ 1
+        x = a.fold == 1 ? fmaxf(x, x1) : x + x1;
+        const float x2 = dpp_f<0x4E>(x);  // lane ^ 2
+        x = a.fold == 1 ? fmaxf(x, x2) : x + x2;
+        const float x4 = dpp_f<0x141>(x);  // lane 7 - m8: the other quad, each uniform by now
+        o[i] = a.fold == 1 ? fmaxf(x, x4) : x + x4;
+      }
+    }
+    if (m16 < (a.fold ? 1 : G))
+      *reinterpret_cast<float4*>(slog + m16 * a.split_rows + (row - begin)) = make_float4(o[0], o[1], o[2], o[3]);
+  };
+  // a probability in two 16-bit parts: this lane's part of four of them
+  auto split_p = [&](auto* ty, const float (&p)[4], uint32_t* out) {
+    const uint32_t h0 = pack_pair(ty, p[0], p[1]), h1 = pack_pair(ty, p[2], p[3]);
+    const f32x2_t u0 = unpack_pair(ty, h0), u1 = unpack_pair(ty, h1);
+    out[0] = hi8 ? pack_pair(ty, p[0] - u0.x, p[1] - u0.y) : h0;
+    out[1] = hi8 ? pack_pair(ty, p[2] - u1.x, p[3] - u1.y) : h1;
+  };
+
+  auto compute = [&](int t, Kv8Tile& x, float* sstage) {
+    float ks[2][4], vs[2][4];
+    bool whole = t >= begin && t + 32 <= main_end;
+    if (MODE == kGather) {
+      // every lane has the scale of one row: the wave's 256 bytes of LDS hand the rows' four to their lane row
+      const bool okl = x.ok != 0;
+      sstage[lane] = lane < 32 ? (okl ? x.sc : 0.f) : (okl ? x.sc : 0.f);
+      const uint64_t oks = __ballot(okl);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float4 kk = *reinterpret_cast<const float4*>(sstage + 16 * s + 4 * j);
+        const float4 vv = *reinterpret_cast<const float4*>(sstage + 32 + 16 * s + 4 * j);
+        ks[s][0] = kk.x; ks[s][1] = kk.y; ks[s][2] = kk.z; ks[s][3] = kk.w;
+        vs[s][0] = vv.x; vs[s][1] = vv.y; vs[s][2] = vv.z; vs[s][3] = vv.w;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (oks != ~0ull) {  // wave-uniform: some entry is padding
+        whole = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((oks >> (16 * hi8 + 4 * j + i)) & 1)) x.v[i] = make_uint4(0, 0, 0, 0);
+        x.ok = (uint32_t)oks;
+      } else {
+        x.ok = 0xffffffffu;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float kk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x.sc), 16 * s));
+        const float vv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x.sc), 32 + 16 * s));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ks[s][i] = kk;
+          vs[s][i] = vv;
+        }
+      }
+      if (MODE == kPaged && x.ok != 3) {
+        whole = false;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          if (!((x.ok >> s) & 1)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              vs[s][i] = 0.f;
+              if (hi8 == s) x.v[i] = make_uint4(0, 0, 0, 0);
+            }
+          }
+      }
+    }
+    float p[2][4];
+    float top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x4_t S = {0.f, 0.f, 0.f, 0.f};
+      const uint4 k0 = x.k[2 * s], k1 = x.k[2 * s + 1];
+      const uint32_t lo[4] = {take8<0xC>(k0.x, k1.x), take8<0xC>(k0.y, k1.y), take8<0xC>(k0.z, k1.z), take8<0xC>(k0.w, k1.w)};
+      const uint32_t up[4] = {take8<0x3>(k1.x, k0.x), take8<0x3>(k1.y, k0.y), take8<0x3>(k1.z, k0.z), take8<0x3>(k1.w, k0.w)};
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const uint4 x0 = make_uint4(decode_pair<0>(F{}, (const T*)nullptr, lo[2 * f]), decode_pair<1>(F{}, (const T*)nullptr, lo[2 * f]),
+                                    decode_pair<0>(F{}, (const T*)nullptr, lo[2 * f + 1]), decode_pair<1>(F{}, (const T*)nullptr, lo[2 * f + 1]));
+        S = mfma16((const T*)nullptr, x0, qf[f], S);
+      }
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const uint4 x1 = make_uint4(decode_pair<0>(F{}, (const T*)nullptr, up[2 * f]), decode_pair<1>(F{}, (const T*)nullptr, up[2 * f]),
+                                    decode_pair<0>(F{}, (const T*)nullptr, up[2 * f + 1]), decode_pair<1>(F{}, (const T*)nullptr, up[2 * f + 1]));
+        S = mfma16((const T*)nullptr, x1, qf[2 + f], S);
+      }
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = S[i] * (ks[s][i] * a.scale);
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = t + 16 * s + 4 * j + i;
+          const bool in = r >= begin && r < main_end &&
+                          (MODE == kContiguous || ((x.ok >> (MODE == kPaged ? s : 16 * s + 4 * j + i)) & 1));
+          v[i] = in ? v[i] : -INFINITY;
+          vs[s][i] = in ? vs[s][i] : 0.f;
+        }
+      }
+      if (scored && t + 16 * s < main_end) stage_logits(t + 16 * s + 4 * j, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[s][i] = v[i] * kLog2e;
+        top = fmaxf(top, p[s][i]);
+      }
+    }
+    raise_max(top);
+    const float neg = m == -INFINITY ? 0.f : -m;
+    uint32_t pa[4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(p[s][i] + neg);
+        l += e;
+        w[i] = e * vs[s][i];
+      }
+      split_p((const BF16*)nullptr, w, pa + 2 * s);
+    }
+    const uint4 pf = make_uint4(pa[0], pa[1], pa[2], pa[3]);
+    // lane m keeps eight elements of the rows of both sixteens
+    uint32_t lo[4][2], up[4][2];  // [row i][dword]: rows 4j + i of the lower and upper sixteen
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i][0] = take8<0xC>(x.v[i].x, x.v[i].z);
+      lo[i][1] = take8<0xC>(x.v[i].y, x.v[i].w);
+      up[i][0] = take8<0x3>(x.v[i].z, x.v[i].x);
+      up[i][1] = take8<0x3>(x.v[i].w, x.v[i].y);
+    }
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // elements 4d + 2h, 4d + 2h + 1
+        const uint32_t sel = h ? 0x07030602u : 0x05010400u;
+        const uint32_t l01 = __builtin_amdgcn_perm(lo[1][d], lo[0][d], sel), l23 = __builtin_amdgcn_perm(lo[3][d], lo[2][d], sel);
+        const uint32_t u01 = __builtin_amdgcn_perm(up[1][d], up[0][d], sel), u23 = __builtin_amdgcn_perm(up[3][d], up[2][d], sel);
+        const BF16* bf = nullptr;
+        const uint4 e0 = make_uint4(decode_pair<0>(F{}, bf, l01), decode_pair<0>(F{}, bf, l23), decode_pair<0>(F{}, bf, u01),
+                                    decode_pair<0>(F{}, bf, u23));
+        const uint4 e1 = make_uint4(decode_pair<1>(F{}, bf, l01), decode_pair<1>(F{}, bf, l23), decode_pair<1>(F{}, bf, u01),
+                                    decode_pair<1>(F{}, bf, u23));
+        acc[4 * d + 2 * h] = mfma16(bf, pf, e0, acc[4 * d + 2 * h]);
+        acc[4 * d + 2 * h + 1] = mfma16(bf, pf, e1, acc[4 * d + 2 * h + 1]);
+      }
+    }
+  };
+
+  float* sstage = lds + a.lds_scales + 64 * wave;
+  {
+    int t = (begin & ~31) + 32 * wave;
+    if (t < main_end) {
+      const int t_last = t + ((last - t) >> 7 << 7);
+      Kv8Rows r0, r1;
+      Kv8Tile x0, x1;
+      rows_of(t, r0);
+      if (t == t_last) {
+        load(t, r0, x0);
+        compute(t, x0, sstage);
+      } else {
+        rows_of(t + 128, r1);
+        load(t, r0, x0);
+        while (true) {  // tile t + 128 in flight while t is consumed; past the last one, the last one again
+          load(min(t + 128, t_last), r1, x1);
+          rows_of(min(t + 256, t_last), r0);
+          compute(t, x0, sstage);
+          t += 128;
+          if (t > t_last) break;
+          load(min(t + 128, t_last), r0, x0);
+          rows_of(min(t + 256, t_last), r1);
+          compute(t, x1, sstage);
+          t += 128;
+          if (t > t_last) break;
         }
       }
     }
+  }
+
+  // ---- 16-bit rows: sixteen per tile, K straight in the A operand's layout
+  if (end > closed) {
+    const int lo = max(begin, closed);
+    const int64_t lts = a.late_token_stride;
+    const int64_t lbase = (int64_t)b * a.late_batch_stride + (int64_t)g * a.late_head_stride;
+    const T* lk = reinterpret_cast<const T*>(a.late[0]) + lbase;
+    const T* lv = reinterpret_cast<const T*>(a.late[1]) + lbase;
+    const T* ty = nullptr;
+    for (int t = lo + 16 * wave; t < end; t += 64) {
+      const int top_row = end - 1 - closed;  // rows counted from the first late one
+      const T* kp = lk + (int64_t)min(t - closed + m16, top_row) * lts + 16 * j;
+      const uint4 kf[4] = {*reinterpret_cast<const uint4*>(kp), *reinterpret_cast<const uint4*>(kp + 8),
+                           *reinterpret_cast<const uint4*>(kp + 64), *reinterpret_cast<const uint4*>(kp + 72)};
+      uint4 vf[4];
 #pragma unroll
-    for (int h = 0; h < kMaxGroup; ++h) {
-      if (h >= G) break;
-      float s = 0.f;
+      for (int i = 0; i < 4; ++i)
+        vf[i] = *reinterpret_cast<const uint4*>(lv + (int64_t)min(t - closed + 4 * j + i, top_row) * lts + 16 * m8 + 8 * hi8);
+      f32x4_t S = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s = fmaf(s_q[h][e0 + i], kv[0][i], s);
-      s += __shfl_xor(s, 1);
-      s += __shfl_xor(s, 2);
-      s += __shfl_xor(s, 4);
-      s = ok ? s * a.scale : -INFINITY;
-      if (a.logits && r < end && r < A && lane8 == 0) a.logits[(int64_t)(b * a.hq + g * G + h) * a.logits_stride + r] = s;
-      if (!ok) continue;
-      const float x = s * kLog2e, mn = fmaxf(m[h], x);
-      const float al = exp2f(m[h] - mn), p = exp2f(x - mn);
-      l[h] = fmaf(l[h], al, p);
+      for (int f = 0; f < 4; ++f) S = mfma16(ty, kf[f], qf[f], S);
+      float v[4], p[4], top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[h][i] = fmaf(o[h][i], al, p * kv[1][i]);
-      m[h] = mn;
+      for (int i = 0; i < 4; ++i) v[i] = t + 4 * j + i < end ? S[i] * a.scale : -INFINITY;
+      if (scored) stage_logits(t + 4 * j, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = v[i] * kLog2e;
+        top = fmaxf(top, p[i]);
+      }
+      raise_max(top);
+      const float neg = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(p[i] + neg);
+        l += p[i];
+      }
+      uint32_t pa[2];
+      split_p(ty, p, pa);
+      const uint4 pf = make_uint4(pa[0], pa[1], 0, 0);  // the upper four of the contraction's eight rows: none
+      const uint32_t r0[4] = {vf[0].x, vf[0].y, vf[0].z, vf[0].w}, r1[4] = {vf[1].x, vf[1].y, vf[1].z, vf[1].w};
+      const uint32_t r2[4] = {vf[2].x, vf[2].y, vf[2].z, vf[2].w}, r3[4] = {vf[3].x, vf[3].y, vf[3].z, vf[3].w};
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        acc[2 * d] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x05040100u),
+                                               __builtin_amdgcn_perm(r3[d], r2[d], 0x05040100u), 0, 0), acc[2 * d]);
+        acc[2 * d + 1] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x07060302u),
+                                                   __builtin_amdgcn_perm(r3[d], r2[d], 0x07060302u), 0, 0), acc[2 * d + 1]);
+      }
     }
   }
-  // the 32 row slots of the workgroup meet: maxima and sums in LDS, outputs over the wave's slots first
-#pragma unroll
-  for (int h = 0; h < kMaxGroup; ++h)
-    if (lane8 == 0) {
-      s_m[slot][h] = m[h];
-      s_l[slot][h] = l[h];
+
+  // ---- a scored split hands its logits over, then LDS changes hands
+  if (scored) {
+    __syncthreads();
+    const int nh = a.fold ? 1 : G;
+    for (int h = 0; h < nh; ++h) {
+      float* dst = a.logits + (int64_t)(b * a.logit_heads + g * nh + h) * a.logits_stride + begin;
+      const float* src = slog + h * a.split_rows;
+      for (int r = 4 * threadIdx.x; r < end - begin; r += 1024) {
+        const float4 v = *reinterpret_cast<const float4*>(src + r);
+        if (begin + r + 3 < end) {
+          *reinterpret_cast<float4*>(dst + r) = v;
+        } else {
+          dst[r] = v.x;
+          if (begin + r + 1 < end) dst[r + 1] = v.y;
+          if (begin + r + 2 < end) dst[r + 2] = v.z;
+        }
+      }
     }
-  __syncthreads();
-  float M[kMaxGroup];
+    __syncthreads();
+  }
+
+  // ---- the four waves meet
+  float* sm = lds;                   // [4][8] running maximum
+  float* sl = lds + 4 * kMaxGroup;   // [4][8] sum of exponentials
+  float* so = lds + 8 * kMaxGroup;   // [4][G][128]
+  l = rows_sum(l);
+  if (lane < kMaxGroup) {
+    sm[wave * kMaxGroup + lane] = m;
+    sl[wave * kMaxGroup + lane] = l;
+  }
 #pragma unroll
-  for (int h = 0; h < kMaxGroup; ++h) {
-    if (h >= G) break;
-    M[h] = -INFINITY;
-    for (int x = 0; x < 32; ++x) M[h] = fmaxf(M[h], s_m[x][h]);
-    const float f = m[h] == -INFINITY ? 0.f : exp2f(m[h] - M[h]);
+  for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = o[h][i] * f;
-      v += __shfl_xor(v, 8);
-      v += __shfl_xor(v, 16);
-      v += __shfl_xor(v, 32);
-      if ((threadIdx.x & 63) < 8) s_o[threadIdx.x >> 6][h][e0 + i] = v;
+    for (int i = 0; i < 4; ++i) {
+      auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[e][i]), __float_as_uint(acc[e][i]), false, false);
+      acc[e][i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int h = 4 * j + i;
+    if (j < 2 && h < G) {
+      float4* dst = reinterpret_cast<float4*>(so + (wave * G + h) * kD + 16 * m8 + 8 * hi8);
+      dst[0] = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
+      dst[1] = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < G * kD; i += 256) {
-    const int h = i / kD, d = i % kD;
-    float Mh = -INFINITY, den = 0.f;
-    for (int x = 0; x < 32; ++x) Mh = fmaxf(Mh, s_m[x][h]);
-    for (int x = 0; x < 32; ++x) den += s_m[x][h] == -INFINITY ? 0.f : s_l[x][h] * exp2f(s_m[x][h] - Mh);
-    const float num = s_o[0][h][d] + s_o[1][h][d] + s_o[2][h][d] + s_o[3][h][d];
+  for (int o = threadIdx.x; o < G * kD; o += 256) {
+    const int h = o / kD, d = o % kD;
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) M = fmaxf(M, sm[x * kMaxGroup + h]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float den = 0.f, num = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = __builtin_amdgcn_exp2f(sm[x * kMaxGroup + h] - Ms);
+      den = fmaf(sl[x * kMaxGroup + h], f, den);
+      num = fmaf(so[(x * G + h) * kD + d], f, num);
+    }
+    // den 0: no row took part (a NaN among the logits leaves NaN)
     const int64_t ph = (int64_t)(b * a.hq + g * G + h) * a.splits + split;
-    a.part_o[ph * kD + d] = Mh == -INFINITY ? 0.f : num / den;
-    if (d == 0) a.part_lse[ph] = Mh == -INFINITY ? -INFINITY : Mh + log2f(den);
+    a.part_o[ph * kD + d] = den == 0.f ? 0.f : num / den;
+    if (d == 0) a.part_lse[ph] = den == 0.f ? -INFINITY : Ms + log2f(den);
   }
 }
 
@@ -231,8 +646,8 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
   }
   for (int t = t0 + threadIdx.x; t < min(t0 + 1024, A); t += 256) {
     float acc = is_max ? -INFINITY : 0.f;
-    for (int h = 0; h < a.hq; ++h) {
-      const float v = a.logits[(int64_t)(b * a.hq + h) * a.logits_stride + t];
+    for (int h = 0; h < a.logit_heads; ++h) {
+      const float v = a.logits[(int64_t)(b * a.logit_heads + h) * a.logits_stride + t];
       const float x = soft ? exp2f(fmaf(v, kLog2e, -s_lse[h])) : v;
       acc = is_max ? fmaxf(acc, x) : acc + x;
     }
@@ -243,35 +658,57 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
 // ---------------------------------------------------------------- host side
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-static int kv8_plan(int batch, int hkv, int64_t rows, int max_score, int* split_rows) {
+// Rows per split: the chip holds two workgroups per CU (their registers allow two waves per SIMD); a scored split stages
+// its logits in LDS, up to 32 KB of them.
+static int kv8_plan(int batch, int hkv, int group, int64_t rows, bool scored, bool folded, int* split_rows) {
   const int64_t work = std::max<int64_t>(rows, 1) * hkv * batch;
   int64_t per = (work + 511) / 512;
-  per = std::max<int64_t>(64, (per + 63) / 64 * 64);
-  *split_rows = (int)std::min<int64_t>(per, 8192);
-  return (int)((rows + *split_rows - 1) / *split_rows) + (max_score > 0 ? 1 : 0);
+  per = std::max<int64_t>(128, (per + 63) / 64 * 64);
+  const int64_t most = scored ? 32768 / 4 / (folded ? 1 : group) / 64 * 64 : 8192;
+  *split_rows = (int)std::min(per, most);
+  return std::max(1, (int)((rows + *split_rows - 1) / *split_rows) + (scored ? 1 : 0));
 }
 
-static size_t kv8_workspace(int batch, int hq, int hkv, int64_t rows, int max_score, Kv8Attn* a, char* p) {
+// Carves the partial results; the bytes they take.  `folded` saves logits, never adds.
+static size_t kv8_workspace(int batch, int hq, int hkv, int64_t rows, int max_score, bool folded, Kv8Attn* a, char* p) {
   int C = 0;
-  const int S = std::max(1, kv8_plan(batch, hkv, rows, max_score, &C));
+  const bool scored = max_score > 0;
+  const int S = kv8_plan(batch, hkv, hq / hkv, rows, scored, folded, &C);
   const size_t o = align256((size_t)batch * hq * S * kD * 4), l = align256((size_t)batch * hq * S * 4);
   const size_t stride = ((size_t)max_score + 63) / 64 * 64;
-  const size_t g = max_score > 0 ? align256((size_t)batch * hq * stride * 4) : 0;
+  const int heads = folded ? hkv : hq;
+  const size_t g = scored ? align256((size_t)batch * heads * stride * 4) : 0;
   if (a) {
     p = (char*)align256((size_t)p);
     a->splits = S;
     a->split_rows = C;
     a->part_o = (float*)p;
     a->part_lse = (float*)(p + o);
-    a->logits = max_score > 0 ? (float*)(p + o + l) : nullptr;
+    a->logits = scored ? (float*)(p + o + l) : nullptr;
     a->logits_stride = (int64_t)stride;
+    a->logit_heads = heads;
   }
   return o + l + g + 256;
 }
 
+template <typename T, typename F, int MODE, bool LOGITS>
+static int launch_split(Kv8Attn& a, int batch, hipStream_t stream) {
+  size_t floats = 8 * kMaxGroup + (size_t)4 * a.group * kD;
+  if (LOGITS) floats = std::max(floats, (size_t)(a.fold ? 1 : a.group) * a.split_rows);
+  a.lds_scales = (int)floats;
+  if (MODE == kGather) floats += 256;
+  hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS>), dim3(a.c.num_kv_heads, a.splits, batch), dim3(256), floats * 4, stream, a);
+  return OKV_OK;
+}
+
 template <typename T, typename F>
-static int launch_kv8(const Kv8Attn& a, int batch, hipStream_t stream) {
-  hipLaunchKernelGGL((kv8_split<T, F>), dim3(a.c.num_kv_heads, a.splits, batch), dim3(256), 0, stream, a);
+static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
+  const bool paged = a.c.page_table != nullptr, scored = a.max_score_len > 0;
+  if (a.idx) launch_split<T, F, kGather, false>(a, batch, stream);
+  else if (paged && scored) launch_split<T, F, kPaged, true>(a, batch, stream);
+  else if (paged) launch_split<T, F, kPaged, false>(a, batch, stream);
+  else if (scored) launch_split<T, F, kContiguous, true>(a, batch, stream);
+  else launch_split<T, F, kContiguous, false>(a, batch, stream);
   hipLaunchKernelGGL(kv8_join<T>, dim3(a.hq + (a.max_score_len + 1023) / 1024, batch), dim3(256), 0, stream, a);
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;
@@ -286,9 +723,11 @@ static int kv8_attend(Kv8Attn& a, int64_t rows, int batch, void* ws, size_t ws_b
   OKV_REQUIRE(a.group <= kMaxGroup, OKV_ERR_UNSUPPORTED, "GQA group size %d not supported (1 to %d)", a.group, kMaxGroup);
   OKV_REQUIRE(a.hq <= kMaxHeads, OKV_ERR_UNSUPPORTED, "%d q heads not supported (at most %d)", a.hq, kMaxHeads);
   OKV_REQUIRE(batch <= 65535, OKV_ERR_UNSUPPORTED, "batch %d not supported", batch);
-  OKV_REQUIRE(rows < (1ll << 31), OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows);
+  OKV_REQUIRE(rows < (1ll << 30), OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows);
   OKV_REQUIRE(ws != nullptr, OKV_ERR_INVALID, "workspace pointer is NULL");
-  const size_t need = kv8_workspace(batch, a.hq, hkv, rows, a.max_score_len, &a, (char*)ws);
+  const bool folded = a.max_score_len > 0 && a.normalise == OKV_NORM_RAW;
+  if (folded) a.fold = a.head_reduce == OKV_REDUCE_MAX ? 1 : 2;
+  const size_t need = kv8_workspace(batch, a.hq, hkv, rows, a.max_score_len, folded, &a, (char*)ws);
   OKV_REQUIRE(ws_bytes >= need, OKV_ERR_WORKSPACE, "workspace too small: have %zu, need %zu", ws_bytes, need);
   OKV_REQUIRE(a.splits <= 65535, OKV_ERR_UNSUPPORTED, "%d splits", a.splits);
   if (a.c.dtype == OKV_BF16)
@@ -307,7 +746,7 @@ int okv_kv8_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_h
   OKV_REQUIRE(out_bytes != nullptr, OKV_ERR_INVALID, "NULL argument");
   OKV_REQUIRE(batch >= 1 && num_kv_heads >= 1 && num_q_heads >= num_kv_heads && max_rows >= 0 && max_score_len >= 0,
               OKV_ERR_INVALID, "bad batch, head counts or lengths");
-  *out_bytes = kv8_workspace(batch, num_q_heads, num_kv_heads, max_rows, max_score_len, nullptr, nullptr);
+  *out_bytes = kv8_workspace(batch, num_q_heads, num_kv_heads, max_rows, max_score_len, false, nullptr, nullptr);
   return OKV_OK;
 }
 
@@ -328,6 +767,11 @@ int okv_kv8_dense_attn(const void* q, int32_t num_q_heads, const okv_kv8_cache_t
   a.scale = scale;
   a.lens = seq_lens;
   a.max_len = max_seq_len;
+  a.late[0] = cache->open_k;
+  a.late[1] = cache->open_v;
+  a.late_token_stride = cache->open_token_stride;
+  a.late_head_stride = cache->open_head_stride;
+  a.late_batch_stride = cache->open_batch_stride;
   a.out = out;
   if (scores) {
     OKV_REQUIRE(max_score_len >= 0 && max_score_len <= max_seq_len, OKV_ERR_INVALID, "max_score_len out of range");
@@ -377,11 +821,11 @@ int okv_kv8_sparse_attn(const void* q, int32_t num_q_heads, const okv_kv8_cache_
   a.max_len = max_sel_len;
   a.idx = idx;
   a.idx_stride = idx_stride;
-  a.tail[0] = tail_k;
-  a.tail[1] = tail_v;
-  a.tail_token_stride = tail_token_stride;
-  a.tail_head_stride = tail_head_stride;
-  a.tail_batch_stride = tail_batch_stride;
+  a.late[0] = tail_k;
+  a.late[1] = tail_v;
+  a.late_token_stride = tail_token_stride;
+  a.late_head_stride = tail_head_stride;
+  a.late_batch_stride = tail_batch_stride;
   a.tail_lens = tail_lens;
   a.max_tail_len = max_tail_len;
   a.out = out;
