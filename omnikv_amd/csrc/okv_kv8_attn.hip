@@ -605,54 +605,133 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
   }
 }
 
-// Blocks [0, Hq) of a request join the splits of one q head; the others finish 1024 scores each, working out
-// the heads' normalisers themselves from the splits' partial log-sum-exps.
-template <typename T>
+// Blocks [0, Hq) of a request join the splits of one q head: 32 float4 columns x 8 split lanes, eight splits of a lane
+// in flight.  The other blocks finish 256 TPT scores each and work out the heads' normalisers themselves from the splits'
+// partial log-sum-exps (a few KB), so that no block waits for another.
+template <typename T, int TPT>
 __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
-  __shared__ float s_lse[kMaxHeads];
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, tid = threadIdx.x;
   const int main_len = clamp_len(a.lens, b, a.max_len);
   const int L = main_len + (a.max_tail_len ? clamp_len(a.tail_lens, b, a.max_tail_len) : 0);
   const int A = kv8_score_len(a, b, main_len);
+  constexpr int U = 8;
   if ((int)blockIdx.x < a.hq) {
-    const int h = blockIdx.x, d = threadIdx.x & (kD - 1), ns = rl_num_splits(a.split_rows, A, L);
+    __shared__ float4 s_num[8][32];
+    __shared__ float s_m[8], s_den[8];
+    const int h = blockIdx.x, dq = tid & 31, sl = tid >> 5, ns = rl_num_splits(a.split_rows, A, L);
     const float* lse = a.part_lse + (int64_t)(b * a.hq + h) * a.splits;
-    const float* po = a.part_o + (int64_t)(b * a.hq + h) * a.splits * kD + d;
-    float M = -INFINITY, den = 0.f, num = 0.f;
-    for (int s = 0; s < ns; ++s) {
-      const float x = lse[s];
-      if (x == -INFINITY) continue;
-      const float mn = fmaxf(M, x), f = exp2f(M - mn), e = exp2f(x - mn);
-      den = fmaf(den, f, e);
-      num = fmaf(num, f, e * po[(int64_t)s * kD]);
-      M = mn;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + (int64_t)(b * a.hq + h) * a.splits * kD) + dq;
+    float m = -INFINITY, den = 0.f;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = sl; s0 < ns; s0 += 8 * U) {
+      float x[U];
+      float4 o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + 8 * u;
+        x[u] = s < ns ? lse[s] : -INFINITY;
+        o[u] = s < ns ? po[(int64_t)s * (kD / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, x[u]);
+      const float ref = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - ref);
+      den *= al;
+      num = make_float4(num.x * al, num.y * al, num.z * al, num.w * al);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float f = __builtin_amdgcn_exp2f(x[u] - ref);
+        den += f;
+        num.x = fmaf(f, o[u].x, num.x);
+        num.y = fmaf(f, o[u].y, num.y);
+        num.z = fmaf(f, o[u].z, num.z);
+        num.w = fmaf(f, o[u].w, num.w);
+      }
+      m = mn;
     }
-    if (threadIdx.x < kD) store1(reinterpret_cast<T*>(a.out) + (int64_t)(b * a.hq + h) * kD + d, den == 0.f ? 0.f : num / den);
+    s_num[sl][dq] = num;
+    if (dq == 0) {
+      s_m[sl] = m;
+      s_den[sl] = den;
+    }
+    __syncthreads();
+    if (tid < kD) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) M = fmaxf(M, s_m[x]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      const float* sn = reinterpret_cast<const float*>(&s_num[0][0]);
+      float n = 0.f, d = 0.f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float f = __builtin_amdgcn_exp2f(s_m[x] - ref);
+        n = fmaf(sn[x * kD + tid], f, n);
+        d = fmaf(s_den[x], f, d);
+      }
+      store1(reinterpret_cast<T*>(a.out) + (int64_t)(b * a.hq + h) * kD + tid, d == 0.f ? 0.f : n / d);
+    }
     return;
   }
-  const int t0 = (blockIdx.x - a.hq) * 1024;
-  if (t0 >= A) return;
+  __shared__ float s_lse[kMaxHeads];
+  const int t0 = ((blockIdx.x - a.hq) * 256 + tid) * TPT;
+  if ((int)(blockIdx.x - a.hq) * 256 * TPT >= A) return;
   const bool soft = a.normalise == OKV_NORM_SOFTMAX, is_max = a.head_reduce == OKV_REDUCE_MAX;
-  if (soft) {
-    const int nA = (A + a.split_rows - 1) / a.split_rows;
-    for (int h = threadIdx.x; h < a.hq; h += 256) {
-      const float* lse = a.part_lse + (int64_t)(b * a.hq + h) * a.splits;
-      float M = -INFINITY, den = 0.f;
-      for (int s = 0; s < nA; ++s) M = fmaxf(M, lse[s]);
-      for (int s = 0; s < nA; ++s) den += lse[s] == -INFINITY ? 0.f : exp2f(lse[s] - M);
-      s_lse[h] = M == -INFINITY ? 0.f : M + log2f(den);
+  if (soft) {  // eight threads per head
+    const int nA = (A + a.split_rows - 1) / a.split_rows, sub = tid & 7;
+    for (int h0 = 0; h0 < a.hq; h0 += 32) {
+      const int h = h0 + (tid >> 3);
+      float m = -INFINITY, den = 0.f;
+      if (h < a.hq) {
+        const float* lse = a.part_lse + (int64_t)(b * a.hq + h) * a.splits;
+        for (int s0 = sub; s0 < nA; s0 += 8 * U) {
+          float x[U], mn = m;
+#pragma unroll
+          for (int u = 0; u < U; ++u) x[u] = s0 + 8 * u < nA ? lse[s0 + 8 * u] : -INFINITY;
+#pragma unroll
+          for (int u = 0; u < U; ++u) mn = fmaxf(mn, x[u]);
+          const float ref = mn == -INFINITY ? 0.f : mn;
+          den *= __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+          for (int u = 0; u < U; ++u) den += __builtin_amdgcn_exp2f(x[u] - ref);
+          m = mn;
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        const float m2 = __shfl_xor(m, o), d2 = __shfl_xor(den, o), mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+        den = den * __builtin_amdgcn_exp2f(m - ref) + d2 * __builtin_amdgcn_exp2f(m2 - ref);
+        m = mn;
+      }
+      if (h < a.hq && sub == 0) s_lse[h] = m == -INFINITY ? 0.f : m + log2f(den);
     }
     __syncthreads();
   }
-  for (int t = t0 + threadIdx.x; t < min(t0 + 1024, A); t += 256) {
-    float acc = is_max ? -INFINITY : 0.f;
-    for (int h = 0; h < a.logit_heads; ++h) {
-      const float v = a.logits[(int64_t)(b * a.logit_heads + h) * a.logits_stride + t];
-      const float x = soft ? exp2f(fmaf(v, kLog2e, -s_lse[h])) : v;
-      acc = is_max ? fmaxf(acc, x) : acc + x;
+  if (t0 >= A) return;
+  float acc[TPT];
+#pragma unroll
+  for (int i = 0; i < TPT; ++i) acc[i] = is_max ? -INFINITY : 0.f;
+  const float* lg = a.logits + (int64_t)b * a.logit_heads * a.logits_stride + t0;
+#pragma unroll 16
+  for (int h = 0; h < a.logit_heads; ++h) {
+    float v[TPT];  // the row ends at a multiple of 64: reading past A stays inside it
+    if constexpr (TPT == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(lg + (int64_t)h * a.logits_stride);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(lg + (int64_t)h * a.logits_stride);
+      v[0] = x.x; v[1] = x.y;
     }
-    a.scores[(int64_t)b * a.score_stride + t] = acc;
+    const float lse = soft ? s_lse[h] : 0.f;
+#pragma unroll
+    for (int i = 0; i < TPT; ++i) {
+      const float x = soft ? __builtin_amdgcn_exp2f(fmaf(v[i], kLog2e, -lse)) : v[i];
+      acc[i] = is_max ? fmaxf(acc[i], x) : acc[i] + x;
+    }
   }
+  float* sp = a.scores + (int64_t)b * a.score_stride + t0;
+#pragma unroll
+  for (int i = 0; i < TPT; ++i)
+    if (t0 + i < A) sp[i] = acc[i];
 }
 
 // ---------------------------------------------------------------- host side
@@ -709,7 +788,11 @@ static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
   else if (paged) launch_split<T, F, kPaged, false>(a, batch, stream);
   else if (scored) launch_split<T, F, kContiguous, true>(a, batch, stream);
   else launch_split<T, F, kContiguous, false>(a, batch, stream);
-  hipLaunchKernelGGL(kv8_join<T>, dim3(a.hq + (a.max_score_len + 1023) / 1024, batch), dim3(256), 0, stream, a);
+  // blocks of 512 scores put more CUs to pulling the logits, but each works out the normalisers anew
+  const int tokens = finish_tokens_for(a.split_rows, a.max_score_len);
+  const dim3 grid(a.hq + (a.max_score_len + tokens - 1) / tokens, batch);
+  if (tokens == 512) hipLaunchKernelGGL((kv8_join<T, 2>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((kv8_join<T, 4>), grid, dim3(256), 0, stream, a);
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;
 }
