@@ -14,6 +14,7 @@ namespace okv {
 
 constexpr int kMaxGroup = 8;
 constexpr int kMaxHeads = 256;
+constexpr int kGatherResident = 3;  // workgroups of the gather mode that a CU holds (160 VGPRs; capped for four it spills: 19.4 against 13.2 us at 8781 rows)
 
 struct Kv8Attn {
   okv_kv8_cache_t c;
@@ -33,14 +34,18 @@ struct Kv8Attn {
   const int32_t* score_lens;
   int32_t max_score_len;
   // partial results
-  float* part_o;    // [batch][Hq][splits][128]
-  float* part_lse;  // [batch][Hq][splits], log2 domain; -inf: no row took part
-  float* logits;    // [batch][Hq][logits_stride], natural units
+  float* part_o;    // [shares][Hq][128]
+  float* part_lse;  // [shares][Hq], log2 domain; -inf: no row took part
+  float* logits;    // [batch][logit_heads][logits_stride], natural units
   int64_t logits_stride;
-  int32_t splits, split_rows;
+  int32_t batch;
+  int32_t target;     // shares the rows of the call are cut into, about
+  int32_t most_rows;  // of a share (its logits are staged in LDS)
+  int32_t items;      // shares the grid and the partial results have room for
   int32_t fold;         // raw scores: the q heads of a kv head are folded by the split (1 max, 2 sum): one logits row per kv head
   int32_t logit_heads;  // rows of `logits` per request
   int32_t lds_scales;   // floats before the scale staging of the gather mode
+  int32_t page_shift, block_shift;  // log2; page_shift -1: the page size is no power of two
   // outputs
   void* out;
   float* scores;
@@ -55,6 +60,89 @@ __device__ __forceinline__ int clamp_len(const int32_t* lens, int b, int most) {
 __device__ __forceinline__ int kv8_score_len(const Kv8Attn& a, int b, int len) {
   const int s = a.max_score_len ? clamp_len(a.score_lens, b, a.max_score_len) : 0;
   return s < len ? s : len;
+}
+
+// ---------------------------------------------------------------- shares
+// The rows of all requests are cut into shares of equal length, worked out on the device from the lengths as they are: a
+// ragged batch, or a length far below its bound, leaves no workgroup idle.  Every wave that needs the
+// cut works it out by itself (a lane per request), so nothing waits for it.
+struct Share {
+  int b;       // request
+  int L, A;    // its rows, and how many of them are scored
+  int main_len;
+  int rows;    // rows of a share
+  int index;   // this share among the request's
+  int first;   // the request's first share among all
+  int count;   // shares of the request
+};
+
+constexpr int kLeastRows = 128;  // one 32-row tile per wave
+
+// inclusive prefix sum over the wave
+__device__ __forceinline__ int lane_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of a row to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+  return x;
+}
+__device__ __forceinline__ int share_rows(int total, const Kv8Attn& a) {
+  const uint32_t r = (((uint32_t)total + a.target - 1) / (uint32_t)a.target + 63) & ~63u;
+  return r < kLeastRows ? kLeastRows : r > (uint32_t)a.most_rows ? a.most_rows : (int)r;
+}
+__device__ __forceinline__ void request_lens(const Kv8Attn& a, int b, int* main_len, int* L, int* A) {
+  *main_len = clamp_len(a.lens, b, a.max_len);
+  *L = *main_len + (a.max_tail_len ? clamp_len(a.tail_lens, b, a.max_tail_len) : 0);
+  *A = kv8_score_len(a, b, *main_len);
+}
+
+// The share `item` (false: there is none), or with item < 0 the shares of request `request`.
+__device__ __forceinline__ bool find_share(const Kv8Attn& a, int item, int request, Share* s) {
+  const int lane = threadIdx.x & 63;
+  if (a.batch == 1) {
+    request_lens(a, 0, &s->main_len, &s->L, &s->A);
+    s->main_len = __builtin_amdgcn_readfirstlane(s->main_len);
+    s->L = __builtin_amdgcn_readfirstlane(s->L);
+    s->A = __builtin_amdgcn_readfirstlane(s->A);
+    s->rows = __builtin_amdgcn_readfirstlane(share_rows(s->L, a));
+    s->b = 0;
+    s->first = 0;
+    s->index = item;
+    s->count = rl_num_splits(s->rows, s->A, s->L);
+    return item < s->count;
+  }
+  int main_len = 0, L = 0, A = 0, total = 0;
+  for (int base = 0; base < a.batch; base += 64) {
+    main_len = L = A = 0;
+    if (base + lane < a.batch) request_lens(a, base + lane, &main_len, &L, &A);
+    total += __builtin_amdgcn_readlane(lane_scan(L), 63);
+  }
+  s->rows = __builtin_amdgcn_readfirstlane(share_rows(total, a));
+  int before = 0;
+  for (int base = 0; base < a.batch; base += 64) {
+    if (a.batch > 64) {
+      main_len = L = A = 0;
+      if (base + lane < a.batch) request_lens(a, base + lane, &main_len, &L, &A);
+    }
+    const int n = rl_num_splits(s->rows, A, L);
+    const int x = lane_scan(n);
+    const uint64_t hit = __ballot(item >= 0 ? before + x > item : base + lane == request);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      s->b = base + at;
+      s->main_len = __builtin_amdgcn_readlane(main_len, at);
+      s->L = __builtin_amdgcn_readlane(L, at);
+      s->A = __builtin_amdgcn_readlane(A, at);
+      s->count = __builtin_amdgcn_readlane(n, at);
+      s->first = before + __builtin_amdgcn_readlane(x, at) - s->count;
+      s->index = item - s->first;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(x, 63);
+  }
+  return false;
 }
 
 // ---------------------------------------------------------------- matrix-core pieces
@@ -143,18 +231,21 @@ struct Kv8Rows {
 // eight elements, turned by byte permutes as they are decoded.
 // Scales of K are applied to the fp32 logits.  One running maximum per q head and wave; the waves meet in LDS.
 template <typename T, typename F, int MODE, bool LOGITS>
-__global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
+__global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv8_split(Kv8Attn a) {
   extern __shared__ float lds[];
   const okv_kv8_cache_t& c = a.c;
-  const int g = blockIdx.x, split = blockIdx.y, b = blockIdx.z, G = a.group;
-  const int main_len = clamp_len(a.lens, b, a.max_len);
-  const int L = main_len + (a.max_tail_len ? clamp_len(a.tail_lens, b, a.max_tail_len) : 0);
-  const int A = LOGITS ? kv8_score_len(a, b, main_len) : 0;
+  const int G = a.group;
+  // workgroups go to the XCDs round-robin: the kv heads of a share run on one XCD, one after the other, so that rows
+  // stored head by head next to each other (pools) are fetched together
+  const int turn = blockIdx.x >> 3, g = turn % c.num_kv_heads;
+  Share sh;
+  if (!find_share(a, (int)((turn / c.num_kv_heads) * 8 + (blockIdx.x & 7)), 0, &sh)) return;
+  const int b = sh.b, main_len = sh.main_len, L = sh.L, A = LOGITS ? sh.A : 0;
   int begin, end;
-  rl_split_range(split, a.split_rows, A, L, &begin, &end);
+  rl_split_range(sh.index, sh.rows, A, L, &begin, &end);
   if (begin >= end) return;
   // rows [0, closed) are codes, the rest 16-bit rows: the open block, or the tail
-  const int closed = a.sparse || !c.open_k ? main_len : main_len / c.block_tokens * c.block_tokens;
+  const int closed = a.sparse || !c.open_k ? main_len : main_len >> a.block_shift << a.block_shift;
   const int main_end = min(end, closed);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -183,11 +274,13 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
   const int32_t* idx = a.idx + (int64_t)b * a.idx_stride;
   const uint32_t room = MODE != kGather ? 0 : a.slots ? (uint32_t)(c.num_pages * c.page_size) : (uint32_t)kv8_room(c);
 
+  auto page_of = [&](int t) -> int { return a.page_shift >= 0 ? t >> a.page_shift : t / c.page_size; };
+  auto slot_of = [&](int t) -> int { return a.page_shift >= 0 ? t & (c.page_size - 1) : t % c.page_size; };
   // ---- what has to be known of a tile's rows before they can be addressed
   auto rows_of = [&](int t, Kv8Rows& r) {
     if (MODE == kPaged) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) r.page[s] = table[min(t + 16 * s, last) / c.page_size];
+      for (int s = 0; s < 2; ++s) r.page[s] = table[page_of(min(t + 16 * s, last))];
     } else if (MODE == kGather) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -212,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
         x.k[i] = load_stream16(kb + (int64_t)t * ts + (uint32_t)rk * ts + kcol);
         x.v[i] = load_stream16(vb + (int64_t)t * ts + (uint32_t)rv * ts + vcol);
       }
-      const int blk = min(t + 16 * (j & 1), last) / c.block_tokens;
+      const int blk = min(t + 16 * (j & 1), last) >> a.block_shift;
       x.sc = (j < 2 ? ksb : vsb)[(int64_t)blk * c.scale_block_stride];
       x.ok = 3;
     } else if (MODE == kPaged) {
@@ -224,9 +317,9 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
         const int u = min(t + 16 * s, last) & ~15;
         const bool in = (uint32_t)r.page[s] < (uint32_t)c.num_pages;
         const int64_t p = in ? r.page[s] : 0;
-        const int slot = u % c.page_size;
+        const int slot = slot_of(u);
         base[s] = p * c.page_stride + (int64_t)slot * ts;
-        const int64_t sb = p * c.scale_page_stride + (int64_t)(slot / c.block_tokens) * c.scale_block_stride;
+        const int64_t sb = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride;
         if ((j & 1) == s) sbase = sb;
         x.ok |= in ? 1u << s : 0u;
       }
@@ -245,14 +338,14 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
         bool in = (uint32_t)t_ < room;
         const int tt = in ? t_ : 0;
         if (c.page_table && !a.slots) {
-          const int pg = table[tt / c.page_size], slot = tt % c.page_size;
+          const int pg = table[page_of(tt)], slot = slot_of(tt);
           in = in && (uint32_t)pg < (uint32_t)c.num_pages;
           const int64_t p = (uint32_t)pg < (uint32_t)c.num_pages ? pg : 0;
           *row = p * c.page_stride + (int64_t)slot * ts;
-          *scale = p * c.scale_page_stride + (int64_t)(slot / c.block_tokens) * c.scale_block_stride;
+          *scale = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride;
         } else {
           *row = (int64_t)tt * ts;
-          *scale = (int64_t)(tt / c.block_tokens) * c.scale_block_stride;
+          *scale = (int64_t)(tt >> a.block_shift) * c.scale_block_stride;
         }
         return in;
       };
@@ -312,7 +405,7 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
       }
     }
     if (m16 < (a.fold ? 1 : G))
-      *reinterpret_cast<float4*>(slog + m16 * a.split_rows + (row - begin)) = make_float4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<float4*>(slog + m16 * sh.rows + (row - begin)) = make_float4(o[0], o[1], o[2], o[3]);
   };
   // a probability in two 16-bit parts: this lane's part of four of them
   auto split_p = [&](auto* ty, const float (&p)[4], uint32_t* out) {
@@ -465,7 +558,13 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
       Kv8Rows r0, r1;
       Kv8Tile x0, x1;
       rows_of(t, r0);
-      if (t == t_last) {
+      if (MODE == kGather) {
+        for (; t <= t_last; t += 128) {
+          load(t, r0, x0);
+          rows_of(min(t + 128, t_last), r0);
+          compute(t, x0, sstage);
+        }
+      } else if (t == t_last) {
         load(t, r0, x0);
         compute(t, x0, sstage);
       } else {
@@ -544,7 +643,7 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
     const int nh = a.fold ? 1 : G;
     for (int h = 0; h < nh; ++h) {
       float* dst = a.logits + (int64_t)(b * a.logit_heads + g * nh + h) * a.logits_stride + begin;
-      const float* src = slog + h * a.split_rows;
+      const float* src = slog + h * sh.rows;
       for (int r = 4 * threadIdx.x; r < end - begin; r += 1024) {
         const float4 v = *reinterpret_cast<const float4*>(src + r);
         if (begin + r + 3 < end) {
@@ -599,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
       num = fmaf(so[(x * G + h) * kD + d], f, num);
     }
     // den 0: no row took part (a NaN among the logits leaves NaN)
-    const int64_t ph = (int64_t)(b * a.hq + g * G + h) * a.splits + split;
+    const int64_t ph = (int64_t)(sh.first + sh.index) * a.hq + g * G + h;
     a.part_o[ph * kD + d] = den == 0.f ? 0.f : num / den;
     if (d == 0) a.part_lse[ph] = den == 0.f ? -INFINITY : Ms + log2f(den);
   }
@@ -611,16 +710,16 @@ __global__ __launch_bounds__(256, 2) void kv8_split(Kv8Attn a) {
 template <typename T, int TPT>
 __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int main_len = clamp_len(a.lens, b, a.max_len);
-  const int L = main_len + (a.max_tail_len ? clamp_len(a.tail_lens, b, a.max_tail_len) : 0);
-  const int A = kv8_score_len(a, b, main_len);
+  Share sh;
+  find_share(a, -1, b, &sh);
+  const int A = sh.A;
   constexpr int U = 8;
   if ((int)blockIdx.x < a.hq) {
     __shared__ float4 s_num[8][32];
     __shared__ float s_m[8], s_den[8];
-    const int h = blockIdx.x, dq = tid & 31, sl = tid >> 5, ns = rl_num_splits(a.split_rows, A, L);
-    const float* lse = a.part_lse + (int64_t)(b * a.hq + h) * a.splits;
-    const float4* po = reinterpret_cast<const float4*>(a.part_o + (int64_t)(b * a.hq + h) * a.splits * kD) + dq;
+    const int h = blockIdx.x, dq = tid & 31, sl = tid >> 5, ns = sh.count;
+    const float* lse = a.part_lse + (int64_t)sh.first * a.hq + h;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + ((int64_t)sh.first * a.hq + h) * kD) + dq;
     float m = -INFINITY, den = 0.f;
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s0 = sl; s0 < ns; s0 += 8 * U) {
@@ -629,8 +728,8 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int s = s0 + 8 * u;
-        x[u] = s < ns ? lse[s] : -INFINITY;
-        o[u] = s < ns ? po[(int64_t)s * (kD / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[u] = s < ns ? lse[(int64_t)s * a.hq] : -INFINITY;
+        o[u] = s < ns ? po[(int64_t)s * a.hq * (kD / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float mn = m;
 #pragma unroll
@@ -677,16 +776,16 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
   if ((int)(blockIdx.x - a.hq) * 256 * TPT >= A) return;
   const bool soft = a.normalise == OKV_NORM_SOFTMAX, is_max = a.head_reduce == OKV_REDUCE_MAX;
   if (soft) {  // eight threads per head
-    const int nA = (A + a.split_rows - 1) / a.split_rows, sub = tid & 7;
+    const int nA = (A + sh.rows - 1) / sh.rows, sub = tid & 7;
     for (int h0 = 0; h0 < a.hq; h0 += 32) {
       const int h = h0 + (tid >> 3);
       float m = -INFINITY, den = 0.f;
       if (h < a.hq) {
-        const float* lse = a.part_lse + (int64_t)(b * a.hq + h) * a.splits;
+        const float* lse = a.part_lse + (int64_t)sh.first * a.hq + h;
         for (int s0 = sub; s0 < nA; s0 += 8 * U) {
           float x[U], mn = m;
 #pragma unroll
-          for (int u = 0; u < U; ++u) x[u] = s0 + 8 * u < nA ? lse[s0 + 8 * u] : -INFINITY;
+          for (int u = 0; u < U; ++u) x[u] = s0 + 8 * u < nA ? lse[(int64_t)(s0 + 8 * u) * a.hq] : -INFINITY;
 #pragma unroll
           for (int u = 0; u < U; ++u) mn = fmaxf(mn, x[u]);
           const float ref = mn == -INFINITY ? 0.f : mn;
@@ -737,33 +836,35 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
 // ---------------------------------------------------------------- host side
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Rows per split: the chip holds two workgroups per CU (their registers allow two waves per SIMD); a scored split stages
-// its logits in LDS, up to 32 KB of them.
-static int kv8_plan(int batch, int hkv, int group, int64_t rows, bool scored, bool folded, int* split_rows) {
-  const int64_t work = std::max<int64_t>(rows, 1) * hkv * batch;
-  int64_t per = (work + 511) / 512;
-  per = std::max<int64_t>(128, (per + 63) / 64 * 64);
-  const int64_t most = scored ? 32768 / 4 / (folded ? 1 : group) / 64 * 64 : 8192;
-  *split_rows = (int)std::min(per, most);
-  return std::max(1, (int)((rows + *split_rows - 1) / *split_rows) + (scored ? 1 : 0));
+// How many shares to cut the rows into.  The chip holds two workgroups per CU (their registers allow two waves per SIMD),
+// three of the gather mode.  One request: one round of them.  A batch: three rounds, since each request ends in a share
+// cut short (sixteen requests of 8K..32K tokens: 136 us with one round, 124 / 121 / 122 / 127 / 136 with 2 / 3 / 4 / 6 / 8).
+// A scored share stages its logits in LDS, up to 32 KB of them.
+static void kv8_cut(bool gather, int batch, int hkv, int group, int64_t rows, int max_score, bool folded, int* target, int* most, int* items) {
+  *target = std::max(1, (gather ? 256 * kGatherResident : 512 * (batch > 1 ? 3 : 1)) / hkv);
+  *most = max_score > 0 ? 32768 / 4 / (folded ? 1 : group) / 64 * 64 : 8192;
+  const int64_t all = std::max<int64_t>(rows, 1) * batch;
+  const int64_t n = std::min((all + kLeastRows - 1) / kLeastRows, std::max<int64_t>(*target, (all + *most - 1) / *most));
+  *items = (int)std::min<int64_t>(n + (int64_t)batch * (max_score > 0 ? 2 : 1), 1 << 30);
 }
 
 // Carves the partial results; the bytes they take.  `folded` saves logits, never adds.
-static size_t kv8_workspace(int batch, int hq, int hkv, int64_t rows, int max_score, bool folded, Kv8Attn* a, char* p) {
-  int C = 0;
-  const bool scored = max_score > 0;
-  const int S = kv8_plan(batch, hkv, hq / hkv, rows, scored, folded, &C);
-  const size_t o = align256((size_t)batch * hq * S * kD * 4), l = align256((size_t)batch * hq * S * 4);
+static size_t kv8_workspace(bool gather, int batch, int hq, int hkv, int64_t rows, int max_score, bool folded, Kv8Attn* a, char* p) {
+  int target, most, items;
+  kv8_cut(gather, batch, hkv, hq / hkv, rows, max_score, folded, &target, &most, &items);
+  const size_t o = align256((size_t)items * hq * kD * 4), l = align256((size_t)items * hq * 4);
   const size_t stride = ((size_t)max_score + 63) / 64 * 64;
   const int heads = folded ? hkv : hq;
-  const size_t g = scored ? align256((size_t)batch * heads * stride * 4) : 0;
+  const size_t g = max_score > 0 ? align256((size_t)batch * heads * stride * 4) : 0;
   if (a) {
     p = (char*)align256((size_t)p);
-    a->splits = S;
-    a->split_rows = C;
+    a->batch = batch;
+    a->target = target;
+    a->most_rows = most;
+    a->items = items;
     a->part_o = (float*)p;
     a->part_lse = (float*)(p + o);
-    a->logits = scored ? (float*)(p + o + l) : nullptr;
+    a->logits = max_score > 0 ? (float*)(p + o + l) : nullptr;
     a->logits_stride = (int64_t)stride;
     a->logit_heads = heads;
   }
@@ -773,10 +874,10 @@ static size_t kv8_workspace(int batch, int hq, int hkv, int64_t rows, int max_sc
 template <typename T, typename F, int MODE, bool LOGITS>
 static int launch_split(Kv8Attn& a, int batch, hipStream_t stream) {
   size_t floats = 8 * kMaxGroup + (size_t)4 * a.group * kD;
-  if (LOGITS) floats = std::max(floats, (size_t)(a.fold ? 1 : a.group) * a.split_rows);
+  if (LOGITS) floats = std::max(floats, (size_t)(a.fold ? 1 : a.group) * a.most_rows);
   a.lds_scales = (int)floats;
   if (MODE == kGather) floats += 256;
-  hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS>), dim3(a.c.num_kv_heads, a.splits, batch), dim3(256), floats * 4, stream, a);
+  hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS>), dim3((a.items + 7) / 8 * 8 * a.c.num_kv_heads), dim3(256), floats * 4, stream, a);
   return OKV_OK;
 }
 
@@ -789,7 +890,8 @@ static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
   else if (scored) launch_split<T, F, kContiguous, true>(a, batch, stream);
   else launch_split<T, F, kContiguous, false>(a, batch, stream);
   // blocks of 512 scores put more CUs to pulling the logits, but each works out the normalisers anew
-  const int tokens = finish_tokens_for(a.split_rows, a.max_score_len);
+  const int64_t shares = a.items / a.batch;
+  const int tokens = shares * ((a.max_score_len + 511) / 512) <= 65536 ? 512 : 1024;
   const dim3 grid(a.hq + (a.max_score_len + tokens - 1) / tokens, batch);
   if (tokens == 512) hipLaunchKernelGGL((kv8_join<T, 2>), grid, dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((kv8_join<T, 4>), grid, dim3(256), 0, stream, a);
@@ -803,16 +905,18 @@ static int kv8_attend(Kv8Attn& a, int64_t rows, int batch, void* ws, size_t ws_b
   OKV_REQUIRE(((uintptr_t)a.q & 15) == 0, OKV_ERR_INVALID, "q must be 16-byte aligned");
   OKV_REQUIRE(a.hq >= hkv && a.hq % hkv == 0, OKV_ERR_INVALID, "bad head counts q=%d kv=%d", a.hq, hkv);
   a.group = a.hq / hkv;
+  a.block_shift = __builtin_ctz(a.c.block_tokens);
+  a.page_shift = a.c.page_table && (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz(a.c.page_size) : -1;
   OKV_REQUIRE(a.group <= kMaxGroup, OKV_ERR_UNSUPPORTED, "GQA group size %d not supported (1 to %d)", a.group, kMaxGroup);
   OKV_REQUIRE(a.hq <= kMaxHeads, OKV_ERR_UNSUPPORTED, "%d q heads not supported (at most %d)", a.hq, kMaxHeads);
   OKV_REQUIRE(batch <= 65535, OKV_ERR_UNSUPPORTED, "batch %d not supported", batch);
-  OKV_REQUIRE(rows < (1ll << 30), OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows);
+  OKV_REQUIRE(rows * batch < (1ll << 31), OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
   OKV_REQUIRE(ws != nullptr, OKV_ERR_INVALID, "workspace pointer is NULL");
   const bool folded = a.max_score_len > 0 && a.normalise == OKV_NORM_RAW;
   if (folded) a.fold = a.head_reduce == OKV_REDUCE_MAX ? 1 : 2;
-  const size_t need = kv8_workspace(batch, a.hq, hkv, rows, a.max_score_len, folded, &a, (char*)ws);
+  const size_t need = kv8_workspace(a.idx != nullptr, batch, a.hq, hkv, rows, a.max_score_len, folded, &a, (char*)ws);
   OKV_REQUIRE(ws_bytes >= need, OKV_ERR_WORKSPACE, "workspace too small: have %zu, need %zu", ws_bytes, need);
-  OKV_REQUIRE(a.splits <= 65535, OKV_ERR_UNSUPPORTED, "%d splits", a.splits);
+  OKV_REQUIRE((int64_t)(a.items + 7) * hkv < (1ll << 31), OKV_ERR_UNSUPPORTED, "%d requests of up to %lld rows", batch, (long long)rows);
   if (a.c.dtype == OKV_BF16)
     return a.c.format == OKV_E4M3 ? launch_kv8<BF16, E4M3>(a, batch, stream) : launch_kv8<BF16, I8>(a, batch, stream);
   return a.c.format == OKV_E4M3 ? launch_kv8<F16, E4M3>(a, batch, stream) : launch_kv8<F16, I8>(a, batch, stream);
@@ -829,7 +933,9 @@ int okv_kv8_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_h
   OKV_REQUIRE(out_bytes != nullptr, OKV_ERR_INVALID, "NULL argument");
   OKV_REQUIRE(batch >= 1 && num_kv_heads >= 1 && num_q_heads >= num_kv_heads && max_rows >= 0 && max_score_len >= 0,
               OKV_ERR_INVALID, "bad batch, head counts or lengths");
-  *out_bytes = kv8_workspace(batch, num_q_heads, num_kv_heads, max_rows, max_score_len, false, nullptr, nullptr);
+  // whichever way the rows are found
+  *out_bytes = std::max(kv8_workspace(false, batch, num_q_heads, num_kv_heads, max_rows, max_score_len, false, nullptr, nullptr),
+                        kv8_workspace(true, batch, num_q_heads, num_kv_heads, max_rows, max_score_len, false, nullptr, nullptr));
   return OKV_OK;
 }
 
