@@ -484,13 +484,14 @@ int okv_kv8_read(const okv_kv8_cache_t* cache, const int32_t* idx, int64_t idx_s
  * on `stream`, so a step of page operations can be captured in a HIP graph.  The pool's data are
  * `buffers`: for every layer's K, V and scales one array of num_pages pages, page p at base +
  * p*page_bytes (base and page_bytes multiples of 4; of 16 for speed), listed in HOST memory.  Pages
- * are handed out lowest first, in the order of the call's entries, so results are reproducible.
+ * are handed out lowest first, in the order of the call's entries, so results are reproducible.  Fork and extend
+ * take at most 1024 entries in one call.
  *
  * status (device int32[2], may be NULL): [0] pages the pool was short of -- then the call changed
  * nothing --, [1] entries that were refused and skipped.  Entries refused: sequence numbers
  * outside [0, num_seqs); a number that an earlier entry of the call named (children in fork,
- * sequences in free and extend); a fork into a row that is not empty or is its own parent; growth
- * beyond max_pages.
+ * sequences in extend); a fork into a row that is not empty or is its own parent; growth
+ * beyond max_pages.  (Freeing a sequence twice in one call, or one that is empty, is no refusal.)
  * No counterpart in the reference's path, which keeps one request (its serving stack's token
  * slots are managed on the host, common/mem_manager.py).
  */
@@ -521,7 +522,7 @@ int okv_pages_fork(const okv_page_pool_t* pool, const int32_t* parents, const in
 /* Room for more[i] more tokens (negative: none) in sequence seqs[i]: its length grows by it and the pages it
  * lacks are taken from the free ones. */
 int okv_pages_extend(const okv_page_pool_t* pool, const int32_t* seqs, const int32_t* more, int32_t n,
-                     int32_t* status, void* ws, size_t ws_bytes, okv_stream_t stream);
+                     int32_t* status, okv_stream_t stream);
 
 /* Pages dst[i] = pages src[i] of every buffer, i < count[0] (device) or n when count is NULL.
  * No page may be both a source and a destination, and the destinations are distinct; page numbers

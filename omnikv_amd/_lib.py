@@ -211,7 +211,7 @@ def _declare(l):
                                  vp]),
         ("okv_pages_free", [pool, vp, i32, vp, vp]),
         ("okv_pages_fork", [pool, vp, vp, i32, bufs, i32, vp, vp, sz, vp]),
-        ("okv_pages_extend", [pool, vp, vp, i32, vp, vp, sz, vp]),
+        ("okv_pages_extend", [pool, vp, vp, i32, vp, vp]),
         ("okv_pages_copy", [bufs, i32, i32, vp, vp, vp, i32, vp]),
         ("okv_pages_compact", [pool, vp, i64, vp, vp, bufs, i32, vp, sz, vp]),
         ("okv_pages_workspace_bytes", [pool, i32, C.POINTER(sz)]),

@@ -8,6 +8,9 @@ namespace okv {
 
 constexpr int kBuffersPerLaunch = 128;
 constexpr int kPlanThreads = 1024;
+constexpr int kMaxEntries = kPlanThreads;  // entries of a call: one per thread of the plan
+constexpr int kPerThread = 4;              // pages of a plan's trip through the counts, per thread
+constexpr int kTrip = kPlanThreads * kPerThread;
 
 struct BufferList {
   okv_page_buffer_t b[kBuffersPerLaunch];
@@ -17,56 +20,85 @@ __device__ __forceinline__ int pages_of(int64_t tokens, int page_size) {
   return (int)((tokens + page_size - 1) / page_size);
 }
 
-// inclusive prefix sum over the 1024 threads of a plan; total: of all
-__device__ __forceinline__ int block_scan(int v, int* total) {
-  __shared__ int s_wave[kPlanThreads / 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();  // the last scan's sums have been read
-  if (lane == 63) s_wave[wave] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w < wave) before += s_wave[w];
-    all += s_wave[w];
-  }
-  *total = all;
-  return x + before;
+__device__ __forceinline__ int wave_scan(int x) {  // inclusive prefix sum over the wave
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of a row to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+  return x;
 }
 
-// Scratch of a plan, shared through the second-level cache: every cell is written and read with device-scope
-// accesses, since atomics pass the first level by.
-__device__ __forceinline__ int get(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void put(int32_t* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// Exclusive prefix sum over the threads of a plan, and the sum of all.  `turn` counts the calls: two sets of cells in
+// turn, so that one barrier per call is enough.
+__device__ __forceinline__ int block_scan(int v, int* total, int& turn) {
+  constexpr int W = kPlanThreads / 64;
+  __shared__ int s_wave[2][W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int x = wave_scan(v);
+  int* cells = s_wave[turn & 1];
+  ++turn;
+  if (lane == 63) cells[wave] = x;
+  __syncthreads();
+  const int sums = wave_scan(lane < W ? cells[lane] : 0);  // the waves' sums, by every wave
+  *total = __builtin_amdgcn_readlane(sums, W - 1);
+  return x - v + (wave ? __builtin_amdgcn_readlane(sums, __builtin_amdgcn_readfirstlane(wave) - 1) : 0);
+}
+
+// The counts of a trip's pages, four per thread in order; 1 behind the last page (in use).
+__device__ __forceinline__ int4 load_refs(const okv_page_pool_t& p, int base) {
+  const int id = base + kPerThread * (int)threadIdx.x;
+  if (id + 3 < p.num_pages && ((uintptr_t)p.refs & 15) == 0) return *reinterpret_cast<const int4*>(p.refs + id);
+  int4 r = make_int4(1, 1, 1, 1);
+  if (id < p.num_pages) r.x = p.refs[id];
+  if (id + 1 < p.num_pages) r.y = p.refs[id + 1];
+  if (id + 2 < p.num_pages) r.z = p.refs[id + 2];
+  if (id + 3 < p.num_pages) r.w = p.refs[id + 3];
+  return r;
+}
+
+// Which entry names a sequence first: an open-addressed table in LDS, cleared by its first barrier's other side.
+constexpr int kCells = 2 * kMaxEntries;
+__device__ __forceinline__ bool first_to_name(int seq, bool valid) {
+  __shared__ int s_key[kCells], s_first[kCells];
+  for (int i = threadIdx.x; i < kCells; i += kPlanThreads) {
+    s_key[i] = -1;
+    s_first[i] = kMaxEntries;
+  }
+  __syncthreads();
+  int cell = 0;
+  if (valid) {
+    cell = (int)(((uint32_t)seq * 2654435761u) >> 21) & (kCells - 1);
+    while (true) {  // at most kMaxEntries keys in twice as many cells: an empty one is always found
+      const int seen = atomicCAS(&s_key[cell], -1, seq);
+      if (seen == -1 || seen == seq) break;
+      cell = (cell + 1) & (kCells - 1);
+    }
+    atomicMin(&s_first[cell], (int)threadIdx.x);
+  }
+  __syncthreads();
+  return valid && s_first[cell] == (int)threadIdx.x;
+}
 
 struct PagesWs {
-  int32_t* first;  // [num_seqs] lowest entry that names the sequence
-  int32_t* fresh;  // [num_pages] free pages, ascending (compact: the new number of every page)
-  int32_t* count;  // [4] 0: moves of a compaction
-  int32_t* a;      // [n] fork: shared pages of the pair; extend: pages held
-  int32_t* b;      // [n] fork: page to copy or -1;       extend: pages after
-  int32_t* c;      // [n] fork: page to copy it to;       extend: place of its first page in `fresh`
-  int32_t *src, *dst;  // compact: [num_pages] moves
+  int32_t* count;  // [16] 0: moves of a compaction
+  int32_t* full;   // [n] fork: shared pages of the pair, -1: nothing to do
+  int32_t *src, *dst;  // fork [n], compact [num_pages / 2]: pages to copy and where to; -1: none
+  int32_t* to;     // compact: [num_pages] the page's new number
 };
 static size_t pages_ws_bytes(const okv_page_pool_t* p, int64_t n) {
-  return 4 * ((size_t)p->num_seqs + 3 * (size_t)p->num_pages + 16 + 3 * (size_t)n) + 256;
+  return 4 * (2 * (size_t)p->num_pages + 16 + 3 * (size_t)n) + 256;
 }
 static PagesWs carve(const okv_page_pool_t* p, int64_t n, void* ws) {
   int32_t* x = (int32_t*)(((size_t)ws + 255) & ~(size_t)255);
   PagesWs w;
-  w.first = x; x += p->num_seqs;
-  w.fresh = x; x += p->num_pages;
-  w.src = x; x += p->num_pages;
-  w.dst = x; x += p->num_pages;
   w.count = x; x += 16;
-  w.a = x; x += n;
-  w.b = x; x += n;
-  w.c = x;
+  w.full = x; x += n;
+  const int64_t m = n > 0 ? n : p->num_pages / 2;
+  w.src = x; x += m;
+  w.dst = x; x += m;
+  w.to = x;
   return w;
 }
 
@@ -100,225 +132,262 @@ __global__ __launch_bounds__(256) void pages_free_kernel(okv_page_pool_t p, cons
   }
 }
 
-// first[s] = the lowest entry that names sequence s; every thread of the plan calls it
-__device__ void claim(const okv_page_pool_t& p, const int32_t* seqs, int n, int32_t* first) {
-  for (int i = threadIdx.x; i < n; i += kPlanThreads)
-    if ((uint32_t)seqs[i] < (uint32_t)p.num_seqs) put(&first[seqs[i]], 0x7fffffff);
-  __threadfence();
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kPlanThreads)
-    if ((uint32_t)seqs[i] < (uint32_t)p.num_seqs) atomicMin(&first[seqs[i]], i);
-  __threadfence();
-  __syncthreads();
-}
-
-// The `want` lowest free pages into fresh[]; returns how many there are (at most want).
-__device__ int find_free(const okv_page_pool_t& p, int want, int32_t* fresh) {
-  int have = 0;
-  for (int base = 0; base < p.num_pages && have < want; base += kPlanThreads) {
-    const int id = base + (int)threadIdx.x;
-    const int is_free = id < p.num_pages && p.refs[id] <= 0;
-    int total;
-    const int at = have + block_scan(is_free, &total) - is_free;
-    if (is_free && at < want) put(&fresh[at], id);
-    have += total;
-  }
-  __threadfence();
-  __syncthreads();
-  return have < want ? have : want;
-}
-
+// One thread per pair.  A chain of three round trips to memory (the pair, the lengths, the last page's number), with
+// the counts of the first 4096 pages on their way meanwhile.
 __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan(okv_page_pool_t p, const int32_t* parents,
                                                                const int32_t* children, int n, int32_t* status, PagesWs w) {
-  claim(p, children, n, w.first);
-  int want = 0, bad = 0;
-  for (int base = 0; base < n; base += kPlanThreads) {
-    const int i = base + (int)threadIdx.x;
-    int need = 0, refuse = 0;
-    if (i < n) {
-      const int from = parents[i], to = children[i];
-      bool ok = (uint32_t)from < (uint32_t)p.num_seqs && (uint32_t)to < (uint32_t)p.num_seqs && from != to;
-      ok = ok && get(&w.first[to]) == i && p.lens[to] <= 0;
-      const int len = ok ? p.lens[from] : 0;
-      const int full = len > 0 ? len / p.page_size : 0;
-      const int part = len > 0 && len % p.page_size && full < p.max_pages;
-      const int old = part ? p.table[(int64_t)from * p.table_stride + full] : -1;
-      refuse = !ok;
-      need = part;
-      w.a[i] = ok ? min(full, p.max_pages) : -1;
-      w.b[i] = (uint32_t)old < (uint32_t)p.num_pages ? old : -1;
-    }
+  __shared__ int s_fresh[kMaxEntries];
+  const int i = threadIdx.x;
+  int turn = 0;
+  int4 refs = load_refs(p, 0);
+  const int from = i < n ? parents[i] : -1, to = i < n ? children[i] : -1;
+  const bool from_in = (uint32_t)from < (uint32_t)p.num_seqs, to_in = (uint32_t)to < (uint32_t)p.num_seqs;
+  int len = from_in ? p.lens[from] : 0;
+  const int held = to_in ? p.lens[to] : 0;
+  const bool named_first = first_to_name(to, to_in);
+  const bool ok = named_first && from_in && from != to && held <= 0;
+  if (!ok || len < 0) len = 0;
+  const int full = min(len / p.page_size, p.max_pages);
+  const bool part = len % p.page_size != 0 && full < p.max_pages;
+  const int old = part ? p.table[(int64_t)from * p.table_stride + full] : -1;
+  int want, bad;
+  const int at = block_scan(part, &want, turn);
+  block_scan(i < n && !ok, &bad, turn);
+  int have = 0;
+  for (int base = 0; base < p.num_pages && have < want; base += kTrip) {
+    if (base) refs = load_refs(p, base);
+    const int f[4] = {refs.x <= 0, refs.y <= 0, refs.z <= 0, refs.w <= 0};
     int total;
-    const int at = want + block_scan(need, &total) - need;
-    if (i < n) w.c[i] = need ? at : -1;
-    want += total;
-    block_scan(refuse, &total);
-    bad += total;
-  }
-  const int have = find_free(p, want, w.fresh);
-  const bool enough = have == want;
-  for (int i = threadIdx.x; i < n; i += kPlanThreads) {  // each thread its own entries of a, b, c
-    const int full = w.a[i];
-    if (!enough || full < 0) {
-      w.a[i] = -1;
-      w.c[i] = -1;
-      continue;
+    int k = have + block_scan(f[0] + f[1] + f[2] + f[3], &total, turn);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (f[x] && k < want) s_fresh[k] = base + kPerThread * i + x;
+      k += f[x];
     }
-    const int at = w.c[i];
-    if (at >= 0) {
-      const int page = get(&w.fresh[at]);
-      w.c[i] = page;
-      p.refs[page] = 1;
-    }
+    have = min(have + total, want);
   }
-  __syncthreads();  // every length has been read
-  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-    // a parent that is itself a child of this call was empty before it
-    const int from = parents[i];
-    if (w.a[i] > 0 || w.c[i] >= 0) p.lens[children[i]] = p.lens[from];
+  __syncthreads();  // fresh pages known; every length has been read
+  const bool act = have == want && ok && len > 0;
+  const int fresh = act && part ? s_fresh[at] : -1;
+  if (i < n) {
+    w.full[i] = act ? full : -1;
+    w.src[i] = fresh >= 0 ? old : -1;
+    w.dst[i] = fresh;
   }
-  if (status && threadIdx.x == 0) {
+  // a parent that is itself a child of this call was empty before it: its length is not one that is written here
+  if (act) p.lens[to] = len;
+  if (fresh >= 0) p.refs[fresh] = 1;
+  if (status && i == 0) {
     status[0] = want - have;
     status[1] = bad;
   }
 }
 
-// one page of one buffer, by a workgroup of 256 threads
-__device__ __forceinline__ void copy_page(const okv_page_buffer_t& buf, int src, int dst) {
-  const char* s = (const char*)buf.base + (int64_t)src * buf.page_bytes;
-  char* d = (char*)buf.base + (int64_t)dst * buf.page_bytes;
-  if ((((uintptr_t)buf.base | (uintptr_t)buf.page_bytes) & 15) == 0) {
-    for (int64_t o = 16 * threadIdx.x; o < buf.page_bytes; o += 16 * 256)
-      *reinterpret_cast<uint4*>(d + o) = *reinterpret_cast<const uint4*>(s + o);
-  } else {
-    for (int64_t o = 4 * threadIdx.x; o < buf.page_bytes; o += 4 * 256)
-      *reinterpret_cast<uint32_t*>(d + o) = *reinterpret_cast<const uint32_t*>(s + o);
-  }
-}
-
-// grid (n, 1 + buffers): y = 0 names the pages in the child's row, the others copy the partly filled page
-__global__ __launch_bounds__(256) void pages_fork_apply(okv_page_pool_t p, const int32_t* parents, const int32_t* children,
-                                                        PagesWs w, BufferList bufs, int rows) {
-  const int i = blockIdx.x, full = w.a[i], fresh = w.c[i];
-  if (full < 0) return;
-  if (rows && blockIdx.y == 0) {
-    const int32_t* from = p.table + (int64_t)parents[i] * p.table_stride;
-    int32_t* to = p.table + (int64_t)children[i] * p.table_stride;
-    for (int k = threadIdx.x; k < full; k += 256) {
-      const int id = from[k];
-      to[k] = id;
-      if ((uint32_t)id < (uint32_t)p.num_pages) atomicAdd(&p.refs[id], 1);
-    }
-    if (fresh >= 0 && threadIdx.x == 0) to[full] = fresh;
+// Pages of one buffer, by a workgroup of 256 threads: moves [first, first + per), `per` pages of a small buffer side
+// by side, a page of a large one with four loads of a thread in flight.
+template <typename V>
+__device__ __forceinline__ void copy_pages(const okv_page_buffer_t& buf, const int32_t* src, const int32_t* dst, int first, int per,
+                                           int m, int num_pages) {
+  const uint32_t unit = (uint32_t)(buf.page_bytes / (int64_t)sizeof(V));
+  V* base = reinterpret_cast<V*>(buf.base);
+  if (per > 1) {
+    const uint32_t k = threadIdx.x / unit, o = threadIdx.x % unit;
+    const int i = first + (int)k;
+    if ((int)k >= per || i >= m) return;
+    const int s = src[i], d = dst[i];
+    if ((uint32_t)s < (uint32_t)num_pages && (uint32_t)d < (uint32_t)num_pages) base[(int64_t)d * unit + o] = base[(int64_t)s * unit + o];
     return;
   }
-  const int old = w.b[i];
-  if (fresh >= 0 && old >= 0) copy_page(bufs.b[blockIdx.y - rows], old, fresh);
+  if (first >= m) return;
+  const int s = src[first], d = dst[first];
+  if ((uint32_t)s >= (uint32_t)num_pages || (uint32_t)d >= (uint32_t)num_pages || s == d) return;
+  const int64_t pu = buf.page_bytes / (int64_t)sizeof(V);
+  const V* from = base + (int64_t)s * pu;
+  V* to = base + (int64_t)d * pu;
+  int64_t o = threadIdx.x;
+  for (; o + 768 < pu; o += 1024) {
+    const V x0 = __builtin_nontemporal_load(from + o), x1 = __builtin_nontemporal_load(from + o + 256),
+            x2 = __builtin_nontemporal_load(from + o + 512), x3 = __builtin_nontemporal_load(from + o + 768);
+    __builtin_nontemporal_store(x0, to + o);
+    __builtin_nontemporal_store(x1, to + o + 256);
+    __builtin_nontemporal_store(x2, to + o + 512);
+    __builtin_nontemporal_store(x3, to + o + 768);
+  }
+  for (; o < pu; o += 256) to[o] = from[o];
+}
+typedef __attribute__((ext_vector_type(4))) uint32_t page_vec;
+// moves blockIdx.x, + gridDim.x, ... of `m` (in steps of as many pages as a workgroup takes at once)
+__device__ __forceinline__ void copy_moves(const okv_page_buffer_t& buf, const int32_t* src, const int32_t* dst, int m, int num_pages,
+                                           int block, int blocks) {
+  const bool wide = (((uintptr_t)buf.base | (uintptr_t)buf.page_bytes) & 15) == 0;
+  const int64_t unit = buf.page_bytes / (wide ? 16 : 4);
+  const int per = unit <= 128 ? 256 / (int)unit : 1;
+  for (int64_t first = (int64_t)block * per; first < m; first += (int64_t)blocks * per) {
+    if (wide) copy_pages<page_vec>(buf, src, dst, (int)first, per, m, num_pages);
+    else copy_pages<uint32_t>(buf, src, dst, (int)first, per, m, num_pages);
+  }
 }
 
+// grid (n, 1 + buffers): y = 0 names the pages in the child's row, the others copy the partly filled pages
+__global__ __launch_bounds__(256) void pages_fork_apply(okv_page_pool_t p, const int32_t* parents, const int32_t* children,
+                                                        int n, PagesWs w, BufferList bufs, int rows) {
+  if (!rows || blockIdx.y > 0) {
+    copy_moves(bufs.b[blockIdx.y - rows], w.src, w.dst, n, p.num_pages, blockIdx.x, gridDim.x);
+    return;
+  }
+  const int i = blockIdx.x, full = w.full[i], fresh = w.dst[i];
+  if (full < 0) return;
+  const int32_t* from = p.table + (int64_t)parents[i] * p.table_stride;
+  int32_t* to = p.table + (int64_t)children[i] * p.table_stride;
+  for (int k = threadIdx.x; k < full; k += 256) {
+    const int id = from[k];
+    to[k] = id;
+    if ((uint32_t)id < (uint32_t)p.num_pages) atomicAdd(&p.refs[id], 1);
+  }
+  if (fresh >= 0 && threadIdx.x == 0) to[full] = fresh;
+}
+
+// One thread per entry; two trips through the counts: whether there are enough free pages, then who gets which.
 __global__ __launch_bounds__(kPlanThreads) void pages_extend_plan(okv_page_pool_t p, const int32_t* seqs, const int32_t* more,
-                                                                 int n, int32_t* status, PagesWs w) {
-  claim(p, seqs, n, w.first);
-  int want = 0, bad = 0;
-  for (int base = 0; base < n; base += kPlanThreads) {
-    const int i = base + (int)threadIdx.x;
-    int need = 0, refuse = 0;
-    if (i < n) {
-      const int s = seqs[i];
-      bool ok = (uint32_t)s < (uint32_t)p.num_seqs && get(&w.first[s]) == i;
-      const int64_t len = ok ? max(p.lens[s], 0) : 0, to = len + max(more[i], 0);
-      ok = ok && to <= 0x7fffffff && to <= (int64_t)p.max_pages * p.page_size;
-      refuse = !ok;
-      w.a[i] = ok ? pages_of(len, p.page_size) : -1;
-      w.b[i] = ok ? pages_of(to, p.page_size) : -1;
-      need = ok ? w.b[i] - w.a[i] : 0;
-    }
-    int total;
-    const int at = want + block_scan(need, &total) - need;
-    if (i < n) w.c[i] = at;
-    want += total;
-    block_scan(refuse, &total);
-    bad += total;
+                                                                 int n, int32_t* status) {
+  __shared__ int s_at[kMaxEntries + 1], s_seq[kMaxEntries], s_from[kMaxEntries];
+  const int i = threadIdx.x;
+  int turn = 0;
+  int4 refs = load_refs(p, 0);
+  const int s = i < n ? seqs[i] : -1;
+  const int64_t grow = i < n ? max(more[i], 0) : 0;
+  const bool in = (uint32_t)s < (uint32_t)p.num_seqs;
+  const int64_t len = in ? max(p.lens[s], 0) : 0, to = len + grow;
+  const bool ok = first_to_name(s, in) && to <= 0x7fffffff && to <= (int64_t)p.max_pages * p.page_size;
+  const int from = ok ? pages_of(len, p.page_size) : 0, need = ok ? pages_of(to, p.page_size) - from : 0;
+  int want, bad, have = 0, total;
+  s_at[i] = block_scan(need, &want, turn);
+  s_seq[i] = s;
+  s_from[i] = from;
+  block_scan(i < n && !ok, &bad, turn);
+  for (int base = 0; base < p.num_pages && have < want; base += kTrip) {
+    const int4 r = base ? load_refs(p, base) : refs;
+    block_scan((r.x <= 0) + (r.y <= 0) + (r.z <= 0) + (r.w <= 0), &total, turn);
+    have = min(have + total, want);
   }
-  const int have = find_free(p, want, w.fresh);
   if (have == want) {
-    for (int i = 0; i < n; ++i) {
-      const int from = w.a[i], to = w.b[i], at = w.c[i], s = seqs[i];
-      if (from < 0) continue;
-      for (int k = from + (int)threadIdx.x; k < to; k += kPlanThreads) {
-        const int page = get(&w.fresh[at + k - from]);
-        p.table[(int64_t)s * p.table_stride + k] = page;
-        p.refs[page] = 1;
+    if (ok) p.lens[s] = (int)to;
+    for (int base = 0, k0 = 0; base < p.num_pages && k0 < want; base += kTrip) {
+      if (base) refs = load_refs(p, base);
+      const int f[4] = {refs.x <= 0, refs.y <= 0, refs.z <= 0, refs.w <= 0};
+      int k = k0 + block_scan(f[0] + f[1] + f[2] + f[3], &total, turn);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (f[x] && k < want) {
+          int lo = 0, hi = n - 1;  // the last entry whose pages start at or before the k-th
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_at[mid] <= k) lo = mid;
+            else hi = mid - 1;
+          }
+          const int page = base + kPerThread * i + x;
+          p.table[(int64_t)s_seq[lo] * p.table_stride + s_from[lo] + (k - s_at[lo])] = page;
+          p.refs[page] = 1;
+        }
+        k += f[x];
       }
-      if (threadIdx.x == 0) p.lens[s] = max(p.lens[s], 0) + max(more[i], 0);
+      k0 += total;
     }
   }
-  if (status && threadIdx.x == 0) {
+  if (status && i == 0) {
     status[0] = want - have;
     status[1] = bad;
   }
 }
 
-__global__ __launch_bounds__(256) void pages_copy_kernel(BufferList bufs, int num_buffers, int num_pages, const int32_t* src,
-                                                         const int32_t* dst, const int32_t* count, int n) {
-  int m = count ? *count : n;
-  m = m > n ? n : m;
-  for (int64_t u = blockIdx.x; u < (int64_t)m * num_buffers; u += gridDim.x) {
-    const int i = (int)(u / num_buffers), j = (int)(u % num_buffers);
-    const int s = src[i], d = dst[i];
-    if ((uint32_t)s < (uint32_t)num_pages && (uint32_t)d < (uint32_t)num_pages && s != d) copy_page(bufs.b[j], s, d);
-  }
+// grid (blocks, buffers)
+__global__ __launch_bounds__(256) void pages_copy_kernel(BufferList bufs, int num_pages, const int32_t* src, const int32_t* dst,
+                                                         const int32_t* count, int n) {
+  const int m = count ? min(*count, n) : n;
+  copy_moves(bufs.b[blockIdx.y], src, dst, m, num_pages, blockIdx.x, gridDim.x);
 }
 
+// Pages at or above `used` that are in use, in order, go to the free ones below it, in order: equally many of both.
 __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan(okv_page_pool_t p, int32_t* refs_out, int32_t* used_out,
                                                                   PagesWs w) {
-  int used = 0;
-  for (int base = 0; base < p.num_pages; base += kPlanThreads) {
-    const int id = base + (int)threadIdx.x;
-    int total;
-    block_scan(id < p.num_pages && p.refs[id] > 0, &total);
+  const int i = threadIdx.x;
+  int turn = 0, used = 0, total;
+  const int4 first = load_refs(p, 0);
+  auto busy = [&](int base, const int4& r, int x) {
+    const int v = x == 0 ? r.x : x == 1 ? r.y : x == 2 ? r.z : r.w;
+    return v > 0 && base + kPerThread * i + x < p.num_pages;
+  };
+  for (int base = 0; base < p.num_pages; base += kTrip) {
+    const int4 r = base ? load_refs(p, base) : first;
+    block_scan(busy(base, r, 0) + busy(base, r, 1) + busy(base, r, 2) + busy(base, r, 3), &total, turn);
     used += total;
   }
-  int nf = 0, nu = 0;
-  for (int base = 0; base < p.num_pages; base += kPlanThreads) {
-    const int id = base + (int)threadIdx.x;
-    const bool in = id < p.num_pages, busy = in && p.refs[id] > 0;
-    const int hole = in && !busy && id < used, high = busy && id >= used;
-    int total;
-    const int af = nf + block_scan(hole, &total) - hole;
-    nf += total;
-    const int au = nu + block_scan(high, &total) - high;
-    nu += total;
-    if (hole) put(&w.dst[af], id);
-    if (high) put(&w.src[au], id);
-    if (in && !high) put(&w.fresh[id], id);  // keeps its number
+  int holes = 0, highs = 0;
+  for (int base = 0; base < p.num_pages; base += kTrip) {
+    const int4 r = base ? load_refs(p, base) : first;
+    int hole[4], high[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int id = base + kPerThread * i + x;
+      const bool b = busy(base, r, x);
+      hole[x] = id < p.num_pages && id < used && !b;
+      high[x] = b && id >= used;
+      if (id < p.num_pages && !high[x]) w.to[id] = id;
+    }
+    int h = holes + block_scan(hole[0] + hole[1] + hole[2] + hole[3], &total, turn);
+    holes += total;
+    int u = highs + block_scan(high[0] + high[1] + high[2] + high[3], &total, turn);
+    highs += total;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int id = base + kPerThread * i + x;
+      if (hole[x]) w.dst[h] = id;
+      if (high[x]) w.src[u] = id;
+      h += hole[x];
+      u += high[x];
+    }
   }
-  __threadfence();
   __syncthreads();
-  // as many holes below `used` as pages in use at or above it
-  for (int i = threadIdx.x; i < nu; i += kPlanThreads) put(&w.fresh[get(&w.src[i])], get(&w.dst[i]));
-  for (int base = 0; base < p.num_pages; base += kPlanThreads) {  // the pages that stay; refs_out may be refs
-    const int id = base + (int)threadIdx.x;
-    if (id < p.num_pages && id < used && p.refs[id] > 0) refs_out[id] = p.refs[id];
+  for (int k = i; k < highs; k += kPlanThreads) {
+    const int s = w.src[k], d = w.dst[k];
+    w.to[s] = d;
+    refs_out[d] = p.refs[s];  // page s is not below `used`: nothing here has written its count
   }
-  for (int i = threadIdx.x; i < nu; i += kPlanThreads) {
-    const int s = get(&w.src[i]), v = p.refs[s];
-    refs_out[get(&w.dst[i])] = v;
-  }
-  __syncthreads();
-  for (int id = used + (int)threadIdx.x; id < p.num_pages; id += kPlanThreads) refs_out[id] = 0;
-  if (threadIdx.x == 0) {
-    w.count[0] = nu;
+  if (refs_out != p.refs)
+    for (int base = 0; base < used; base += kTrip) {
+      const int4 r = base ? load_refs(p, base) : first;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int id = base + kPerThread * i + x;
+        if (id < used && busy(base, r, x)) refs_out[id] = x == 0 ? r.x : x == 1 ? r.y : x == 2 ? r.z : r.w;
+      }
+    }
+  __syncthreads();  // the moved pages' counts have been read
+  for (int id = used + i; id < p.num_pages; id += kPlanThreads) refs_out[id] = 0;
+  if (i == 0) {
+    w.count[0] = highs;
     if (used_out) *used_out = used;
   }
 }
 
-// grid (blocks, num_seqs): every entry gets its page's new number
-__global__ __launch_bounds__(256) void pages_compact_table(okv_page_pool_t p, int32_t* out, int64_t out_stride, PagesWs w) {
-  const int s = blockIdx.y, k = blockIdx.x * 256 + threadIdx.x;
-  if (k >= p.max_pages) return;
-  const int id = p.table[(int64_t)s * p.table_stride + k];
-  out[(int64_t)s * out_stride + k] = (uint32_t)id < (uint32_t)p.num_pages ? w.fresh[id] : id;
+// grid (blocks, table rows' blocks + buffers): the table's entries get their pages' new numbers, the others move the pages
+__global__ __launch_bounds__(256) void pages_compact_apply(okv_page_pool_t p, int32_t* out, int64_t out_stride, PagesWs w,
+                                                           BufferList bufs, int table) {
+  if (!table || blockIdx.y > 0) {
+    copy_moves(bufs.b[blockIdx.y - table], w.src, w.dst, w.count[0], p.num_pages, blockIdx.x, gridDim.x);
+    return;
+  }
+  for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x)
+    for (int k = threadIdx.x; k < p.max_pages; k += 256) {
+      const int id = p.table[(int64_t)s * p.table_stride + k];
+      out[(int64_t)s * out_stride + k] = (uint32_t)id < (uint32_t)p.num_pages ? w.to[id] : id;
+    }
+}
+
+// Workgroups along x for `moves` moves of each of `buffers` buffers: some thousands in all, which fill the chip.
+static uint32_t copy_blocks(int64_t moves, int buffers) {
+  const int64_t most = buffers > 0 ? (4096 + buffers - 1) / buffers : 4096;
+  return (uint32_t)(moves < 1 ? 1 : moves < most ? moves : most);
 }
 
 static int check_pool(const okv_page_pool_t* p, const char* what, bool lens) {
@@ -378,30 +447,29 @@ int okv_pages_fork(const okv_page_pool_t* pool, const int32_t* parents, const in
   if (!rc) rc = check_buffers(host_buffers, num_buffers, "okv_pages_fork");
   if (rc) return rc;
   OKV_REQUIRE(n >= 1 && parents && children, OKV_ERR_INVALID, "okv_pages_fork: n >= 1 pairs");
+  OKV_REQUIRE(n <= kMaxEntries, OKV_ERR_UNSUPPORTED, "okv_pages_fork: %d pairs in one call (at most %d)", n, kMaxEntries);
   rc = check_ws(pool, n, ws, ws_bytes);
   if (rc) return rc;
   const PagesWs w = carve(pool, n, ws);
   hipLaunchKernelGGL(pages_fork_plan, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, *pool, parents, children, n, status, w);
   for (int lo = 0; lo == 0 || lo < num_buffers; lo += kBuffersPerLaunch) {
     const int m = num_buffers - lo < kBuffersPerLaunch ? num_buffers - lo : kBuffersPerLaunch, rows = lo == 0;
-    hipLaunchKernelGGL(pages_fork_apply, dim3(n, m + rows), dim3(256), 0, (hipStream_t)stream, *pool, parents, children, w,
-                       take(host_buffers + lo, m), rows);
+    hipLaunchKernelGGL(pages_fork_apply, dim3(n, m + rows), dim3(256), 0, (hipStream_t)stream, *pool, parents, children, n,
+                       w, take(host_buffers + lo, m), rows);
   }
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;
 }
 
 int okv_pages_extend(const okv_page_pool_t* pool, const int32_t* seqs, const int32_t* more, int32_t n, int32_t* status,
-                     void* ws, size_t ws_bytes, okv_stream_t stream) {
+                     okv_stream_t stream) {
   int rc = check_pool(pool, "okv_pages_extend", true);
   if (rc) return rc;
   OKV_REQUIRE(n >= 1 && seqs && more, OKV_ERR_INVALID, "okv_pages_extend: n >= 1 entries");
+  OKV_REQUIRE(n <= kMaxEntries, OKV_ERR_UNSUPPORTED, "okv_pages_extend: %d entries in one call (at most %d)", n, kMaxEntries);
   OKV_REQUIRE((int64_t)n * pool->max_pages < (1ll << 30), OKV_ERR_UNSUPPORTED,
               "okv_pages_extend: %d entries of up to %d pages in one call", n, pool->max_pages);
-  rc = check_ws(pool, n, ws, ws_bytes);
-  if (rc) return rc;
-  hipLaunchKernelGGL(pages_extend_plan, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, *pool, seqs, more, n, status,
-                     carve(pool, n, ws));
+  hipLaunchKernelGGL(pages_extend_plan, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, *pool, seqs, more, n, status);
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;
 }
@@ -414,9 +482,8 @@ int okv_pages_copy(const okv_page_buffer_t* host_buffers, int32_t num_buffers, i
   if (n == 0) return OKV_OK;
   for (int lo = 0; lo < num_buffers; lo += kBuffersPerLaunch) {
     const int m = num_buffers - lo < kBuffersPerLaunch ? num_buffers - lo : kBuffersPerLaunch;
-    const int64_t units = (int64_t)n * m;
-    hipLaunchKernelGGL(pages_copy_kernel, dim3((uint32_t)(units < 4096 ? units : 4096)), dim3(256), 0, (hipStream_t)stream,
-                       take(host_buffers + lo, m), m, num_pages, src, dst, count, n);
+    hipLaunchKernelGGL(pages_copy_kernel, dim3(copy_blocks(n, m), m), dim3(256), 0, (hipStream_t)stream, take(host_buffers + lo, m),
+                       num_pages, src, dst, count, n);
   }
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;
@@ -429,16 +496,18 @@ int okv_pages_compact(const okv_page_pool_t* pool, int32_t* table_out, int64_t t
   if (!rc) rc = check_buffers(host_buffers, num_buffers, "okv_pages_compact");
   if (rc) return rc;
   OKV_REQUIRE(table_out && refs_out && table_out_stride >= pool->max_pages, OKV_ERR_INVALID, "okv_pages_compact: bad outputs");
-  OKV_REQUIRE(pool->num_seqs <= 65535, OKV_ERR_UNSUPPORTED, "okv_pages_compact: %d sequences", pool->num_seqs);
   rc = check_ws(pool, 0, ws, ws_bytes);
   if (rc) return rc;
   const PagesWs w = carve(pool, 0, ws);
   hipLaunchKernelGGL(pages_compact_plan, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, *pool, refs_out, used_out, w);
-  hipLaunchKernelGGL(pages_compact_table, dim3((pool->max_pages + 255) / 256, pool->num_seqs), dim3(256), 0,
-                     (hipStream_t)stream, *pool, table_out, table_out_stride, w);
+  for (int lo = 0; lo == 0 || lo < num_buffers; lo += kBuffersPerLaunch) {
+    const int m = num_buffers - lo < kBuffersPerLaunch ? num_buffers - lo : kBuffersPerLaunch, table = lo == 0;
+    const uint32_t blocks = copy_blocks(pool->num_pages / 2 > pool->num_seqs ? pool->num_pages / 2 : pool->num_seqs, m + table);
+    hipLaunchKernelGGL(pages_compact_apply, dim3(blocks, m + table), dim3(256), 0, (hipStream_t)stream, *pool, table_out,
+                       table_out_stride, w, take(host_buffers + lo, m), table);
+  }
   OKV_HIP_CHECK(hipGetLastError());
-  if (num_buffers == 0) return OKV_OK;
-  return okv_pages_copy(host_buffers, num_buffers, pool->num_pages, w.src, w.dst, w.count, pool->num_pages / 2, stream);
+  return OKV_OK;
 }
 
 }  // extern "C"

@@ -8,7 +8,6 @@ token-major store are read in place.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
 import math
@@ -505,25 +504,33 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 # ---------------------------------------------------------------- 8-bit K/V cache
 KV8_FORMATS = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+_SCALE128 = 1.0 / math.sqrt(128)
 _KV8_CODES = {torch.float8_e4m3fn: _lib.OKV_E4M3, torch.int8: _lib.OKV_I8}
-_NO_SWITCH = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _on(device: torch.device):
-    """The device's context when it is not the current one: a launch goes to the current device."""
-    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(device: torch.device, fn, *args) -> None:
+    """fn(*args, current stream of `device`), with that device current: a launch goes to the current one."""
+    i = device.index
+    if i != torch.cuda.current_device():
+        with torch.cuda.device(i):
+            check(fn(*args, _raw_stream(i)))
+        return
+    rc = fn(*args, _raw_stream(i))
+    if rc:
+        check(rc)
 
 
 def _scratch(device, nbytes: int) -> torch.Tensor:
-    """Scratch of one call, from torch's allocator: it may be reused by what the same stream runs next, and a
-    captured graph keeps a piece of its own pool, so two graphs never share one."""
+    """Scratch of one call, from torch's allocator: it may be reused by what the same stream runs next, two threads
+    never hold the same piece, and a captured graph keeps a piece of its own pool, so two graphs do not share one."""
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _dev_i32(t: Optional[torch.Tensor], n: int, device, name: str):
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != device or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on {device}")
     return t.data_ptr()
 
@@ -598,6 +605,7 @@ class KV8:
                 c.open_k, c.open_v = open_k.data_ptr(), open_v.data_ptr()
                 c.open_batch_stride, c.open_head_stride, c.open_token_stride = open_k.stride()[:3]
             self._c[dt] = c
+        self._ref = {dt: C.byref(c) for dt, c in self._c.items()}
 
     @classmethod
     def empty(cls, bsz: int, num_kv_heads: int, capacity: int, fmt: str = "e4m3", block: int = 64,
@@ -634,7 +642,7 @@ class KV8:
         return torch.where(ok, slots.to(torch.int32), -1)
 
     def _struct(self, dtype: torch.dtype):
-        c = self._c.get(dtype)
+        c = self._ref.get(dtype)
         if c is None:
             raise ValueError(f"{dtype} next to this cache: it takes " + " and ".join(str(d) for d in self._c))
         return c
@@ -666,14 +674,13 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, t
         return
     on_dev = isinstance(start, torch.Tensor)
     starts = _dev_i32(start, cache.bsz, cache.device, "start") if on_dev else None
-    with _on(cache.device):
-        check(lib().okv_kv8_append(C.byref(c), k.data_ptr(), v.data_ptr(), st, sg, sb, starts, 0 if on_dev else int(start),
-                                   _dev_i32(new_lens, cache.bsz, cache.device, "new_lens"), n, int(close), cache.bsz,
-                                   _stream_ptr(cache.device)))
+    _launch(cache.device, lib().okv_kv8_append, c, k.data_ptr(), v.data_ptr(), st, sg, sb, starts, 0 if on_dev else int(start),
+            _dev_i32(new_lens, cache.bsz, cache.device, "new_lens"), n, int(close), cache.bsz)
 
 
 def _kv8_query(q: torch.Tensor, cache: KV8):
-    q = _q3(q)
+    if q.dim() != 3 or not q.is_contiguous():
+        q = _q3(q)
     if q.dim() != 3 or q.shape[0] != cache.bsz or q.shape[2] != 128:
         raise ValueError(f"q must be ({cache.bsz}, Hq, 128) or ({cache.bsz}, Hq, 1, 128)")
     if q.device != cache.device:
@@ -708,15 +715,16 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
         elif scores.shape != (bsz, slen) or scores.dtype != torch.float32 or scores.stride(1) != 1 or scores.device != dev:
             raise ValueError("scores_out must be (bsz, score_len) float32 with contiguous rows, on the cache's GPU")
         sp, ss, sl = scores.data_ptr(), scores.stride(0), _dev_i32(score_lens, bsz, dev, "score_lens")
-    ws = _scratch(dev, _kv8_workspace_bytes(dev.index, bsz, hq, hkv, seq_len, slen))
-    with _on(dev):
-        check(lib().okv_kv8_dense_attn(q.data_ptr(), hq, C.byref(c), _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz,
-                                       scale if scale is not None else 1.0 / math.sqrt(128), out.data_ptr(), sl, slen, red,
-                                       norm, sp, ss, ws.data_ptr(), ws.numel(), _stream_ptr(dev)))
-        if selector is None:
-            return out
-        if select_k is None:
-            return out, scores
+    nbytes = _kv8_workspace_bytes(dev.index, bsz, hq, hkv, seq_len, slen)
+    ws = _scratch(dev, nbytes) if nbytes else None
+    _launch(dev, lib().okv_kv8_dense_attn, q.data_ptr(), hq, c, _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz,
+            scale if scale is not None else _SCALE128, out.data_ptr(), sl, slen, red, norm, sp, ss,
+            ws.data_ptr() if nbytes else None, nbytes)
+    if selector is None:
+        return out
+    if select_k is None:
+        return out, scores
+    with torch.cuda.device(dev):
         return out, scores, topk(scores, select_k, score_lens, k_per_seg, out=idx_out)
 
 
@@ -750,28 +758,28 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
     tkp = tvp = None
     tts = ths = tbs = 0
     if tail_k is not None:
-        if (tail_k.dim() != 4 or tail_v is None or tail_k.shape != tail_v.shape or tail_k.stride() != tail_v.stride()
-                or tail_k.stride(-1) != 1 or tail_k.shape[0] != bsz or tail_k.shape[1] != hkv or tail_k.shape[3] != 128):
+        shape, strides = tail_k.shape, tail_k.stride()
+        if (tail_k.dim() != 4 or tail_v is None or shape != tail_v.shape or strides != tail_v.stride()
+                or strides[3] != 1 or shape[0] != bsz or shape[1] != hkv or shape[3] != 128):
             raise ValueError("tail_k / tail_v must be (bsz, Hkv, T, 128), same strides, contiguous last dimension")
-        if tail_k.dtype != q.dtype or tail_v.dtype != q.dtype or tail_k.device != dev or tail_v.device != dev:
+        if tail_k.dtype is not q.dtype or tail_v.dtype is not q.dtype or tail_k.device != dev or tail_v.device != dev:
             raise ValueError("tail and q differ in dtype or GPU")
         if tail_len is None:
-            tail_len = tail_k.shape[2]
-        elif tail_len > tail_k.shape[2]:
+            tail_len = shape[2]
+        elif tail_len > shape[2]:
             raise ValueError("tail_len exceeds the tail")
         tkp, tvp = tail_k.data_ptr(), tail_v.data_ptr()
-        tts, ths, tbs = tail_k.stride(2), tail_k.stride(1), tail_k.stride(0)
+        tbs, ths, tts, _ = strides
     elif tail_len:
         raise ValueError("tail_len without a tail")
     tail_len = tail_len or 0
     out = torch.empty_like(q)
-    ws = _scratch(dev, _kv8_workspace_bytes(dev.index, bsz, hq, hkv, sel_len + tail_len, 0))
-    with _on(dev):
-        check(lib().okv_kv8_sparse_attn(q.data_ptr(), hq, C.byref(c), ip, istride, int(slots is not None),
-                                        _dev_i32(sel_lens, bsz, dev, "sel_lens"), sel_len, tkp, tvp, tts, ths, tbs,
-                                        _dev_i32(tail_lens, bsz, dev, "tail_lens"), tail_len, bsz,
-                                        scale if scale is not None else 1.0 / math.sqrt(128), out.data_ptr(), ws.data_ptr(),
-                                        ws.numel(), _stream_ptr(dev)))
+    nbytes = _kv8_workspace_bytes(dev.index, bsz, hq, hkv, sel_len + tail_len, 0)
+    ws = _scratch(dev, nbytes) if nbytes else None
+    _launch(dev, lib().okv_kv8_sparse_attn, q.data_ptr(), hq, c, ip, istride, int(slots is not None),
+            _dev_i32(sel_lens, bsz, dev, "sel_lens"), sel_len, tkp, tvp, tts, ths, tbs,
+            _dev_i32(tail_lens, bsz, dev, "tail_lens"), tail_len, bsz, scale if scale is not None else _SCALE128,
+            out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 
@@ -789,10 +797,8 @@ def kv8_read(cache: KV8, dtype: torch.dtype, idx: Optional[torch.Tensor] = None,
         n = idx.shape[1]
     k, v = (torch.empty((bsz, cache.num_kv_heads, n, 128), dtype=dtype, device=dev) for _ in "kv")
     sb, sg, st, _ = k.stride()
-    with _on(dev):
-        check(lib().okv_kv8_read(C.byref(c), idx.data_ptr() if idx is not None else None, n, n,
-                                 _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz, k.data_ptr(), v.data_ptr(), st, sg,
-                                 sb, _stream_ptr(dev)))
+    _launch(dev, lib().okv_kv8_read, c, idx.data_ptr() if idx is not None else None, n, n,
+            _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz, k.data_ptr(), v.data_ptr(), st, sg, sb)
     return k, v
 
 
@@ -812,7 +818,7 @@ class PageBuffers:
                 raise ValueError("buffers must be contiguous (num_pages, ...) tensors on one GPU")
             b.base, b.page_bytes = t.data_ptr(), t.numel() // max(1, self.num_pages) * t.element_size()
 
-    def __len__(self):
+    def __len__(self) -> int:
         return len(self.tensors)
 
 
@@ -821,61 +827,67 @@ def _buffers(buffers) -> PageBuffers:
 
 
 def _page_pool(table, lens, refs, page_size):
-    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or not table.is_cuda:
+    rows, width = table.shape
+    stride, unit = table.stride()
+    if table.dtype is not torch.int32 or unit != 1 or not table.is_cuda:
         raise ValueError("table must be a (num_seqs, max_pages) int32 GPU tensor with contiguous rows")
-    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
-        raise ValueError("table rows must not overlap")
-    lp = _dev_i32(lens, table.shape[0], table.device, "lens")
-    rp = _dev_i32(refs, refs.numel(), table.device, "refs")
-    return _lib.PagePool(table.data_ptr(), lp, rp, max(table.stride(0), table.shape[1]), table.shape[0], table.shape[1],
-                         refs.numel(), page_size)
+    if stride < width:
+        if rows > 1:
+            raise ValueError("table rows must not overlap")
+        stride = width
+    dev, pages = table.device, refs.numel()
+    return dev, _lib.PagePool(table.data_ptr(), _dev_i32(lens, rows, dev, "lens"), _dev_i32(refs, pages, dev, "refs"), stride,
+                              rows, width, pages, page_size)
 
 
 def _entries(t, n, device, name):
-    if t.dim() != 1 or t.numel() < 1:
+    if t.dim() != 1 or n < 1:
         raise ValueError(f"{name} must be a list of at least one entry")
-    return _dev_i32(t, t.numel() if n is None else n, device, name)
+    return _dev_i32(t, n, device, name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _pages_workspace_bytes(num_seqs: int, num_pages: int, n: int) -> int:
+    out = C.c_size_t(0)
+    check(lib().okv_pages_workspace_bytes(C.byref(_lib.PagePool(None, None, None, 0, num_seqs, 0, num_pages, 0)), n, C.byref(out)))
+    return out.value
 
 
 def _pages_scratch(pool, n, device):
-    out = C.c_size_t(0)
-    check(lib().okv_pages_workspace_bytes(C.byref(pool), n, C.byref(out)))
-    return _scratch(device, out.value)
+    return _scratch(device, _pages_workspace_bytes(pool.num_seqs, pool.num_pages, n))
 
 
 def pages_free(table, lens, refs, seqs, page_size: int, status: Optional[torch.Tensor] = None) -> None:
     """Sequences `seqs` give their pages back, in place: reference counts drop, table rows become -1, lengths 0.  table
     (num_seqs, max_pages), lens (num_seqs,), refs (num_pages,), seqs (n,): int32 on the GPU; status (2,) int32
     receives [0, entries outside the table].  okv_pages_free."""
-    dev, pool = table.device, _page_pool(table, lens, refs, page_size)
-    with _on(dev):
-        check(lib().okv_pages_free(C.byref(pool), _entries(seqs, None, dev, "seqs"), seqs.numel(),
-                                   _dev_i32(status, 2, dev, "status"), _stream_ptr(dev)))
+    dev, pool = _page_pool(table, lens, refs, page_size)
+    n = seqs.numel()
+    _launch(dev, lib().okv_pages_free, pool, _entries(seqs, n, dev, "seqs"), n, _dev_i32(status, 2, dev, "status"))
 
 
 def pages_fork(table, lens, refs, parents, children, page_size: int, buffers, status: Optional[torch.Tensor] = None) -> None:
     """Sequence children[i] (empty) becomes a continuation of parents[i], in place: it shares the full pages and gets a copy
     of a partly filled last one in every buffer (a PageBuffers or a list of tensors; the lowest free pages).  status
-    (2,) int32 receives [pages short, pairs refused]; short of pages, nothing changes.  okv_pages_fork."""
-    dev, pool, bufs = table.device, _page_pool(table, lens, refs, page_size), _buffers(buffers)
+    (2,) int32 receives [pages short, pairs refused]; short of pages, nothing changes.  At most 1024 pairs.  okv_pages_fork."""
+    dev, pool = _page_pool(table, lens, refs, page_size)
+    bufs = _buffers(buffers)
     if bufs.device != dev or bufs.num_pages != refs.numel():
         raise ValueError("buffers must hold refs.numel() pages on the table's GPU")
     n = parents.numel()
+    parents, children = _entries(parents, n, dev, "parents"), _entries(children, n, dev, "children")
     ws = _pages_scratch(pool, n, dev)
-    with _on(dev):
-        check(lib().okv_pages_fork(C.byref(pool), _entries(parents, None, dev, "parents"), _entries(children, n, dev, "children"),
-                                   n, bufs._c, len(bufs), _dev_i32(status, 2, dev, "status"), ws.data_ptr(), ws.numel(),
-                                   _stream_ptr(dev)))
+    _launch(dev, lib().okv_pages_fork, pool, parents, children, n, bufs._c, len(bufs), _dev_i32(status, 2, dev, "status"),
+            ws.data_ptr(), ws.numel())
 
 
 def pages_extend(table, lens, refs, seqs, more, page_size: int, status: Optional[torch.Tensor] = None) -> None:
     """Sequence seqs[i] grows by more[i] tokens, in place: it takes the pages it lacks from the lowest free ones.  status as in
     pages_fork.  okv_pages_extend."""
-    dev, pool, n = table.device, _page_pool(table, lens, refs, page_size), seqs.numel()
-    ws = _pages_scratch(pool, n, dev)
-    with _on(dev):
-        check(lib().okv_pages_extend(C.byref(pool), _entries(seqs, None, dev, "seqs"), _entries(more, n, dev, "more"), n,
-                                     _dev_i32(status, 2, dev, "status"), ws.data_ptr(), ws.numel(), _stream_ptr(dev)))
+    dev, pool = _page_pool(table, lens, refs, page_size)
+    n = seqs.numel()
+    _launch(dev, lib().okv_pages_extend, pool, _entries(seqs, n, dev, "seqs"), _entries(more, n, dev, "more"), n,
+            _dev_i32(status, 2, dev, "status"))
 
 
 def pages_copy(buffers, src: torch.Tensor, dst: torch.Tensor, count: Optional[torch.Tensor] = None) -> None:
@@ -885,17 +897,16 @@ def pages_copy(buffers, src: torch.Tensor, dst: torch.Tensor, count: Optional[to
     dev = bufs.device
     if n == 0:
         return
-    with _on(dev):
-        check(lib().okv_pages_copy(bufs._c, len(bufs), bufs.num_pages, _entries(src, None, dev, "src"),
-                                   _entries(dst, n, dev, "dst"), _dev_i32(count, 1, dev, "count"), n, _stream_ptr(dev)))
+    _launch(dev, lib().okv_pages_copy, bufs._c, len(bufs), bufs.num_pages, _entries(src, n, dev, "src"),
+            _entries(dst, n, dev, "dst"), _dev_i32(count, 1, dev, "count"), n)
 
 
 def pages_compact(table, refs, buffers, table_out: Optional[torch.Tensor] = None, refs_out: Optional[torch.Tensor] = None):
     """Moves the pool's U used pages to pages 0 .. U-1 (those at or above U go to the free ones below, in order) and returns
     (table, refs, used): the renamed table and counts (new tensors, or table_out / refs_out, which may be the inputs) and
     U as a (1,) int32 GPU tensor.  okv_pages_compact."""
-    dev, bufs = table.device, _buffers(buffers)
-    pool = _page_pool(table, None, refs, 1)
+    dev, pool = _page_pool(table, None, refs, 1)
+    bufs = _buffers(buffers)
     if bufs.device != dev or bufs.num_pages != refs.numel():
         raise ValueError("buffers must hold refs.numel() pages on the table's GPU")
     if table_out is None:
@@ -906,8 +917,6 @@ def pages_compact(table, refs, buffers, table_out: Optional[torch.Tensor] = None
         refs_out = torch.empty_like(refs)
     used = torch.empty(1, dtype=torch.int32, device=dev)
     ws = _pages_scratch(pool, 0, dev)
-    with _on(dev):
-        check(lib().okv_pages_compact(C.byref(pool), table_out.data_ptr(), max(table_out.stride(0), table_out.shape[1]),
-                                      _dev_i32(refs_out, refs.numel(), dev, "refs_out"), used.data_ptr(), bufs._c, len(bufs),
-                                      ws.data_ptr(), ws.numel(), _stream_ptr(dev)))
+    _launch(dev, lib().okv_pages_compact, pool, table_out.data_ptr(), max(table_out.stride(0), table_out.shape[1]),
+            _dev_i32(refs_out, refs.numel(), dev, "refs_out"), used.data_ptr(), bufs._c, len(bufs), ws.data_ptr(), ws.numel())
     return table_out, refs_out, used
