@@ -42,6 +42,8 @@ struct Kv8Attn {
   int32_t target;     // shares the rows of the call are cut into, about
   int32_t most_rows;  // of a share (its logits are staged in LDS)
   int32_t items;      // shares the grid and the partial results have room for
+  int32_t fine;       // long shares of a batch are cut in three
+  int32_t direct;     // one share per request, which writes the output itself: no second launch
   int32_t fold;         // raw scores: the q heads of a kv head are folded by the split (1 max, 2 sum): one logits row per kv head
   int32_t logit_heads;  // rows of `logits` per request
   int32_t lds_scales;   // floats before the scale staging of the gather mode
@@ -77,6 +79,7 @@ struct Share {
 };
 
 constexpr int kLeastRows = 128;  // one 32-row tile per wave
+constexpr uint32_t kFineRows = 1024;
 
 // inclusive prefix sum over the wave
 __device__ __forceinline__ int lane_scan(int x) {
@@ -89,7 +92,8 @@ __device__ __forceinline__ int lane_scan(int x) {
   return x;
 }
 __device__ __forceinline__ int share_rows(int total, const Kv8Attn& a) {
-  const uint32_t r = (((uint32_t)total + a.target - 1) / (uint32_t)a.target + 63) & ~63u;
+  uint32_t r = (((uint32_t)total + a.target - 1) / (uint32_t)a.target + 63) & ~63u;
+  if (a.fine && r > kFineRows) r = max((r / 3 + 63) & ~63u, kFineRows);
   return r < kLeastRows ? kLeastRows : r > (uint32_t)a.most_rows ? a.most_rows : (int)r;
 }
 __device__ __forceinline__ void request_lens(const Kv8Attn& a, int b, int* main_len, int* L, int* A) {
@@ -101,6 +105,17 @@ __device__ __forceinline__ void request_lens(const Kv8Attn& a, int b, int* main_
 // The share `item` (false: there is none), or with item < 0 the shares of request `request`.
 __device__ __forceinline__ bool find_share(const Kv8Attn& a, int item, int request, Share* s) {
   const int lane = threadIdx.x & 63;
+  if (a.direct) {
+    const int b = item;
+    if (b >= a.batch) return false;
+    request_lens(a, b, &s->main_len, &s->L, &s->A);
+    s->main_len = __builtin_amdgcn_readfirstlane(s->main_len);
+    s->L = __builtin_amdgcn_readfirstlane(s->L);
+    s->b = b;
+    s->index = s->first = 0;
+    s->rows = max(s->L, 1);
+    return true;
+  }
   if (a.batch == 1) {
     request_lens(a, 0, &s->main_len, &s->L, &s->A);
     s->main_len = __builtin_amdgcn_readfirstlane(s->main_len);
@@ -243,7 +258,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   const int b = sh.b, main_len = sh.main_len, L = sh.L, A = LOGITS ? sh.A : 0;
   int begin, end;
   rl_split_range(sh.index, sh.rows, A, L, &begin, &end);
-  if (begin >= end) return;
+  if (begin >= end && !a.direct) return;  // (a request without rows gets its zeros below)
   // rows [0, closed) are codes, the rest 16-bit rows: the open block, or the tail
   const int closed = a.sparse || !c.open_k ? main_len : main_len >> a.block_shift << a.block_shift;
   const int main_end = min(end, closed);
@@ -698,6 +713,10 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       num = fmaf(so[(x * G + h) * kD + d], f, num);
     }
     // den 0: no row took part (a NaN among the logits leaves NaN)
+    if (a.direct) {
+      store1(reinterpret_cast<T*>(a.out) + (int64_t)(b * a.hq + g * G + h) * kD + d, den == 0.f ? 0.f : num / den);
+      continue;
+    }
     const int64_t ph = (int64_t)(sh.first + sh.index) * a.hq + g * G + h;
     a.part_o[ph * kD + d] = den == 0.f ? 0.f : num / den;
     if (d == 0) a.part_lse[ph] = den == 0.f ? -INFINITY : Ms + log2f(den);
@@ -836,21 +855,39 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
 // ---------------------------------------------------------------- host side
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// How many shares to cut the rows into.  The chip holds two workgroups per CU (their registers allow two waves per SIMD),
-// three of the gather mode.  One request: one round of them.  A batch: three rounds, since each request ends in a share
-// cut short (sixteen requests of 8K..32K tokens: 136 us with one round, 124 / 121 / 122 / 127 / 136 with 2 / 3 / 4 / 6 / 8).
-// A scored share stages its logits in LDS, up to 32 KB of them.
+// How many shares to cut the rows into: one round of workgroups, of which the chip holds two per CU (their registers allow
+// two waves per SIMD), three of the gather mode.  In a batch every request ends in a share cut short, so long shares are
+// cut in three (sixteen requests of 8K..32K tokens: 136 us in one round, 124 / 121 / 122 / 127 / 136 in 2 / 3 / 4 / 6 / 8);
+// short ones are not: a workgroup's first microseconds move nothing.  A scored share stages its logits in LDS, up to 32 KB.
 static void kv8_cut(bool gather, int batch, int hkv, int group, int64_t rows, int max_score, bool folded, int* target, int* most, int* items) {
-  *target = std::max(1, (gather ? 256 * kGatherResident : 512 * (batch > 1 ? 3 : 1)) / hkv);
+  *target = std::max(1, 256 * (gather ? kGatherResident : 2) / hkv);
   *most = max_score > 0 ? 32768 / 4 / (folded ? 1 : group) / 64 * 64 : 8192;
   const int64_t all = std::max<int64_t>(rows, 1) * batch;
-  const int64_t n = std::min((all + kLeastRows - 1) / kLeastRows, std::max<int64_t>(*target, (all + *most - 1) / *most));
+  const bool fine = !gather && batch > 1;
+  const int64_t n = std::min((all + kLeastRows - 1) / kLeastRows,
+                             std::max<int64_t>((fine ? 3 : 1) * (int64_t)*target, (all + *most - 1) / *most));
   *items = (int)std::min<int64_t>(n + (int64_t)batch * (max_score > 0 ? 2 : 1), 1 << 30);
 }
 
 // Carves the partial results; the bytes they take.  `folded` saves logits, never adds.
+// A share per request, and no second launch: where requests are short, and longer ones where there are many, the rows a
+// wave then takes one after the other cost less than the join and the round trip through memory.  Measured (bf16, int8,
+// eight kv heads; one launch against two, us): 1 x 333 rows 7.6 / 8.0, 1 x 512 8.2 / 7.8, 16 x 1024 13.6 / 17.0,
+// 64 x 1536 37.8 / 54.3; through an index 1 x 256 7.3 / 8.3, 1 x 333 9.9 / 8.8, 16 x 512 12.9 / 13.1, 64 x 1536 42.1 / 61.1.
+static bool kv8_direct(bool gather, int batch, int hkv, int64_t rows, int max_score) {
+  const int64_t heads = (int64_t)batch * hkv;
+  return max_score == 0 && rows <= std::min<int64_t>(2048, gather ? std::max<int64_t>(256, 4 * heads) : std::max<int64_t>(384, 8 * heads));
+}
+
 static size_t kv8_workspace(bool gather, int batch, int hq, int hkv, int64_t rows, int max_score, bool folded, Kv8Attn* a, char* p) {
   int target, most, items;
+  if (kv8_direct(gather, batch, hkv, rows, max_score)) {
+    if (a) {
+      a->batch = batch;
+      a->direct = 1;
+    }
+    return 0;
+  }
   kv8_cut(gather, batch, hkv, hq / hkv, rows, max_score, folded, &target, &most, &items);
   const size_t o = align256((size_t)items * hq * kD * 4), l = align256((size_t)items * hq * 4);
   const size_t stride = ((size_t)max_score + 63) / 64 * 64;
@@ -862,6 +899,7 @@ static size_t kv8_workspace(bool gather, int batch, int hq, int hkv, int64_t row
     a->target = target;
     a->most_rows = most;
     a->items = items;
+    a->fine = !gather && batch > 1;
     a->part_o = (float*)p;
     a->part_lse = (float*)(p + o);
     a->logits = max_score > 0 ? (float*)(p + o + l) : nullptr;
@@ -877,6 +915,7 @@ static int launch_split(Kv8Attn& a, int batch, hipStream_t stream) {
   if (LOGITS) floats = std::max(floats, (size_t)(a.fold ? 1 : a.group) * a.most_rows);
   a.lds_scales = (int)floats;
   if (MODE == kGather) floats += 256;
+  if (a.direct) a.items = a.batch;
   hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS>), dim3((a.items + 7) / 8 * 8 * a.c.num_kv_heads), dim3(256), floats * 4, stream, a);
   return OKV_OK;
 }
@@ -890,6 +929,10 @@ static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
   else if (scored) launch_split<T, F, kContiguous, true>(a, batch, stream);
   else launch_split<T, F, kContiguous, false>(a, batch, stream);
   // blocks of 512 scores put more CUs to pulling the logits, but each works out the normalisers anew
+  if (a.direct) {
+    OKV_HIP_CHECK(hipGetLastError());
+    return OKV_OK;
+  }
   const int64_t shares = a.items / a.batch;
   const int tokens = shares * ((a.max_score_len + 511) / 512) <= 65536 ? 512 : 1024;
   const dim3 grid(a.hq + (a.max_score_len + tokens - 1) / tokens, batch);
@@ -911,7 +954,7 @@ static int kv8_attend(Kv8Attn& a, int64_t rows, int batch, void* ws, size_t ws_b
   OKV_REQUIRE(a.hq <= kMaxHeads, OKV_ERR_UNSUPPORTED, "%d q heads not supported (at most %d)", a.hq, kMaxHeads);
   OKV_REQUIRE(batch <= 65535, OKV_ERR_UNSUPPORTED, "batch %d not supported", batch);
   OKV_REQUIRE(rows * batch < (1ll << 31), OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
-  OKV_REQUIRE(ws != nullptr, OKV_ERR_INVALID, "workspace pointer is NULL");
+  OKV_REQUIRE(ws != nullptr || kv8_direct(a.idx != nullptr, batch, hkv, rows, a.max_score_len), OKV_ERR_INVALID, "workspace pointer is NULL");
   const bool folded = a.max_score_len > 0 && a.normalise == OKV_NORM_RAW;
   if (folded) a.fold = a.head_reduce == OKV_REDUCE_MAX ? 1 : 2;
   const size_t need = kv8_workspace(a.idx != nullptr, batch, a.hq, hkv, rows, a.max_score_len, folded, &a, (char*)ws);

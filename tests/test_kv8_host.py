@@ -82,8 +82,8 @@ def test_attention_refusals():
     assert dense(cache(), n=1025) == INVALID
     assert dense(cache(), batch=0) == INVALID
     assert dense(cache(), q=PTR + 8) == INVALID
-    assert dense(cache(), ws=None) == INVALID
-    assert dense(cache(), nbytes=256) == WORKSPACE
+    assert dense(cache(), n=1000, ws=None) == INVALID
+    assert dense(cache(), n=1000, nbytes=256) == WORKSPACE
     assert dense(cache(), scores=PTR, score_len=101) == INVALID
     assert dense(cache(), scores=PTR, score_len=50, red=2) == INVALID
     assert dense(cache(), scores=PTR, score_len=50, norm=2) == INVALID
@@ -93,7 +93,7 @@ def test_attention_refusals():
     assert sparse(cache(), slots=1) == INVALID  # no page table
     assert sparse(cache(), tail_len=3) == INVALID
     assert sparse(cache(), tail=PTR, tail_len=3, tts=1028) == INVALID
-    assert sparse(cache(), nbytes=256) == WORKSPACE
+    assert sparse(cache(), n=500, stride=500, nbytes=256) == WORKSPACE
     gap = dict(page_table=PTR, page_size=64, page_table_stride=4, num_pages=9, page_stride=65 * 128 * 8, token_stride=1024)
     assert sparse(cache(**gap), slots=1) == INVALID
     n = C.c_size_t(0)
