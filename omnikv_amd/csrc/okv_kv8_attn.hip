@@ -220,14 +220,28 @@ __device__ __forceinline__ float rows_sum(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// `bytes` bytes at p as a buffer: what lies beyond them reads as zero and is not fetched, and the loads take a lane's 32-bit
+// offset as it is, so that the loop computes no addresses per lane.  (A lane's address registers, taken from those of loads
+// under way, would make the next tile's loads wait for this one's.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t as_buffer(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x27000);
+}
+__device__ __forceinline__ uint4 buffer16(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+  const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 2);  // 2: non-temporal
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ float buffer4(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0));
+}
+
 enum { kContiguous = 0, kPaged = 1, kGather = 2 };
 
-// A wave's 32 rows: K rows (m & 7) + 8x, 16-byte chunk j + 4(m >> 3), and V rows 4j + i of the upper or lower sixteen
-// (m >> 3), chunk m & 7, of lane l = 16j + m: every load covers whole 128-byte rows.
+// A wave's 32 rows as lane l = 16j + m holds them: load i has K row 8i + (m & 7), chunk j + 4(m >> 3) of sixteen bytes, and
+// V row 16(i / 2) + 4j + 2(i % 2) + (m >> 3), chunk m & 7; every load covers eight whole 128-byte rows.
 struct Kv8Tile {
   uint4 k[4], v[4];
-  float sc;   // dense: lane row 0..3 = K scale of rows 0-15, of 16-31, V scales likewise; gather: lanes 0..31 K, 32..63 V scale of row l % 32
-  uint32_t ok;  // dense: bit s = page of rows 16s.. lies in the pool; gather: this lane's own row (l % 32) takes part
+  float ks[2], vs[2];  // dense: scales of rows 0-15 and 16-31; gather: ks[0] alone, see load()
+  uint32_t ok;   // dense: bit s = page of rows 16s.. lies in the pool; gather: this lane's own row (l % 32) takes part
 };
 struct Kv8Rows {
   int page[2];         // paged
@@ -284,6 +298,12 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   const float* ksb = c.k_scale + shead;
   const float* vsb = c.v_scale + shead;
   const uint32_t kcol = 16 * (j + 4 * hi8), vcol = 16 * m8;
+  uint32_t koff[4], voff[4];  // of the lane's rows in a tile
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    koff[i] = (uint32_t)(8 * (MODE == kPaged ? i & 1 : i) + m8) * ts + kcol;
+    voff[i] = (uint32_t)((MODE == kPaged ? 0 : 16 * (i >> 1)) + 4 * j + 2 * (i & 1) + hi8) * ts + vcol;
+  }
   const int last = main_end - 1;
   const int32_t* table = c.page_table + (int64_t)b * c.page_table_stride;
   const int32_t* idx = a.idx + (int64_t)b * a.idx_stride;
@@ -299,7 +319,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     } else if (MODE == kGather) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int rk = min(t + 8 * x + m8, last), rv = min(t + 16 * hi8 + 4 * j + x, last);
+        const int rk = min(t + 8 * x + m8, last), rv = min(t + 16 * (x >> 1) + 4 * j + 2 * (x & 1) + hi8, last);
         r.k[x] = a.idx ? idx[rk] : rk;
         r.v[x] = a.idx ? idx[rv] : rv;
       }
@@ -309,44 +329,40 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   };
   auto load = [&](int t, const Kv8Rows& r, Kv8Tile& x) {
     if (MODE == kContiguous) {
-      const bool whole = t + 32 <= main_end;
+      const int n = min(32, main_end - t);  // rows of the tile; none: past the last tile
+      const uint32_t bytes = n > 0 ? (uint32_t)(n - 1) * ts + kD : 0;
+      const __amdgpu_buffer_rsrc_t kr = as_buffer(kb + (int64_t)t * ts, bytes), vr = as_buffer(vb + (int64_t)t * ts, bytes);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        int rk = 8 * i + m8, rv = 16 * hi8 + 4 * j + i;
-        if (!whole) {
-          rk = min(rk, last - t);
-          rv = min(rv, last - t);
-        }
-        x.k[i] = load_stream16(kb + (int64_t)t * ts + (uint32_t)rk * ts + kcol);
-        x.v[i] = load_stream16(vb + (int64_t)t * ts + (uint32_t)rv * ts + vcol);
+      for (int i = 0; i < 4; ++i) x.k[i] = buffer16(kr, koff[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.v[i] = buffer16(vr, voff[i]);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {  // the same four bytes for every lane
+        const int64_t so = (int64_t)((t + 16 * s) >> a.block_shift) * c.scale_block_stride;
+        x.ks[s] = buffer4(as_buffer(ksb + so, n > 16 * s ? 4 : 0), 0);
+        x.vs[s] = buffer4(as_buffer(vsb + so, n > 16 * s ? 4 : 0), 0);
       }
-      const int blk = min(t + 16 * (j & 1), last) >> a.block_shift;
-      x.sc = (j < 2 ? ksb : vsb)[(int64_t)blk * c.scale_block_stride];
       x.ok = 3;
     } else if (MODE == kPaged) {
-      int64_t base[2];
       x.ok = 0;
-      int64_t sbase = 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int u = min(t + 16 * s, last) & ~15;
+        const int u = t + 16 * s, n = min(16, main_end - u);
         const bool in = (uint32_t)r.page[s] < (uint32_t)c.num_pages;
         const int64_t p = in ? r.page[s] : 0;
         const int slot = slot_of(u);
-        base[s] = p * c.page_stride + (int64_t)slot * ts;
-        const int64_t sb = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride;
-        if ((j & 1) == s) sbase = sb;
+        const int64_t base = p * c.page_stride + (int64_t)slot * ts;
+        const uint32_t bytes = in && n > 0 ? (uint32_t)(n - 1) * ts + kD : 0;
+        const __amdgpu_buffer_rsrc_t kr = as_buffer(kb + base, bytes), vr = as_buffer(vb + base, bytes);
+        x.k[2 * s] = buffer16(kr, koff[2 * s]);
+        x.k[2 * s + 1] = buffer16(kr, koff[2 * s + 1]);
+        x.v[2 * s] = buffer16(vr, voff[2 * s]);
+        x.v[2 * s + 1] = buffer16(vr, voff[2 * s + 1]);
+        const int64_t so = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride;
+        x.ks[s] = buffer4(as_buffer(ksb + so, bytes ? 4 : 0), 0);
+        x.vs[s] = buffer4(as_buffer(vsb + so, bytes ? 4 : 0), 0);
         x.ok |= in ? 1u << s : 0u;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // rows past the last one: the last one again (its tile and page are those of u)
-        const int sk = i >> 1, rk = min((8 * i + m8) & 15, (last - t - 16 * sk < 0 ? last & 15 : min(15, last - t - 16 * sk)));
-        const int lv = last - t - 16 * hi8, rv = min(4 * j + i, lv < 0 ? last & 15 : min(15, lv));
-        x.k[i] = load_stream16(kb + base[sk] + (uint32_t)rk * ts + kcol);
-        x.v[i] = load_stream16(vb + (hi8 ? base[1] : base[0]) + (uint32_t)rv * ts + vcol);
-      }
-      x.sc = (j < 2 ? ksb : vsb)[sbase];
     } else {
       // an entry outside the request's room is read as row 0 and takes no part
       auto at = [&](int t_, int64_t* row, int64_t* scale) -> bool {
@@ -377,7 +393,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
         x.v[i] = load_stream16(vb + row + vcol);
       }
       x.ok = at(r.s, &row, &scale);
-      x.sc = (lane < 32 ? ksb : vsb)[scale];
+      x.ks[0] = (lane < 32 ? ksb : vsb)[scale];  // lanes 0..31: K scales of rows l, 32..63: V scales of rows l - 32
     }
   };
 
@@ -436,7 +452,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     if (MODE == kGather) {
       // every lane has the scale of one row: the wave's 256 bytes of LDS hand the rows' four to their lane row
       const bool okl = x.ok != 0;
-      sstage[lane] = lane < 32 ? (okl ? x.sc : 0.f) : (okl ? x.sc : 0.f);
+      sstage[lane] = okl ? x.ks[0] : 0.f;
       const uint64_t oks = __ballot(okl);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -454,7 +470,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
         whole = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!((oks >> (16 * hi8 + 4 * j + i)) & 1)) x.v[i] = make_uint4(0, 0, 0, 0);
+          if (!((oks >> (16 * (i >> 1) + 4 * j + 2 * (i & 1) + hi8)) & 1)) x.v[i] = make_uint4(0, 0, 0, 0);
         x.ok = (uint32_t)oks;
       } else {
         x.ok = 0xffffffffu;
@@ -462,12 +478,10 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     } else {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const float kk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x.sc), 16 * s));
-        const float vv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x.sc), 32 + 16 * s));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          ks[s][i] = kk;
-          vs[s][i] = vv;
+          ks[s][i] = x.ks[s];
+          vs[s][i] = x.vs[s];
         }
       }
       if (MODE == kPaged && x.ok != 3) {
@@ -476,10 +490,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
         for (int s = 0; s < 2; ++s)
           if (!((x.ok >> s) & 1)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              vs[s][i] = 0.f;
-              if (hi8 == s) x.v[i] = make_uint4(0, 0, 0, 0);
-            }
+            for (int i = 0; i < 4; ++i) vs[s][i] = 0.f;  // (its codes have come as zeros)
           }
       }
     }
@@ -538,14 +549,18 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       split_p((const BF16*)nullptr, w, pa + 2 * s);
     }
     const uint4 pf = make_uint4(pa[0], pa[1], pa[2], pa[3]);
-    // lane m keeps eight elements of the rows of both sixteens
-    uint32_t lo[4][2], up[4][2];  // [row i][dword]: rows 4j + i of the lower and upper sixteen
+    // lane m keeps eight elements of its lane row's four rows of either sixteen
+    uint32_t lo[4][2], up[4][2];  // [row 4j + i][dword] of the lower and the upper sixteen
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lo[i][0] = take8<0xC>(x.v[i].x, x.v[i].z);
-      lo[i][1] = take8<0xC>(x.v[i].y, x.v[i].w);
-      up[i][0] = take8<0x3>(x.v[i].z, x.v[i].x);
-      up[i][1] = take8<0x3>(x.v[i].w, x.v[i].y);
+    for (int i = 0; i < 2; ++i) {
+      lo[2 * i][0] = take8<0xC>(x.v[i].x, x.v[i].z);
+      lo[2 * i][1] = take8<0xC>(x.v[i].y, x.v[i].w);
+      lo[2 * i + 1][0] = take8<0x3>(x.v[i].z, x.v[i].x);
+      lo[2 * i + 1][1] = take8<0x3>(x.v[i].w, x.v[i].y);
+      up[2 * i][0] = take8<0xC>(x.v[2 + i].x, x.v[2 + i].z);
+      up[2 * i][1] = take8<0xC>(x.v[2 + i].y, x.v[2 + i].w);
+      up[2 * i + 1][0] = take8<0x3>(x.v[2 + i].z, x.v[2 + i].x);
+      up[2 * i + 1][1] = take8<0x3>(x.v[2 + i].w, x.v[2 + i].y);
     }
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
@@ -585,14 +600,18 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       } else {
         rows_of(t + 128, r1);
         load(t, r0, x0);
-        while (true) {  // tile t + 128 in flight while t is consumed; past the last one, the last one again
-          load(min(t + 128, t_last), r1, x1);
-          rows_of(min(t + 256, t_last), r0);
+        while (true) {  // tile t + 128 in flight while t is consumed; past the last one nothing is fetched.  The loads stay
+          __builtin_amdgcn_sched_barrier(0);  // where they are: among the arithmetic they would wait for its data.
+          load(t + 128, r1, x1);
+          rows_of(t + 256, r0);
+          __builtin_amdgcn_sched_barrier(0);
           compute(t, x0, sstage);
           t += 128;
           if (t > t_last) break;
-          load(min(t + 128, t_last), r0, x0);
-          rows_of(min(t + 256, t_last), r1);
+          __builtin_amdgcn_sched_barrier(0);
+          load(t + 128, r0, x0);
+          rows_of(t + 256, r1);
+          __builtin_amdgcn_sched_barrier(0);
           compute(t, x1, sstage);
           t += 128;
           if (t > t_last) break;
