@@ -39,7 +39,7 @@ struct Kv8Attn {
   float* logits;    // [batch][logit_heads][logits_stride], natural units
   int64_t logits_stride;
   int32_t batch;
-  int32_t target;     // shares the rows of the call are cut into, about
+  float inv_target, inv_fine;  // 1 / full shares that fit next to the requests' last, short ones (half a share each)
   int32_t most_rows;  // of a share (its logits are staged in LDS)
   int32_t items;      // shares the grid and the partial results have room for
   int32_t fine;       // long shares of a batch are cut in three
@@ -92,10 +92,22 @@ __device__ __forceinline__ int lane_scan(int x) {
   return x;
 }
 __device__ __forceinline__ int share_rows(int total, const Kv8Attn& a) {
-  uint32_t r = (((uint32_t)total + a.target - 1) / (uint32_t)a.target + 63) & ~63u;
-  if (a.fine && r > kFineRows) r = max((r / 3 + 63) & ~63u, kFineRows);
+  // (less than one off where it is not cut to most_rows anyway: at or above total / target)
+  uint32_t r = ((uint32_t)((float)total * a.inv_target) + 64) & ~63u;
+  if (a.fine && r > kFineRows) r = max(((uint32_t)((float)total * a.inv_fine) + 64) & ~63u, kFineRows);
   return r < kLeastRows ? kLeastRows : r > (uint32_t)a.most_rows ? a.most_rows : (int)r;
 }
+// x / rows, rounded up: quotients below 2^16 from a product with the reciprocal, put right by one step
+__device__ __forceinline__ int shares_up(int x, int rows) {
+  if (x <= 0) return 0;
+  int q = (int)((float)(x - 1) * __builtin_amdgcn_rcpf((float)rows));
+  const int r = x - 1 - q * rows;
+  q += r >= rows ? 1 : r < 0 ? -1 : 0;
+  return q + 1;
+}
+// The scored rows [0, A) and the rest [A, L) are cut separately: no share holds both.
+__device__ __forceinline__ int shares_of(int rows, int A, int L) { return shares_up(A, rows) + shares_up(L - A, rows); }
+
 __device__ __forceinline__ void request_lens(const Kv8Attn& a, int b, int* main_len, int* L, int* A) {
   *main_len = clamp_len(a.lens, b, a.max_len);
   *L = *main_len + (a.max_tail_len ? clamp_len(a.tail_lens, b, a.max_tail_len) : 0);
@@ -125,7 +137,7 @@ __device__ __forceinline__ bool find_share(const Kv8Attn& a, int item, int reque
     s->b = 0;
     s->first = 0;
     s->index = item;
-    s->count = rl_num_splits(s->rows, s->A, s->L);
+    s->count = shares_of(s->rows, s->A, s->L);
     return item < s->count;
   }
   int main_len = 0, L = 0, A = 0, total = 0;
@@ -141,7 +153,7 @@ __device__ __forceinline__ bool find_share(const Kv8Attn& a, int item, int reque
       main_len = L = A = 0;
       if (base + lane < a.batch) request_lens(a, base + lane, &main_len, &L, &A);
     }
-    const int n = rl_num_splits(s->rows, A, L);
+    const int n = shares_of(s->rows, A, L);
     const int x = lane_scan(n);
     const uint64_t hit = __ballot(item >= 0 ? before + x > item : base + lane == request);
     if (hit) {
@@ -263,6 +275,15 @@ template <typename T, typename F, int MODE, bool LOGITS>
 __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv8_split(Kv8Attn a) {
   extern __shared__ float lds[];
   const okv_kv8_cache_t& c = a.c;
+  if constexpr (MODE != kPaged) {  // one batch of scalar loads instead of a round trip before each first use (the paged mode's
+    // page descriptors leave too few scalar registers for that: 131 against 121 us)
+    fetch_now(c.k_codes); fetch_now(c.v_codes); fetch_now(c.k_scale); fetch_now(c.v_scale); fetch_now(c.token_stride);
+    fetch_now(c.head_stride); fetch_now(c.batch_stride); fetch_now(c.scale_block_stride); fetch_now(c.scale_head_stride);
+    fetch_now(c.scale_batch_stride); fetch_now(a.q); fetch_now(a.lens); fetch_now(a.idx); fetch_now(a.idx_stride);
+    fetch_now(a.batch); fetch_now(a.inv_target); fetch_now(a.max_len); fetch_now(a.max_tail_len); fetch_now(a.tail_lens);
+    fetch_now(a.late[0]); fetch_now(a.late[1]); fetch_now(a.late_token_stride); fetch_now(a.late_head_stride);
+    fetch_now(a.late_batch_stride);
+  }
   const int G = a.group;
   // workgroups go to the XCDs round-robin: the kv heads of a share run on one XCD, one after the other, so that rows
   // stored head by head next to each other (pools) are fetched together
@@ -271,7 +292,11 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   if (!find_share(a, (int)((turn / c.num_kv_heads) * 8 + (blockIdx.x & 7)), 0, &sh)) return;
   const int b = sh.b, main_len = sh.main_len, L = sh.L, A = LOGITS ? sh.A : 0;
   int begin, end;
-  rl_split_range(sh.index, sh.rows, A, L, &begin, &end);
+  {
+    const int nA = LOGITS ? shares_up(A, sh.rows) : 0;
+    begin = sh.index < nA ? sh.index * sh.rows : A + (sh.index - nA) * sh.rows;
+    end = min(begin + sh.rows, sh.index < nA ? A : L);
+  }
   if (begin >= end && !a.direct) return;  // (a request without rows gets its zeros below)
   // rows [0, closed) are codes, the rest 16-bit rows: the open block, or the tail
   const int closed = a.sparse || !c.open_k ? main_len : main_len >> a.block_shift << a.block_shift;
@@ -814,7 +839,7 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
   if ((int)(blockIdx.x - a.hq) * 256 * TPT >= A) return;
   const bool soft = a.normalise == OKV_NORM_SOFTMAX, is_max = a.head_reduce == OKV_REDUCE_MAX;
   if (soft) {  // eight threads per head
-    const int nA = (A + sh.rows - 1) / sh.rows, sub = tid & 7;
+    const int nA = shares_up(A, sh.rows), sub = tid & 7;
     for (int h0 = 0; h0 < a.hq; h0 += 32) {
       const int h = h0 + (tid >> 3);
       float m = -INFINITY, den = 0.f;
@@ -879,12 +904,12 @@ static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // cut in three (sixteen requests of 8K..32K tokens: 136 us in one round, 124 / 121 / 122 / 127 / 136 in 2 / 3 / 4 / 6 / 8);
 // short ones are not: a workgroup's first microseconds move nothing.  A scored share stages its logits in LDS, up to 32 KB.
 static void kv8_cut(bool gather, int batch, int hkv, int group, int64_t rows, int max_score, bool folded, int* target, int* most, int* items) {
-  *target = std::max(1, 256 * (gather ? kGatherResident : 2) / hkv);
+  *target = std::max(1, 256 * (gather ? kGatherResident : 2) / hkv);  // shares of one round
   *most = max_score > 0 ? 32768 / 4 / (folded ? 1 : group) / 64 * 64 : 8192;
   const int64_t all = std::max<int64_t>(rows, 1) * batch;
   const bool fine = !gather && batch > 1;
   const int64_t n = std::min((all + kLeastRows - 1) / kLeastRows,
-                             std::max<int64_t>((fine ? 3 : 1) * (int64_t)*target, (all + *most - 1) / *most));
+                             std::max<int64_t>((fine ? 3 : 1) * (int64_t)*target + 1, (all + *most - 1) / *most));
   *items = (int)std::min<int64_t>(n + (int64_t)batch * (max_score > 0 ? 2 : 1), 1 << 30);
 }
 
@@ -915,7 +940,8 @@ static size_t kv8_workspace(bool gather, int batch, int hq, int hkv, int64_t row
   if (a) {
     p = (char*)align256((size_t)p);
     a->batch = batch;
-    a->target = target;
+    a->inv_target = 1.f / (float)std::max(target - batch / 2, (target + 1) / 2);
+    a->inv_fine = 1.f / (float)std::max(3 * target - batch / 2, target);
     a->most_rows = most;
     a->items = items;
     a->fine = !gather && batch > 1;
