@@ -422,7 +422,7 @@ typedef struct okv_kv8_cache {
 /*
  * Appends new_len rows of K and V per request behind its first `start` rows: the blocks they
  * complete become codes, the rest waits in the open buffers.  New element (b, r, g, d) at
- * new_k + b*new_batch_stride + r*new_token_stride + g*new_head_stride + d (strides in elements,
+ * new_k + b*k_batch_stride + r*k_token_stride + g*k_head_stride + d, of V likewise (strides in elements,
  * multiples of 8, 16-byte aligned).  starts (device int32[batch]) or start for every request;
  * new_lens (device int32[batch]) or max_new for every request.  close = 1 quantises a short last
  * block too (over its own rows; the rows behind it are left as they were): with close, or without
@@ -430,9 +430,9 @@ typedef struct okv_kv8_cache {
  * close must be 1 or every request must end at a block's border (max_new a multiple, new_lens NULL).
  * A request whose rows would not fit (start < 0, or start + new_len beyond its room) is left as it was.
  */
-int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, const void* new_v,
-                   int64_t new_token_stride, int64_t new_head_stride, int64_t new_batch_stride,
-                   const int32_t* starts, int32_t start, const int32_t* new_lens, int32_t max_new,
+int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, int64_t k_token_stride,
+                   int64_t k_head_stride, int64_t k_batch_stride, const void* new_v, int64_t v_token_stride,
+                   int64_t v_head_stride, int64_t v_batch_stride, const int32_t* starts, int32_t start, const int32_t* new_lens, int32_t max_new,
                    int32_t close, int32_t batch, okv_stream_t stream);
 
 /* Scratch of the two attention calls: `max_rows` is max_seq_len, or max_sel_len + max_tail_len;

@@ -203,7 +203,7 @@ def _declare(l):
     l.okv_silu_mul.argtypes = [vp, vp, i64, i32, vp, vp]
     cache, pool, bufs = C.POINTER(KV8Cache), C.POINTER(PagePool), C.POINTER(PageBuffer)
     for name, args in (
-        ("okv_kv8_append", [cache, vp, vp, i64, i64, i64, vp, i32, vp, i32, i32, i32, vp]),
+        ("okv_kv8_append", [cache, vp, i64, i64, i64, vp, i64, i64, i64, vp, i32, vp, i32, i32, i32, vp]),
         ("okv_kv8_read", [cache, vp, i64, i32, vp, i32, i32, vp, vp, i64, i64, i64, vp]),
         ("okv_kv8_workspace_bytes", [i32, i32, i32, i32, i32, C.POINTER(sz)]),
         ("okv_kv8_dense_attn", [vp, i32, cache, vp, i32, i32, f32, vp, vp, i32, i32, i32, vp, i64, vp, sz, vp]),

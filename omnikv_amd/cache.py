@@ -86,12 +86,61 @@ class _Store:
         return self.k[:, :, lo:hi], self.v[:, :, lo:hi]
 
 
+class _Store8:
+    """K and V of one layer as 8-bit codes with a scale per block of tokens and head (ops.KV8).  An open store holds the
+    rows of its last, not yet full block in 16 bits; a closed one (a layer that reads selected rows: its store is the prompt) takes
+    one append and quantises the short last block too."""
+
+    def __init__(self, bsz, capacity, hkv, dtype, device, fmt, block, closed):
+        self.kv = ops.KV8.empty(bsz, hkv, capacity, fmt, block, None if closed else dtype, device)
+        self.dtype, self.closed, self.fmt = dtype, closed, fmt
+        self.len = 0
+
+    @property
+    def capacity(self):
+        return self.kv.capacity
+
+    def reserve(self, n):
+        if n <= self.capacity:
+            return
+        old = self.kv
+        hkv, blocks = old.num_kv_heads, old.capacity // old.block
+        new = ops.KV8.empty(old.bsz, hkv, max(n, int(old.capacity * 1.5) + 64), self.fmt, old.block,
+                            None if self.closed else self.dtype, old.device)
+        for name in ("k", "v"):
+            getattr(new, name).view(torch.uint8)[:, :, : old.capacity].copy_(getattr(old, name).view(torch.uint8))
+            getattr(new, name + "_scale")[:, :, :blocks].copy_(getattr(old, name + "_scale"))
+            if not self.closed:
+                getattr(new, "open_" + name).copy_(getattr(old, "open_" + name))
+        self.kv = new
+
+    def append(self, key_states, value_states):
+        n = key_states.shape[2]
+        if self.closed and self.len:
+            raise NotImplementedError("an 8-bit layer that reads selected rows takes its prompt in one prefill call")
+        self.reserve(self.len + n)
+        ops.kv8_append(self.kv, key_states, value_states, self.len, close=self.closed)
+        self.len += n
+
+    def read(self, idx=None):
+        """The stored values in 16 bits, (bsz, Hkv, n, D): rows idx, or all of them."""
+        return ops.kv8_read(self.kv, self.dtype, idx=idx, seq_len=self.len)
+
+
 class OmniKVMultiStageCache:
     """Drop-in for the reference class of the same name (default DenseMore=True)."""
 
     def __init__(self, full_attn_layers: List, num_hidden_layers, num_wait_load_layers=2, real_offload=True,
                  max_new_tokens: int = 1024, offload_mode: str = "zero_copy", cpu_num_threads: int = 8,
-                 skip_threshold: Optional[float] = None):
+                 skip_threshold: Optional[float] = None, kv_format: Optional[str] = None, kv_block: int = 64):
+        """kv_format "e4m3" or "int8": K and V of every layer in 8 bits, one scale per kv_block tokens and head
+        (generated tokens behind a selection, and the last block of the others, in 16); GPU resident only."""
+        if kv_format is not None:
+            if kv_format not in ops.KV8_FORMATS:
+                raise ValueError(f"kv_format must be one of {sorted(ops.KV8_FORMATS)} or None")
+            if real_offload:
+                raise NotImplementedError("the host tier keeps 16-bit rows: an 8-bit cache takes real_offload=False")
+        self.kv_format, self.kv_block = kv_format, kv_block
         self.stage = "prefill"
         # lazy re-selection (OmniKVLazyCache.set_out_idx, modeling/spec_cache.py:539-557): a new
         # selection whose IoU with the one in use exceeds the threshold is dropped
@@ -148,7 +197,12 @@ class OmniKVMultiStageCache:
         st = self._store.get(layer_idx)
         if st is None:
             b, hkv, _, d = like.shape
-            st = _Store(b, n_first + self.max_new_tokens, hkv, d, like.dtype, like.device)
+            if self.kv_format is not None:
+                closed = self.layer_state[layer_idx][0]
+                st = _Store8(b, n_first + (0 if closed else self.max_new_tokens), hkv, like.dtype, like.device, self.kv_format,
+                             self.kv_block, closed)
+            else:
+                st = _Store(b, n_first + self.max_new_tokens, hkv, d, like.dtype, like.device)
             self._store[layer_idx] = st
         return st
 
@@ -161,7 +215,7 @@ class OmniKVMultiStageCache:
             h = self._host_kv[layer_idx]
             self.key_cache[layer_idx] = h[:, 0].permute(1, 0, 2)[None]
             self.value_cache[layer_idx] = h[:, 1].permute(1, 0, 2)[None]
-        else:
+        elif self.kv_format is None:  # (codes are no tensors of K and V: their layers' entries stay None)
             self.key_cache[layer_idx], self.value_cache[layer_idx] = self._store[layer_idx].views()
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
@@ -182,7 +236,7 @@ class OmniKVMultiStageCache:
         if self._static:
             return
         any_store = next(iter(self._store.values()))
-        dev = any_store.k.device
+        dev = any_store.k.device if self.kv_format is None else any_store.kv.device
         n = self._seen_tokens
         self._finish_prefill_offload()
         for layer_idx, sparse in ((i, s[0]) for i, s in self.layer_state.items()):
@@ -193,7 +247,10 @@ class OmniKVMultiStageCache:
                         b, hkv, d, dt = 1, host.shape[2], host.shape[3], host.dtype
                     else:
                         st = self._store[layer_idx]
-                        (b, hkv, _, d), dt = st.k.shape, st.k.dtype
+                        if self.kv_format is not None:
+                            b, hkv, d, dt = st.kv.bsz, st.kv.num_kv_heads, 128, st.dtype
+                        else:
+                            (b, hkv, _, d), dt = st.k.shape, st.k.dtype
                     self._tail[layer_idx] = _Store(b, self.max_new_tokens, hkv, d, dt, dev)
             else:
                 self._store[layer_idx].reserve(n + self.max_new_tokens)
@@ -201,6 +258,7 @@ class OmniKVMultiStageCache:
         t0 = tails[0] if tails else 0
         self._pos = torch.tensor([n], dtype=torch.int64, device=dev)
         self._len32 = torch.tensor([n + 1], dtype=torch.int32, device=dev)
+        self._pos32 = torch.tensor([n], dtype=torch.int32, device=dev) if self.kv_format is not None else None
         self._tail_pos = torch.tensor([t0], dtype=torch.int64, device=dev)
         self._tail_len32 = torch.tensor([t0 + 1], dtype=torch.int32, device=dev)
         # how many static steps the preallocated buffers take: every step writes one row at
@@ -236,6 +294,8 @@ class OmniKVMultiStageCache:
         dense_cap, tail_cap = self._static_caps
         self._pos.add_(1).clamp_(max=dense_cap - 1)
         self._len32.add_(1).clamp_(max=dense_cap)
+        if self._pos32 is not None:
+            self._pos32.add_(1).clamp_(max=dense_cap - 1)
         self._tail_pos.add_(1).clamp_(max=tail_cap - 1)
         self._tail_len32.add_(1).clamp_(max=tail_cap)
 
@@ -247,6 +307,9 @@ class OmniKVMultiStageCache:
         sparse = self.layer_state[layer_idx][0]
         if self._static:
             st = self._tail[layer_idx] if sparse else self._store[layer_idx]
+            if isinstance(st, _Store8):
+                ops.kv8_append(st.kv, key_states, value_states, self._pos32)
+                return
             where = self._tail_pos if sparse else self._pos
             st.k.index_copy_(2, where, key_states)
             st.v.index_copy_(2, where, value_states)
@@ -322,6 +385,12 @@ class OmniKVMultiStageCache:
             self._seen_tokens += 1
         sparse = self.layer_state[layer_idx][0]
         st = self._tail[layer_idx] if sparse else self._store[layer_idx]
+        if isinstance(st, _Store8):
+            hkv = st.kv.num_kv_heads
+            q, k = ops.rope(q_lin, k_lin, cos, sin, num_q_heads, hkv)
+            v = v_lin.view(v_lin.shape[0], 1, hkv, -1).transpose(1, 2)
+            ops.kv8_append(st.kv, k, v, self._pos32)
+            return q
         return ops.rope_append(q_lin, k_lin, v_lin, cos, sin, num_q_heads, st.k.shape[1], st.k, st.v,
                                self._tail_pos if sparse else self._pos)
 
@@ -336,6 +405,8 @@ class OmniKVMultiStageCache:
             pk, pv = self._materialised_part(layer_idx)
             return (torch.cat([pk, self.tail_k[layer_idx]], dim=-2),
                     torch.cat([pv, self.tail_v[layer_idx]], dim=-2))
+        if self.kv_format is not None:
+            return self._store[layer_idx].read()
         return self.key_cache[layer_idx], self.value_cache[layer_idx]
 
     def set_idx_on_gpu(self, idx: torch.Tensor, sel_layer_idx: int) -> None:
@@ -554,6 +625,8 @@ class OmniKVMultiStageCache:
                     part = part.index_select(1, order)
                 pk = part[:, :, 0].permute(0, 2, 1, 3)
                 pv = part[:, :, 1].permute(0, 2, 1, 3)
+            elif self.kv_format is not None:
+                pk, pv = self._store[layer_idx].read(idx32)
             else:
                 kview, vview = self._store[layer_idx].views(0, self._prefill_rows(layer_idx))
                 pk = ops.gather_rows(kview, idx32)
@@ -580,10 +653,15 @@ class OmniKVMultiStageCache:
             st = self._store[layer_idx]
             if self.layer_state[layer_idx][0]:
                 tl = self._tail[layer_idx]
+                if self.kv_format is not None:
+                    return ops.kv8_sparse_attn(query_states, st.kv, idx=self._idx[self.layer_state[layer_idx][1]], tail_k=tl.k,
+                                               tail_v=tl.v, tail_len=tl.capacity, tail_lens=self._tail_len32, scale=scale)
                 kview, vview = st.views()
                 return ops.sparse_attn(query_states, kview, vview, idx=self._idx[self.layer_state[layer_idx][1]],
                                        tail_k=tl.k, tail_v=tl.v, tail_len=tl.capacity, tail_lens=self._tail_len32,
                                        scale=scale)
+            if self.kv_format is not None:
+                return ops.kv8_dense_attn(query_states, st.kv, seq_lens=self._len32, scale=scale)
             return ops.dense_attn(query_states, st.k, st.v, seq_len=st.capacity, seq_lens=self._len32, scale=scale)
         if self.layer_state[layer_idx][0] and self.stage != "prefill":
             sel = self.layer_state[layer_idx][1]
@@ -594,8 +672,13 @@ class OmniKVMultiStageCache:
                 pk = part[:, :, 0].permute(0, 2, 1, 3)
                 pv = part[:, :, 1].permute(0, 2, 1, 3)
                 return ops.sparse_attn(query_states, pk, pv, tail_k=tk, tail_v=tv, scale=scale)
+            if self.kv_format is not None:
+                return ops.kv8_sparse_attn(query_states, self._store[layer_idx].kv, idx=self._idx[sel], tail_k=tk, tail_v=tv,
+                                           scale=scale)
             kview, vview = self._store[layer_idx].views()
             return ops.sparse_attn(query_states, kview, vview, idx=self._idx[sel], tail_k=tk, tail_v=tv, scale=scale)
+        if self.kv_format is not None:
+            return ops.kv8_dense_attn(query_states, self._store[layer_idx].kv, seq_len=self._store[layer_idx].len, scale=scale)
         kview, vview = self._store[layer_idx].views()
         return ops.dense_attn(query_states, kview, vview, scale=scale)
 
@@ -608,6 +691,7 @@ class OmniKVMultiStageCache:
         set_idx_on_gpu.  In static decode everything has a fixed shape and lands in a fixed index
         buffer, so the step can be captured.  Returns the int32 (bsz, k) selection."""
         from . import selector
+        self._require_16_bit(selector_cls)
         if not self._static:
             idx = selector.select_from_query(query_states, self.key_cache[layer_idx], num_selected_tokens, consider_len,
                                              selector_cls)
@@ -631,6 +715,11 @@ class OmniKVMultiStageCache:
             self._stage_static(layer_idx, buf)
         return buf
 
+    def _require_16_bit(self, selector_cls: str) -> None:
+        if self.kv_format is not None:
+            raise NotImplementedError(f"selector {selector_cls!r} scores 16-bit keys: an 8-bit cache takes the selectors of "
+                                      f"attend_and_select ({', '.join(ops.SELECTOR_MODES)})")
+
     def attend_and_select_window(self, query_states: torch.Tensor, query_window: torch.Tensor, layer_idx: int,
                                  num_selected_tokens: int, consider_len: int, selector_cls: str, forced_tail: int = 0,
                                  scale: Optional[float] = None):
@@ -639,6 +728,7 @@ class OmniKVMultiStageCache:
         instead of three.  query_states: (bsz, Hq, 1, D), the attention's query; query_window:
         (bsz, Hq, W, D), rotated.  Returns (attention output, idx int32 (bsz, k)).  Operands the
         kernel does not take (fp32, more than 64 window columns per kv head) go the separate way."""
+        self._require_16_bit(selector_cls)
         st = self._store[layer_idx]
         if not ops.window_supported(query_window, st.k):
             idx = self.select_with_query(query_window, layer_idx, num_selected_tokens, consider_len, selector_cls,
@@ -684,16 +774,25 @@ class OmniKVMultiStageCache:
             if buf is None or buf.shape[1] != k:
                 buf = torch.empty((query_states.shape[0], k), dtype=torch.int32, device=query_states.device)
                 self._idx[layer_idx] = buf  # the sparse layers keep reading this very buffer
-            out, _, _ = ops.dense_attn(query_states, st.k, st.v, seq_len=st.capacity, seq_lens=self._len32,
-                                       selector=selector_cls, score_len=consider_len, scale=scale, select_k=k,
-                                       idx_out=buf)
+            if self.kv_format is not None:
+                out, _, _ = ops.kv8_dense_attn(query_states, st.kv, seq_lens=self._len32, selector=selector_cls,
+                                               score_len=consider_len, scale=scale, select_k=k, idx_out=buf)
+            else:
+                out, _, _ = ops.dense_attn(query_states, st.k, st.v, seq_len=st.capacity, seq_lens=self._len32,
+                                           selector=selector_cls, score_len=consider_len, scale=scale, select_k=k,
+                                           idx_out=buf)
             self._sel_gen[layer_idx] = self._sel_gen.get(layer_idx, 0) + 1  # same buffer, new selection
             if self.real_offload:
                 self._stage_static(layer_idx, buf)
             return out, buf
-        kview, vview = self._store[layer_idx].views()
-        out, _, idx = ops.dense_attn(query_states, kview, vview, selector=selector_cls, score_len=consider_len,
-                                     scale=scale, select_k=k)
+        if self.kv_format is not None:
+            st = self._store[layer_idx]
+            out, _, idx = ops.kv8_dense_attn(query_states, st.kv, seq_len=st.len, selector=selector_cls, score_len=consider_len,
+                                             scale=scale, select_k=k)
+        else:
+            kview, vview = self._store[layer_idx].views()
+            out, _, idx = ops.dense_attn(query_states, kview, vview, selector=selector_cls, score_len=consider_len,
+                                         scale=scale, select_k=k)
         self.set_idx_on_gpu(idx, layer_idx)
         return out, idx
 

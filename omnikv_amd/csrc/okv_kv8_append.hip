@@ -48,7 +48,7 @@ int kv8_validate(const okv_kv8_cache_t* c, const char* what) {
 struct AppendArgs {
   okv_kv8_cache_t c;
   const void* rows[2];  // new K, new V
-  int64_t token_stride, head_stride, batch_stride;
+  int64_t token_stride[2], head_stride[2], batch_stride[2];
   const int32_t* starts;
   const int32_t* new_lens;
   int32_t start, max_new, close;
@@ -71,7 +71,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   const int end = start + n;
   const int first = start / B, blk = first + blockIdx.x;
   if (blk * B >= end) return;
-  const T* src = reinterpret_cast<const T*>(a.rows[is_v]) + (int64_t)b * a.batch_stride + (int64_t)g * a.head_stride;
+  const T* src = reinterpret_cast<const T*>(a.rows[is_v]) + (int64_t)b * a.batch_stride[is_v] + (int64_t)g * a.head_stride[is_v];
+  const int64_t row_stride = a.token_stride[is_v];
   T* open = reinterpret_cast<T*>(is_v ? c.open_v : c.open_k);
   if (open) open += (int64_t)b * c.open_batch_stride + (int64_t)g * c.open_head_stride;
   const int tid = threadIdx.x, col = tid & 15, row = tid >> 4;
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
       const int r = 16 * p + row, t = blk * B + r;
       x[p] = make_uint4(0, 0, 0, 0);
       if (r < B && t < end) {
-        const T* q = t >= start ? src + (int64_t)(t - start) * a.token_stride : open + (int64_t)r * c.open_token_stride;
+        const T* q = t >= start ? src + (int64_t)(t - start) * row_stride : open + (int64_t)r * c.open_token_stride;
         x[p] = *reinterpret_cast<const uint4*>(q + 8 * col);
       }
       float v[8];
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   const int lo = max(start, end / B * B);
   for (int t = lo + row; t < end; t += 16)
     *reinterpret_cast<uint4*>(open + (int64_t)(t % B) * c.open_token_stride + 8 * col) =
-        *reinterpret_cast<const uint4*>(src + (int64_t)(t - start) * a.token_stride + 8 * col);
+        *reinterpret_cast<const uint4*>(src + (int64_t)(t - start) * row_stride + 8 * col);
 }
 
 struct ReadArgs {
@@ -179,11 +180,6 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
   for (int i = 0; i < 8; ++i) store1(dst + i, v[i]);
 }
 
-template <typename A>
-static bool wide_rows(const A& a) {
-  return a.token_stride % 8 == 0 && a.head_stride % 8 == 0 && a.batch_stride % 8 == 0;
-}
-
 }  // namespace okv
 
 using namespace okv;
@@ -201,17 +197,20 @@ using namespace okv;
 
 extern "C" {
 
-int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, const void* new_v, int64_t new_token_stride,
-                   int64_t new_head_stride, int64_t new_batch_stride, const int32_t* starts, int32_t start,
+int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, int64_t k_token_stride, int64_t k_head_stride,
+                   int64_t k_batch_stride, const void* new_v, int64_t v_token_stride, int64_t v_head_stride,
+                   int64_t v_batch_stride, const int32_t* starts, int32_t start,
                    const int32_t* new_lens, int32_t max_new, int32_t close, int32_t batch, okv_stream_t stream) {
   int rc = kv8_validate(cache, "okv_kv8_append");
   if (rc) return rc;
   const int B = cache->block_tokens;
   OKV_REQUIRE(new_k && new_v, OKV_ERR_INVALID, "new_k or new_v is NULL");
   OKV_REQUIRE(batch >= 1 && max_new >= 0, OKV_ERR_INVALID, "bad batch or length");
-  AppendArgs a{*cache, {new_k, new_v}, new_token_stride, new_head_stride, new_batch_stride, starts, new_lens, start, max_new,
-               close ? 1 : 0};
-  OKV_REQUIRE(((uintptr_t)new_k & 15) == 0 && ((uintptr_t)new_v & 15) == 0 && wide_rows(a), OKV_ERR_INVALID,
+  const AppendArgs a{*cache, {new_k, new_v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
+                     {k_batch_stride, v_batch_stride}, starts, new_lens, start, max_new, close ? 1 : 0};
+  OKV_REQUIRE(((uintptr_t)new_k & 15) == 0 && ((uintptr_t)new_v & 15) == 0 &&
+                  ((k_token_stride | k_head_stride | k_batch_stride | v_token_stride | v_head_stride | v_batch_stride) & 7) == 0,
+              OKV_ERR_INVALID,
               "new rows: 16-byte aligned, strides multiples of 8 elements");
   if (!starts)
     OKV_REQUIRE(start >= 0 && (new_lens || (int64_t)start + max_new <= kv8_room(*cache)), OKV_ERR_INVALID,
@@ -243,7 +242,8 @@ int okv_kv8_read(const okv_kv8_cache_t* cache, const int32_t* idx, int64_t idx_s
   if (idx) OKV_REQUIRE(idx_stride >= max_rows, OKV_ERR_INVALID, "idx_stride < max_rows");
   ReadArgs a{*cache, idx, idx_stride, seq_lens, max_seq_len, max_rows, {k_out, v_out}, out_token_stride, out_head_stride,
              out_batch_stride};
-  OKV_REQUIRE(((uintptr_t)k_out & 15) == 0 && ((uintptr_t)v_out & 15) == 0 && wide_rows(a), OKV_ERR_INVALID,
+  OKV_REQUIRE(((uintptr_t)k_out & 15) == 0 && ((uintptr_t)v_out & 15) == 0 &&
+                  ((out_token_stride | out_head_stride | out_batch_stride) & 7) == 0, OKV_ERR_INVALID,
               "outputs: 16-byte aligned, strides multiples of 8 elements");
   if (max_rows == 0) return OKV_OK;
   OKV_REQUIRE(cache->num_kv_heads <= 65535 && batch <= 32767, OKV_ERR_UNSUPPORTED, "too many heads or requests");

@@ -30,6 +30,7 @@ def main():
     ap.add_argument("--select-layers", default="2,8,18")
     ap.add_argument("--real-offload", action="store_true")
     ap.add_argument("--offload-mode", default="zero_copy", choices=["zero_copy", "memcpy", "incremental"])
+    ap.add_argument("--kv-format", default=None, choices=["e4m3", "int8"], help="K and V in 8 bits, GPU resident")
     ap.add_argument("--full-attention", action="store_true", help="no selection: every layer attends to everything")
     ap.add_argument("--graph", action="store_true", help="replay the decode step from a HIP graph")
     ap.add_argument("--trace", default=None, metavar="DESC",
@@ -47,6 +48,8 @@ def main():
     cfg = OmniKVConfig(model_cls="multi", cache_cls="multi", do_select_layers=sel, num_wait_load_layers=1,
                        real_offload=args.real_offload and not args.full_attention, dense_more=True,
                        num_of_selected_tokens=args.ratio, selector_cls=args.selector, window_size=16)
+    if args.kv_format:
+        cfg.set_config(kv_format=args.kv_format)
     torch.set_default_dtype(torch.bfloat16)
     with torch.device(dev):
         lm = OmniKVMulLM(shape, cfg)
@@ -104,7 +107,8 @@ def main():
         "model": f"random-init Llama-3-8B shape, {args.layers} layers, bf16", "context": args.ctx,
         "decode_steps": args.steps, "select_layers": sel, "selected": int(args.ratio * args.ctx),
         "selector": args.selector, "real_offload": bool(args.real_offload and not args.full_attention),
-        "offload_mode": args.offload_mode if args.real_offload else None, "full_attention": args.full_attention, "launch": "hip_graph_replay" if args.graph else "eager",
+        "offload_mode": args.offload_mode if args.real_offload else None, "kv_format": args.kv_format or "bf16",
+        "full_attention": args.full_attention, "launch": "hip_graph_replay" if args.graph else "eager",
         "prefill_s": prefill_s, "decode_ms_per_token": dt * 1e3 / args.steps, "decode_tokens_per_s": args.steps / dt,
         "hbm_gb_allocated": round(torch.cuda.max_memory_allocated() / 1e9, 1),
         "first_tokens": toks,

@@ -215,6 +215,8 @@ class OmniKVMulLayer(nn.Module):
             q = attn.q_and_append(hidden_states, position_ids, rope, past_key_value)
             if trace.idx_tracer is not None:
                 # every layer reports what it would select (modeling/offload_select_once.py:170-174)
+                if past_key_value.kv_format is not None:
+                    raise NotImplementedError("selection tracing scores 16-bit keys")
                 trace.idx_tracer.observe(self.layer_idx, q, past_key_value.key_cache[self.layer_idx], consider_len)
             if self.layer_idx in self.do_select_layers:
                 if not self.config.get("dense_more", False):
@@ -352,6 +354,9 @@ class OmniKVMulLM(nn.Module):
         full = list(range(0, sel[0])) + sel + [self.shape.num_hidden_layers]  # modeling/omnikv.py:322-331
         if hasattr(self.config, "skip_threshold"):
             kwargs.setdefault("skip_threshold", self.config.get("skip_threshold"))
+        for key in ("kv_format", "kv_block"):  # K and V in 8 bits (cache.OmniKVMultiStageCache)
+            if hasattr(self.config, key):
+                kwargs.setdefault(key, self.config.get(key))
         return self.cache_cls(full, self.shape.num_hidden_layers,
                               self.config.get("num_wait_load_layers", 2), self.config.get("real_offload", True), **kwargs)
 

@@ -663,19 +663,20 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, t
     short last block as well (start then an int at a block's border).  A request whose rows would not
     fit is left as it was.  okv_kv8_append."""
     c = cache._struct(k.dtype)
-    if k.dim() != 4 or k.shape[0] != cache.bsz or k.shape[1] != cache.num_kv_heads or k.shape[3] != 128:
+    if k.dim() != 4 or v.dim() != 4 or k.shape[0] != cache.bsz or k.shape[1] != cache.num_kv_heads or k.shape[3] != 128:
         raise ValueError(f"new rows must be ({cache.bsz}, {cache.num_kv_heads}, n, 128)")
-    if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype or k.stride(3) != 1:
-        raise ValueError("new K and V must share shape, strides and dtype, with a contiguous last dimension")
+    (kb, kg, kt, k1), (vb, vg, vt, v1) = k.stride(), v.stride()
+    if v.shape != k.shape or v.dtype is not k.dtype or k1 != 1 or v1 != 1:
+        raise ValueError("new K and V must share shape and dtype, with a contiguous last dimension")
     if k.device != cache.device or v.device != cache.device:
         raise ValueError("new rows and cache must be on one GPU")
-    n, (sb, sg, st, _) = k.shape[2], k.stride()
+    n = k.shape[2]
     if n == 0:
         return
     on_dev = isinstance(start, torch.Tensor)
     starts = _dev_i32(start, cache.bsz, cache.device, "start") if on_dev else None
-    _launch(cache.device, lib().okv_kv8_append, c, k.data_ptr(), v.data_ptr(), st, sg, sb, starts, 0 if on_dev else int(start),
-            _dev_i32(new_lens, cache.bsz, cache.device, "new_lens"), n, int(close), cache.bsz)
+    _launch(cache.device, lib().okv_kv8_append, c, k.data_ptr(), kt, kg, kb, v.data_ptr(), vt, vg, vb, starts,
+            0 if on_dev else int(start), _dev_i32(new_lens, cache.bsz, cache.device, "new_lens"), n, int(close), cache.bsz)
 
 
 def _kv8_query(q: torch.Tensor, cache: KV8):

@@ -118,7 +118,7 @@ def test_append_strides_ragged_lengths_and_what_does_not_fit():
     g = torch.Generator().manual_seed(3)
     cache = ops.KV8.empty(4, 2, 96, "int8", 32, BF, DEV)
     x = rows(g, 4, 40, 2).transpose(1, 2)  # (b, heads, n, 128), token-major storage
-    y = rows(g, 4, 40, 2).transpose(1, 2)
+    y = rows(g, 4, 2, 40)  # V in other strides than K
     starts = torch.tensor([0, 60, -1, 57], dtype=torch.int32, device=DEV)  # 60 + 40 and -1 do not fit
     lens = torch.tensor([33, 40, 40, 7], dtype=torch.int32, device=DEV)
     ops.kv8_append(cache, x.to(DEV), y.to(DEV), starts, lens)

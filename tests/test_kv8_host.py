@@ -21,7 +21,7 @@ def cache(**kw):
 
 
 def append(c, starts=None, start=0, new_lens=None, n=4, close=0, batch=1, row=1024, k=PTR):
-    return _lib.lib().okv_kv8_append(C.byref(c), k, PTR, row, 128, 0, starts, start, new_lens, n, close, batch, None)
+    return _lib.lib().okv_kv8_append(C.byref(c), k, row, 128, 0, PTR, 1024, 128, 0, starts, start, new_lens, n, close, batch, None)
 
 
 def dense(c, hq=32, n=100, batch=1, ws=PTR, nbytes=1 << 40, scores=None, score_len=0, red=0, norm=0, q=PTR):
