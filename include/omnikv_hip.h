@@ -393,7 +393,7 @@ int okv_offload_fetch(const void* src, int64_t row_bytes, const int32_t* fetch_t
  *   its scale:            contiguous  scale + b*scale_batch_stride + (t/block)*scale_block_stride + g*scale_head_stride
  *                         paged       scale + page*scale_page_stride + (t%page_size/block)*scale_block_stride + g*scale_head_stride
  * Code strides are in bytes and multiples of 16, scale strides in floats; block_tokens divides
- * page_size and capacity.  A page number outside [0, num_pages) is never followed: reading, its tokens take no part in
+ * page_size and capacity.  A page that is written belongs to one request.  A page number outside [0, num_pages) is never followed: reading, its tokens take no part in
  * the softmax (their raw score is -inf); writing, its rows are dropped.
  */
 typedef struct okv_kv8_cache {
@@ -514,10 +514,12 @@ int okv_pages_free(const okv_page_pool_t* pool, const int32_t* seqs, int32_t n, 
 
 /* Sequence children[i] becomes a continuation of parents[i]: it names the parent's full pages
  * (counted once more) and gets a copy of a partly filled last one, so both may grow on their own.
- * All parents are read as they were before the call.  ws: okv_pages_workspace_bytes(pool, n). */
+ * All parents are read as they were before the call.  host_rows: arrays of one row per sequence (row s at
+ * base + s*page_bytes; an 8-bit cache's open buffers) whose parents' rows are copied to the children's.
+ * ws: okv_pages_workspace_bytes(pool, n). */
 int okv_pages_fork(const okv_page_pool_t* pool, const int32_t* parents, const int32_t* children, int32_t n,
-                   const okv_page_buffer_t* host_buffers, int32_t num_buffers, int32_t* status, void* ws,
-                   size_t ws_bytes, okv_stream_t stream);
+                   const okv_page_buffer_t* host_buffers, int32_t num_buffers, const okv_page_buffer_t* host_rows,
+                   int32_t num_rows, int32_t* status, void* ws, size_t ws_bytes, okv_stream_t stream);
 
 /* Room for more[i] more tokens (negative: none) in sequence seqs[i]: its length grows by it and the pages it
  * lacks are taken from the free ones. */

@@ -210,7 +210,7 @@ def _declare(l):
         ("okv_kv8_sparse_attn", [vp, i32, cache, vp, i64, i32, vp, i32, vp, vp, i64, i64, i64, vp, i32, i32, f32, vp, vp, sz,
                                  vp]),
         ("okv_pages_free", [pool, vp, i32, vp, vp]),
-        ("okv_pages_fork", [pool, vp, vp, i32, bufs, i32, vp, vp, sz, vp]),
+        ("okv_pages_fork", [pool, vp, vp, i32, bufs, i32, bufs, i32, vp, vp, sz, vp]),
         ("okv_pages_extend", [pool, vp, vp, i32, vp, vp]),
         ("okv_pages_copy", [bufs, i32, i32, vp, vp, vp, i32, vp]),
         ("okv_pages_compact", [pool, vp, i64, vp, vp, bufs, i32, vp, sz, vp]),

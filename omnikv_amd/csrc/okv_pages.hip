@@ -86,9 +86,10 @@ struct PagesWs {
   int32_t* full;   // [n] fork: shared pages of the pair, -1: nothing to do
   int32_t *src, *dst;  // fork [n], compact [num_pages / 2]: pages to copy and where to; -1: none
   int32_t* to;     // compact: [num_pages] the page's new number
+  int32_t *from_seq, *to_seq;  // fork [n]: sequences of the pairs that are served, -1: none
 };
 static size_t pages_ws_bytes(const okv_page_pool_t* p, int64_t n) {
-  return 4 * (2 * (size_t)p->num_pages + 16 + 3 * (size_t)n) + 256;
+  return 4 * (2 * (size_t)p->num_pages + 16 + 5 * (size_t)n) + 256;
 }
 static PagesWs carve(const okv_page_pool_t* p, int64_t n, void* ws) {
   int32_t* x = (int32_t*)(((size_t)ws + 255) & ~(size_t)255);
@@ -98,6 +99,8 @@ static PagesWs carve(const okv_page_pool_t* p, int64_t n, void* ws) {
   const int64_t m = n > 0 ? n : p->num_pages / 2;
   w.src = x; x += m;
   w.dst = x; x += m;
+  w.from_seq = x; x += n;
+  w.to_seq = x; x += n;
   w.to = x;
   return w;
 }
@@ -173,6 +176,8 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan(okv_page_pool_t 
     w.full[i] = act ? full : -1;
     w.src[i] = fresh >= 0 ? old : -1;
     w.dst[i] = fresh;
+    w.from_seq[i] = act ? from : -1;
+    w.to_seq[i] = act ? to : -1;
   }
   // a parent that is itself a child of this call was empty before it: its length is not one that is written here
   if (act) p.lens[to] = len;
@@ -228,11 +233,14 @@ __device__ __forceinline__ void copy_moves(const okv_page_buffer_t& buf, const i
   }
 }
 
-// grid (n, 1 + buffers): y = 0 names the pages in the child's row, the others copy the partly filled pages
+// grid (n, 1 + buffers): y = 0 names the pages in the child's row, the others copy the partly filled pages, and from buffer
+// `first_row` on the sequences' rows
 __global__ __launch_bounds__(256) void pages_fork_apply(okv_page_pool_t p, const int32_t* parents, const int32_t* children,
-                                                        int n, PagesWs w, BufferList bufs, int rows) {
+                                                        int n, PagesWs w, BufferList bufs, int first_row, int rows) {
   if (!rows || blockIdx.y > 0) {
-    copy_moves(bufs.b[blockIdx.y - rows], w.src, w.dst, n, p.num_pages, blockIdx.x, gridDim.x);
+    const int j = (int)blockIdx.y - rows;
+    if (j < first_row) copy_moves(bufs.b[j], w.src, w.dst, n, p.num_pages, blockIdx.x, gridDim.x);
+    else copy_moves(bufs.b[j], w.from_seq, w.to_seq, n, p.num_seqs, blockIdx.x, gridDim.x);
     return;
   }
   const int i = blockIdx.x, full = w.full[i], fresh = w.dst[i];
@@ -412,9 +420,10 @@ static int check_ws(const okv_page_pool_t* p, int64_t n, void* ws, size_t ws_byt
   OKV_REQUIRE(ws_bytes >= need, OKV_ERR_WORKSPACE, "workspace too small: have %zu, need %zu", ws_bytes, need);
   return OKV_OK;
 }
-static BufferList take(const okv_page_buffer_t* b, int n) {
+// `n` buffers from number `lo` on, of the list `b` of `nb` and the list `c` behind it
+static BufferList take(const okv_page_buffer_t* b, int lo, int n, int nb = 1 << 30, const okv_page_buffer_t* c = nullptr) {
   BufferList l{};
-  for (int i = 0; i < n; ++i) l.b[i] = b[i];
+  for (int i = 0; i < n; ++i) l.b[i] = lo + i < nb ? b[lo + i] : c[lo + i - nb];
   return l;
 }
 
@@ -441,10 +450,11 @@ int okv_pages_free(const okv_page_pool_t* pool, const int32_t* seqs, int32_t n, 
 }
 
 int okv_pages_fork(const okv_page_pool_t* pool, const int32_t* parents, const int32_t* children, int32_t n,
-                   const okv_page_buffer_t* host_buffers, int32_t num_buffers, int32_t* status, void* ws, size_t ws_bytes,
-                   okv_stream_t stream) {
+                   const okv_page_buffer_t* host_buffers, int32_t num_buffers, const okv_page_buffer_t* host_rows,
+                   int32_t num_rows, int32_t* status, void* ws, size_t ws_bytes, okv_stream_t stream) {
   int rc = check_pool(pool, "okv_pages_fork", true);
   if (!rc) rc = check_buffers(host_buffers, num_buffers, "okv_pages_fork");
+  if (!rc) rc = check_buffers(host_rows, num_rows, "okv_pages_fork, rows");
   if (rc) return rc;
   OKV_REQUIRE(n >= 1 && parents && children, OKV_ERR_INVALID, "okv_pages_fork: n >= 1 pairs");
   OKV_REQUIRE(n <= kMaxEntries, OKV_ERR_UNSUPPORTED, "okv_pages_fork: %d pairs in one call (at most %d)", n, kMaxEntries);
@@ -452,10 +462,11 @@ int okv_pages_fork(const okv_page_pool_t* pool, const int32_t* parents, const in
   if (rc) return rc;
   const PagesWs w = carve(pool, n, ws);
   hipLaunchKernelGGL(pages_fork_plan, dim3(1), dim3(kPlanThreads), 0, (hipStream_t)stream, *pool, parents, children, n, status, w);
-  for (int lo = 0; lo == 0 || lo < num_buffers; lo += kBuffersPerLaunch) {
-    const int m = num_buffers - lo < kBuffersPerLaunch ? num_buffers - lo : kBuffersPerLaunch, rows = lo == 0;
-    hipLaunchKernelGGL(pages_fork_apply, dim3(n, m + rows), dim3(256), 0, (hipStream_t)stream, *pool, parents, children, n,
-                       w, take(host_buffers + lo, m), rows);
+  const int all = num_buffers + num_rows;
+  for (int lo = 0; lo == 0 || lo < all; lo += kBuffersPerLaunch) {
+    const int m = all - lo < kBuffersPerLaunch ? all - lo : kBuffersPerLaunch, table = lo == 0;
+    hipLaunchKernelGGL(pages_fork_apply, dim3(n, m + table), dim3(256), 0, (hipStream_t)stream, *pool, parents, children, n, w,
+                       take(host_buffers, lo, m, num_buffers, host_rows), num_buffers - lo, table);
   }
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;
@@ -482,7 +493,7 @@ int okv_pages_copy(const okv_page_buffer_t* host_buffers, int32_t num_buffers, i
   if (n == 0) return OKV_OK;
   for (int lo = 0; lo < num_buffers; lo += kBuffersPerLaunch) {
     const int m = num_buffers - lo < kBuffersPerLaunch ? num_buffers - lo : kBuffersPerLaunch;
-    hipLaunchKernelGGL(pages_copy_kernel, dim3(copy_blocks(n, m), m), dim3(256), 0, (hipStream_t)stream, take(host_buffers + lo, m),
+    hipLaunchKernelGGL(pages_copy_kernel, dim3(copy_blocks(n, m), m), dim3(256), 0, (hipStream_t)stream, take(host_buffers, lo, m),
                        num_pages, src, dst, count, n);
   }
   OKV_HIP_CHECK(hipGetLastError());
@@ -504,7 +515,7 @@ int okv_pages_compact(const okv_page_pool_t* pool, int32_t* table_out, int64_t t
     const int m = num_buffers - lo < kBuffersPerLaunch ? num_buffers - lo : kBuffersPerLaunch, table = lo == 0;
     const uint32_t blocks = copy_blocks(pool->num_pages / 2 > pool->num_seqs ? pool->num_pages / 2 : pool->num_seqs, m + table);
     hipLaunchKernelGGL(pages_compact_apply, dim3(blocks, m + table), dim3(256), 0, (hipStream_t)stream, *pool, table_out,
-                       table_out_stride, w, take(host_buffers + lo, m), table);
+                       table_out_stride, w, take(host_buffers, lo, m), table);
   }
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;

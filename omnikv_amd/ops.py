@@ -535,6 +535,16 @@ def _dev_i32(t: Optional[torch.Tensor], n: int, device, name: str):
     return t.data_ptr()
 
 
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether two indices of t may name one element (an expanded tensor, say)."""
+    reach = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride < reach:
+            return True
+        reach = stride * (size - 1) + reach
+    return False
+
+
 class KV8:
     """An 8-bit K/V cache: codes (torch.float8_e4m3fn or torch.int8) with one fp32 scale per `block` tokens and kv
     head (include/omnikv_hip.h, okv_kv8_cache_t, has the format).
@@ -606,6 +616,8 @@ class KV8:
                 c.open_batch_stride, c.open_head_stride, c.open_token_stride = open_k.stride()[:3]
             self._c[dt] = c
         self._ref = {dt: C.byref(c) for dt, c in self._c.items()}
+        # an expanded cache (one prompt shared by several requests) can be attended to, not written
+        self._writable = not any(_overlaps(t) for t in (k, k_scale, open_k) if t is not None)
 
     @classmethod
     def empty(cls, bsz: int, num_kv_heads: int, capacity: int, fmt: str = "e4m3", block: int = 64,
@@ -670,6 +682,8 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, t
         raise ValueError("new K and V must share shape and dtype, with a contiguous last dimension")
     if k.device != cache.device or v.device != cache.device:
         raise ValueError("new rows and cache must be on one GPU")
+    if not cache._writable:
+        raise ValueError("rows of this cache share memory: it can be read only")
     n = k.shape[2]
     if n == 0:
         return
@@ -867,19 +881,23 @@ def pages_free(table, lens, refs, seqs, page_size: int, status: Optional[torch.T
     _launch(dev, lib().okv_pages_free, pool, _entries(seqs, n, dev, "seqs"), n, _dev_i32(status, 2, dev, "status"))
 
 
-def pages_fork(table, lens, refs, parents, children, page_size: int, buffers, status: Optional[torch.Tensor] = None) -> None:
+def pages_fork(table, lens, refs, parents, children, page_size: int, buffers, status: Optional[torch.Tensor] = None,
+               rows: Optional[PageBuffers] = None) -> None:
     """Sequence children[i] (empty) becomes a continuation of parents[i], in place: it shares the full pages and gets a copy
-    of a partly filled last one in every buffer (a PageBuffers or a list of tensors; the lowest free pages).  status
+    of a partly filled last one in every buffer (a PageBuffers or a list of tensors; the lowest free pages).  rows: tensors
+    (num_seqs, ...) whose row is copied from parent to child (an 8-bit cache's open buffers).  status
     (2,) int32 receives [pages short, pairs refused]; short of pages, nothing changes.  At most 1024 pairs.  okv_pages_fork."""
     dev, pool = _page_pool(table, lens, refs, page_size)
     bufs = _buffers(buffers)
     if bufs.device != dev or bufs.num_pages != refs.numel():
         raise ValueError("buffers must hold refs.numel() pages on the table's GPU")
+    if rows is not None and (rows.device != dev or rows.num_pages != table.shape[0]):
+        raise ValueError("rows must hold one row per sequence on the table's GPU")
     n = parents.numel()
     parents, children = _entries(parents, n, dev, "parents"), _entries(children, n, dev, "children")
     ws = _pages_scratch(pool, n, dev)
-    _launch(dev, lib().okv_pages_fork, pool, parents, children, n, bufs._c, len(bufs), _dev_i32(status, 2, dev, "status"),
-            ws.data_ptr(), ws.numel())
+    _launch(dev, lib().okv_pages_fork, pool, parents, children, n, bufs._c, len(bufs), rows._c if rows else None,
+            len(rows) if rows else 0, _dev_i32(status, 2, dev, "status"), ws.data_ptr(), ws.numel())
 
 
 def pages_extend(table, lens, refs, seqs, more, page_size: int, status: Optional[torch.Tensor] = None) -> None:

@@ -5,8 +5,8 @@ okv_page_pool_t) and the list of arrays whose pages move together: the pools of 
 a paged `ops.KV8`, which read and write through the same `table`.  Nothing here waits for the GPU
 except `status()`; a step of page operations on tensors of sequence numbers can be captured in a HIP graph.
 
-An 8-bit cache's open buffers belong to the sequences, not to the pages: `fork` copies the children's from their
-parents' for every cache that `add_cache` named.
+An 8-bit cache's open buffers belong to the sequences, not to the pages: `fork` copies a child's from its parent's, for
+every cache that `add_cache` named.
 """
 from __future__ import annotations
 
@@ -33,6 +33,7 @@ class PagePool:
         self._arrays: List[torch.Tensor] = []
         self._buffers: Optional[ops.PageBuffers] = None
         self._open: List[torch.Tensor] = []
+        self._rows: Optional[ops.PageBuffers] = None
 
     def add(self, *arrays: torch.Tensor) -> None:
         """Arrays (num_pages, ...) whose pages move with the pool's (the pools of a PagedKV)."""
@@ -48,6 +49,7 @@ class PagePool:
         self.add(cache.k, cache.v, cache.k_scale, cache.v_scale)
         if cache.open_k is not None:
             self._open += [cache.open_k, cache.open_v]
+            self._rows = ops.PageBuffers(self._open)
 
     def _numbers(self, x: Numbers) -> torch.Tensor:
         return x if isinstance(x, torch.Tensor) else torch.tensor(list(x), dtype=torch.int32, device=self.table.device)
@@ -63,13 +65,10 @@ class PagePool:
         self._sum += self._status
 
     def fork(self, parents: Numbers, children: Numbers) -> None:
-        """Children continue their parents (ops.pages_fork).  With caches that hold open rows the children are
-        distinct and none is a parent, in range: their open rows are copied whatever the pool's pages allow."""
-        parents, children = self._numbers(parents), self._numbers(children)
-        ops.pages_fork(self.table, self.lens, self.refs, parents, children, self.page_size, self._require_buffers(), self._status)
+        """Children continue their parents (ops.pages_fork)."""
+        ops.pages_fork(self.table, self.lens, self.refs, self._numbers(parents), self._numbers(children), self.page_size,
+                       self._require_buffers(), self._status, self._rows)
         self._sum += self._status
-        for t in self._open:
-            t.index_copy_(0, children.long(), t.index_select(0, parents.long()))
 
     def free(self, seqs: Numbers) -> None:
         """Sequences end (ops.pages_free)."""

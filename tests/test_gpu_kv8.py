@@ -288,6 +288,40 @@ def test_sparse(fmt, dtype, block, page, hkv, group, lens, picks, tails):
         check_attention(none, q, wk, wv, 128 ** -0.5, dtype)
 
 
+@pytest.mark.parametrize("page", [0, 32])
+def test_batch_of_many_ragged_requests(page):
+    """More requests than a wave has lanes: the shares of all of them, scored and not, through an index and not."""
+    g = torch.Generator().manual_seed(25)
+    lens = [int(x) for x in torch.randint(0, 900, (131,), generator=g)]
+    lens[0], lens[64], lens[130] = 2500, 0, 2900
+    cache, ks, vs = make(g, "int8", BF, 16, page, lens, 1)
+    q = rows(g, 131, 2)
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=2900), q, ks, vs, 128 ** -0.5, BF)
+    out, raw = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=2900, selector="last", score_len=2900, score_lens=t - 1)
+    check_attention(out, q, ks, vs, 128 ** -0.5, BF)
+    for b in (0, 1, 77, 130):
+        _, x, _, _, mass = ref.attention(q[b], ks[b], vs[b], 128 ** -0.5)
+        n = max(lens[b] - 1, 0)
+        assert bool(((raw[b, :n].cpu().double() - x.amax(0)[:n]).abs() <= ref.logit_error(mass).amax(0)[:n]).all())
+    closed = [n // 16 * 16 for n in lens]
+    idx = torch.arange(0, 2900, 3, dtype=torch.int32, device=DEV).expand(131, -1).contiguous()
+    picks = torch.tensor([(n + 2) // 3 for n in closed], dtype=torch.int32, device=DEV)
+    got = ops.kv8_sparse_attn(q.to(DEV), cache, idx=idx, sel_lens=picks)
+    check_attention(got, q, [k[:, :n:3] for k, n in zip(ks, closed)], [v[:, :n:3] for v, n in zip(vs, closed)], 128 ** -0.5, BF)
+
+
+def test_a_shared_prompt_can_be_read_by_several_requests_and_not_written():
+    g = torch.Generator().manual_seed(26)
+    one, ks, vs = make(g, "e4m3", BF, 32, 0, [600], 2, open_rows=False)
+    ex = [t.expand(3, *t.shape[1:]) for t in (one.k, one.v, one.k_scale, one.v_scale)]
+    cache = ops.KV8(*ex, 32)
+    q = rows(g, 3, 8)
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache, seq_len=600), q, ks * 3, vs * 3, 128 ** -0.5, BF)
+    with pytest.raises(ValueError, match="read only"):
+        ops.kv8_append(cache, q[:, :2, None].to(DEV), q[:, :2, None].to(DEV), 0, close=True)
+
+
 def test_sparse_without_an_index_and_with_a_tail_alone():
     g = torch.Generator().manual_seed(22)
     cache, ks, vs = make(g, "int8", BF, 32, 0, [130, 77], 2, open_rows=False)

@@ -94,6 +94,46 @@ def test_short_of_pages_changes_nothing():
     same(table, lt, refs, bufs, m)
 
 
+def test_fork_copies_the_sequences_rows_of_served_pairs_only():
+    page = 4
+    table, lt, refs, bufs, m = make(5, 8, 6, 40, page, [7, 8, 0, 5])
+    g = torch.Generator().manual_seed(5)
+    rows = [torch.randn((8, 3, 4), generator=g).to(DEV), torch.randn((8, 500, 4), generator=g).to(DEV)]
+    want = [r.clone() for r in rows]
+    parents, children = [0, 1, 0, 99, 2, 3], [4, 5, 4, 6, 6, -1]  # again 4; out of range; an empty parent
+    status = torch.zeros(2, dtype=torch.int32, device=DEV)
+    ops.pages_fork(table, lt, refs, i32(parents), i32(children), page, bufs, status, ops.PageBuffers(rows))
+    assert status.tolist() == m.fork(parents, children)
+    same(table, lt, refs, bufs, m)
+    for r, w in zip(rows, want):
+        w[4], w[5] = w[0], w[1]
+        assert torch.equal(r, w)
+
+
+def test_the_largest_call_and_growth_over_many_trips_through_the_counts():
+    """1024 entries at once; a pool of more pages than one trip through the counts covers."""
+    page, seqs = 2, 2048
+    r = random.Random(9)
+    lens = [r.randint(0, 9) for _ in range(1024)]
+    table, lt, refs, bufs, m = make(9, seqs, 12, 30000, page, lens, shapes=((2,),))
+    status = torch.zeros(2, dtype=torch.int32, device=DEV)
+    children = list(range(1024, 2048))
+    r.shuffle(children)
+    ops.pages_fork(table, lt, refs, i32(list(range(1024))), i32(children), page, bufs, status)
+    assert status.tolist() == m.fork(list(range(1024)), children) == [0, 0]
+    same(table, lt, refs, bufs, m)
+    seqs_, more = r.sample(range(2048), 1024), [r.randint(-2, 12) for _ in range(1024)]
+    ops.pages_extend(table, lt, refs, i32(seqs_), i32(more), page, status)
+    assert status.tolist() == m.extend(seqs_, more)
+    same(table, lt, refs, bufs, m)
+    gone = r.sample(range(2048), 1500)
+    ops.pages_free(table, lt, refs, i32(gone), page, status)
+    m.free(gone)
+    t, rf, n = ops.pages_compact(table, refs, bufs)
+    assert int(n) == m.compact()
+    same(t, lt, rf, bufs, m)
+
+
 @pytest.mark.parametrize("pages, seqs", [(1, 1), (2, 1), (63, 4), (1024, 10), (1025, 40), (5000, 700)])
 @pytest.mark.parametrize("used", [0.0, 0.3, 0.97, 1.0])
 @pytest.mark.parametrize("in_place", [False, True])

@@ -113,20 +113,21 @@ def test_page_refusals():
         bad = _lib.PagePool(PTR, PTR, PTR, 8, 4, 8, 100, 16)
         setattr(bad, field, value)
         assert l.okv_pages_free(C.byref(bad), PTR, 1, None, None) == INVALID
-        assert l.okv_pages_fork(C.byref(bad), PTR, PTR, 1, buf, 1, None, PTR, big, None) == INVALID
+        assert l.okv_pages_fork(C.byref(bad), PTR, PTR, 1, buf, 1, None, 0, None, PTR, big, None) == INVALID
         assert l.okv_pages_extend(C.byref(bad), PTR, PTR, 1, None, None) == INVALID
         if field != "lens":
             assert l.okv_pages_compact(C.byref(bad), PTR, 8, PTR, None, buf, 1, PTR, big, None) == INVALID
     assert l.okv_pages_free(C.byref(pool), None, 1, None, None) == INVALID
     assert l.okv_pages_free(C.byref(pool), PTR, 0, None, None) == INVALID
-    assert l.okv_pages_fork(C.byref(pool), PTR, None, 1, buf, 1, None, PTR, big, None) == INVALID
-    assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1, buf, 1, None, PTR, 16, None) == WORKSPACE
-    assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1, None, 1, None, PTR, big, None) == INVALID
+    assert l.okv_pages_fork(C.byref(pool), PTR, None, 1, buf, 1, None, 0, None, PTR, big, None) == INVALID
+    assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1, buf, 1, None, 0, None, PTR, 16, None) == WORKSPACE
+    assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1, None, 1, None, 0, None, PTR, big, None) == INVALID
+    assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1, buf, 1, None, 2, None, PTR, big, None) == INVALID
     assert l.okv_pages_extend(C.byref(pool), PTR, None, 1, None, None) == INVALID
     wide = _lib.PagePool(PTR, PTR, PTR, 1 << 21, 4, 1 << 21, 100, 16)
     assert l.okv_pages_extend(C.byref(wide), PTR, PTR, 1024, None, None) == UNSUPPORTED
     assert l.okv_pages_extend(C.byref(pool), PTR, PTR, 1025, None, None) == UNSUPPORTED
-    assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1025, buf, 1, None, PTR, big, None) == UNSUPPORTED
+    assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1025, buf, 1, None, 0, None, PTR, big, None) == UNSUPPORTED
     assert l.okv_pages_copy(buf, 1, 100, None, PTR, None, 3, None) == INVALID
     assert l.okv_pages_copy(buf, 1, 100, None, None, None, 0, None) == 0
     assert l.okv_pages_compact(C.byref(pool), PTR, 7, PTR, None, buf, 1, PTR, big, None) == INVALID
