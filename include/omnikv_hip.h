@@ -435,10 +435,10 @@ int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, int64_t k_to
                    int64_t v_head_stride, int64_t v_batch_stride, const int32_t* starts, int32_t start, const int32_t* new_lens, int32_t max_new,
                    int32_t close, int32_t batch, okv_stream_t stream);
 
-/* Scratch of the two attention calls: `max_rows` is max_seq_len, or max_sel_len + max_tail_len;
- * max_score_len 0 without scores. */
-int okv_kv8_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t max_rows,
-                            int32_t max_score_len, size_t* out_bytes);
+/* Scratch of the two attention calls over `cache`: max_rows is max_seq_len, or max_sel_len + max_tail_len;
+ * max_score_len 0 without scores; indexed 1 for a sparse call with an index.  0 bytes: ws may be NULL. */
+int okv_kv8_workspace_bytes(const okv_kv8_cache_t* cache, int32_t num_q_heads, int32_t batch, int32_t max_rows,
+                            int32_t max_score_len, int32_t indexed, size_t* out_bytes);
 
 /*
  * okv_dense_attn over an 8-bit cache: the rows [0, seq_len) of each request, those behind the last

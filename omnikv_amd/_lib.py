@@ -205,7 +205,7 @@ def _declare(l):
     for name, args in (
         ("okv_kv8_append", [cache, vp, i64, i64, i64, vp, i64, i64, i64, vp, i32, vp, i32, i32, i32, vp]),
         ("okv_kv8_read", [cache, vp, i64, i32, vp, i32, i32, vp, vp, i64, i64, i64, vp]),
-        ("okv_kv8_workspace_bytes", [i32, i32, i32, i32, i32, C.POINTER(sz)]),
+        ("okv_kv8_workspace_bytes", [cache, i32, i32, i32, i32, i32, C.POINTER(sz)]),
         ("okv_kv8_dense_attn", [vp, i32, cache, vp, i32, i32, f32, vp, vp, i32, i32, i32, vp, i64, vp, sz, vp]),
         ("okv_kv8_sparse_attn", [vp, i32, cache, vp, i64, i32, vp, i32, vp, vp, i64, i64, i64, vp, i32, i32, f32, vp, vp, sz,
                                  vp]),

@@ -42,7 +42,9 @@ struct Kv8Attn {
   float inv_target, inv_fine;  // 1 / full shares that fit next to the requests' last, short ones (half a share each)
   int32_t most_rows;  // of a share (its logits are staged in LDS)
   int32_t items;      // shares the grid and the partial results have room for
-  int32_t fine;       // long shares of a batch are cut in three
+  int32_t least_rows;
+  int32_t pair;       // two kv heads to a wave (NH 2)
+  int32_t fine;       // shares of a batch longer than this are cut in three; 0: not
   int32_t direct;     // one share per request, which writes the output itself: no second launch
   int32_t fold;         // raw scores: the q heads of a kv head are folded by the split (1 max, 2 sum): one logits row per kv head
   int32_t logit_heads;  // rows of `logits` per request
@@ -78,8 +80,6 @@ struct Share {
   int count;   // shares of the request
 };
 
-constexpr int kLeastRows = 128;  // one 32-row tile per wave
-constexpr uint32_t kFineRows = 1024;
 
 // inclusive prefix sum over the wave
 __device__ __forceinline__ int lane_scan(int x) {
@@ -94,8 +94,8 @@ __device__ __forceinline__ int lane_scan(int x) {
 __device__ __forceinline__ int share_rows(int total, const Kv8Attn& a) {
   // (less than one off where it is not cut to most_rows anyway: at or above total / target)
   uint32_t r = ((uint32_t)((float)total * a.inv_target) + 64) & ~63u;
-  if (a.fine && r > kFineRows) r = max(((uint32_t)((float)total * a.inv_fine) + 64) & ~63u, kFineRows);
-  return r < kLeastRows ? kLeastRows : r > (uint32_t)a.most_rows ? a.most_rows : (int)r;
+  if (a.fine && r > (uint32_t)a.fine) r = max(((uint32_t)((float)total * a.inv_fine) + 64) & ~63u, (uint32_t)a.fine);
+  return r < (uint32_t)a.least_rows ? a.least_rows : r > (uint32_t)a.most_rows ? a.most_rows : (int)r;
 }
 // x / rows, rounded up: quotients below 2^16 from a product with the reciprocal, put right by one step
 __device__ __forceinline__ int shares_up(int x, int rows) {
@@ -204,6 +204,13 @@ __device__ __forceinline__ uint32_t decode_pair(I8, const T*, uint32_t x) {
   return pack_pair((const T*)nullptr, (float)(int8_t)(x >> (16 * H)), (float)(int8_t)(x >> (16 * H + 8)));
 }
 
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+// D(16x16 fp32) += A(16 x 16) . B(16 x 16) in bf16: four elements of the contraction per lane
+__device__ __forceinline__ f32x4_t mfma16k16(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, make_uint2(a0, a1)),
+                                                   __builtin_bit_cast(s16x4_t, make_uint2(b0, b1)), c, 0, 0, 0);
+}
+
 // lanes 8..15 (MASK 0xC) or 0..7 (MASK 0x3) of every 16-lane row take `from` of the lane eight away, the others keep `own`
 template <int MASK>
 __device__ __forceinline__ uint32_t take8(uint32_t own, uint32_t from) {
@@ -271,9 +278,15 @@ struct Kv8Rows {
 // scale of a row is folded into its p; V's codes, exact in bf16, are the B operand: a lane's eight rows x
 // eight elements, turned by byte permutes as they are decoded.
 // Scales of K are applied to the fp32 logits.  One running maximum per q head and wave; the waves meet in LDS.
-template <typename T, typename F, int MODE, bool LOGITS>
+//
+// NH 2 (paged, an even number of kv heads): a wave takes sixteen rows of two neighbouring heads instead of 32 rows of one;
+// what is said of the upper sixteen rows then holds for the second head.  A pool stores a token's heads next to each other,
+// and 128-byte pieces a token's row apart reach memory less well than 256-byte ones: 288000 tokens of one request
+// 122.3 -> 113.2 us, sixteen of 18000 each 121.1 -> 117.6.  Through an index it made no difference (22.1, 22.6).
+template <typename T, typename F, int MODE, bool LOGITS, int NH>
 __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv8_split(Kv8Attn a) {
   extern __shared__ float lds[];
+  constexpr int TR = 32 / NH, kStep = 4 * TR;  // rows of a tile, and between a wave's tiles
   const okv_kv8_cache_t& c = a.c;
   if constexpr (MODE != kPaged) {  // one batch of scalar loads instead of a round trip before each first use (the paged mode's
     // page descriptors leave too few scalar registers for that: 131 against 121 us)
@@ -287,9 +300,9 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   const int G = a.group;
   // workgroups go to the XCDs round-robin: the kv heads of a share run on one XCD, one after the other, so that rows
   // stored head by head next to each other (pools) are fetched together
-  const int turn = blockIdx.x >> 3, g = turn % c.num_kv_heads;
+  const int turn = blockIdx.x >> 3, groups = c.num_kv_heads / NH, g = turn % groups * NH;
   Share sh;
-  if (!find_share(a, (int)((turn / c.num_kv_heads) * 8 + (blockIdx.x & 7)), 0, &sh)) return;
+  if (!find_share(a, (int)((turn / groups) * 8 + (blockIdx.x & 7)), 0, &sh)) return;
   const int b = sh.b, main_len = sh.main_len, L = sh.L, A = LOGITS ? sh.A : 0;
   int begin, end;
   {
@@ -305,14 +318,15 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m16 = lane & 15, j = lane >> 4, m8 = m16 & 7, hi8 = m16 >> 3;
 
-  uint4 qf[4];
-  {
+  uint4 qf[NH][4];
+#pragma unroll
+  for (int s = 0; s < NH; ++s) {
     const int h = m8 < G ? m8 : G - 1;
-    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(b * a.hq + g * G + h) * kD + 16 * j;
-    qf[0] = *reinterpret_cast<const uint4*>(qp);
-    qf[1] = *reinterpret_cast<const uint4*>(qp + 8);
-    qf[2] = *reinterpret_cast<const uint4*>(qp + 64);
-    qf[3] = *reinterpret_cast<const uint4*>(qp + 72);
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(b * a.hq + (g + s) * G + h) * kD + 16 * j;
+    qf[s][0] = *reinterpret_cast<const uint4*>(qp);
+    qf[s][1] = *reinterpret_cast<const uint4*>(qp + 8);
+    qf[s][2] = *reinterpret_cast<const uint4*>(qp + 64);
+    qf[s][3] = *reinterpret_cast<const uint4*>(qp + 72);
   }
 
   const uint32_t ts = (uint32_t)c.token_stride;
@@ -340,16 +354,14 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   auto rows_of = [&](int t, Kv8Rows& r) {
     if (MODE == kPaged) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) r.page[s] = table[page_of(min(t + 16 * s, last))];
+      for (int s = 0; s < 2 / NH; ++s) r.page[s] = table[page_of(min(t + 16 * s, last))];
     } else if (MODE == kGather) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const int rk = min(t + 8 * x + m8, last), rv = min(t + 16 * (x >> 1) + 4 * j + 2 * (x & 1) + hi8, last);
-        r.k[x] = a.idx ? idx[rk] : rk;
-        r.v[x] = a.idx ? idx[rv] : rv;
+        r.k[x] = idx[min(t + 8 * x + m8, last)];
+        r.v[x] = idx[min(t + 16 * (x >> 1) + 4 * j + 2 * (x & 1) + hi8, last)];
       }
-      const int rs = min(t + (lane & 31), last);
-      r.s = a.idx ? idx[rs] : rs;
+      r.s = idx[min(t + (lane & 31), last)];
     }
   };
   auto load = [&](int t, const Kv8Rows& r, Kv8Tile& x) {
@@ -372,18 +384,19 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       x.ok = 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int u = t + 16 * s, n = min(16, main_end - u);
-        const bool in = (uint32_t)r.page[s] < (uint32_t)c.num_pages;
-        const int64_t p = in ? r.page[s] : 0;
+        const int u = t + (NH == 1 ? 16 * s : 0), n = min(16, main_end - u), page = r.page[NH == 1 ? s : 0];
+        const bool in = (uint32_t)page < (uint32_t)c.num_pages;
+        const int64_t p = in ? page : 0;
         const int slot = slot_of(u);
-        const int64_t base = p * c.page_stride + (int64_t)slot * ts;
+        const int64_t base = p * c.page_stride + (int64_t)slot * ts + (NH == 1 ? 0 : s * c.head_stride);
         const uint32_t bytes = in && n > 0 ? (uint32_t)(n - 1) * ts + kD : 0;
         const __amdgpu_buffer_rsrc_t kr = as_buffer(kb + base, bytes), vr = as_buffer(vb + base, bytes);
         x.k[2 * s] = buffer16(kr, koff[2 * s]);
         x.k[2 * s + 1] = buffer16(kr, koff[2 * s + 1]);
         x.v[2 * s] = buffer16(vr, voff[2 * s]);
         x.v[2 * s + 1] = buffer16(vr, voff[2 * s + 1]);
-        const int64_t so = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride;
+        const int64_t so = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride +
+                           (NH == 1 ? 0 : s * c.scale_head_stride);
         x.ks[s] = buffer4(as_buffer(ksb + so, bytes ? 4 : 0), 0);
         x.vs[s] = buffer4(as_buffer(vsb + so, bytes ? 4 : 0), 0);
         x.ok |= in ? 1u << s : 0u;
@@ -406,7 +419,6 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
         return in;
       };
       int64_t row, scale;
-      bool bad = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         at(r.k[i], &row, &scale);
@@ -414,39 +426,43 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        bad = !at(r.v[i], &row, &scale) || bad;
+        at(r.v[i], &row, &scale);
         x.v[i] = load_stream16(vb + row + vcol);
       }
-      x.ok = at(r.s, &row, &scale);
-      x.ks[0] = (lane < 32 ? ksb : vsb)[scale];  // lanes 0..31: K scales of rows l, 32..63: V scales of rows l - 32
+      x.ok = at(r.s, &row, &scale);  // lanes 0..31: the K scales of rows l, 32..63: the V scales of rows l - 32
+      x.ks[0] = (lane < 32 ? ksb : vsb)[scale];
     }
   };
 
-  float m = -INFINITY;  // running maximum of head m8's logits, times log2(e), over the wave's rows
-  float l = 0.f;        // sum of exponentials over the rows of lane row j, relative to m
-  f32x4_t acc[8];       // acc[e][i]: element 16 m8 + 8 hi8 + e of head (4j + i) % 8; j < 2: from bf16(p), else the rest
+  float m[NH];          // running maximum of q head m8's logits, times log2(e), over the wave's rows
+  float l[NH];          // sum of exponentials over the rows of lane row j, relative to m
+  f32x4_t acc[NH][8];   // acc[.][e][i]: element 16 m8 + 8 hi8 + e of q head (4j + i) % 8; j < 2: from bf16(p), else the rest
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const float rest = hi8 ? 1.f : 0.f;
+  for (int s = 0; s < NH; ++s) {
+    m[s] = -INFINITY;
+    l[s] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[s][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
   const bool scored = LOGITS && begin < A;
-  float* slog = lds;  // [G, or 1 when the heads are folded][split_rows]: handed over at the end
+  float* slog = lds;  // [NH][G, or 1 when the heads are folded][rows]: handed over at the end
 
-  auto raise_max = [&](float top) {
-    if (__ballot(top > m) == 0ull) return;
-    const float mn = rows_max(fmaxf(top, m));
-    const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-    l *= al;
-    m = mn;
+  auto raise_max = [&](int n, float top) {  // n: of the wave's kv heads
+    if (__ballot(top > m[n]) == 0ull) return;
+    const float mn = rows_max(fmaxf(top, m[n]));
+    const float al = __builtin_amdgcn_exp2f(m[n] - (mn == -INFINITY ? 0.f : mn));
+    l[n] *= al;
+    m[n] = mn;
     const float lo[4] = {row_lane<0>(al), row_lane<1>(al), row_lane<2>(al), row_lane<3>(al)};
     const float hi[4] = {row_lane<4>(al), row_lane<5>(al), row_lane<6>(al), row_lane<7>(al)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float f = (j & 1) ? hi[i] : lo[i];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e][i] *= f;
+      for (int e = 0; e < 8; ++e) acc[n][e][i] *= f;
     }
   };
-  auto stage_logits = [&](int row, const float (&v)[4]) {  // natural units, rows row .. +4
+  auto stage_logits = [&](int n, int row, const float (&v)[4]) {  // natural units, rows row .. +4
     float o[4] = {v[0], v[1], v[2], v[3]};
     if (a.fold) {
 #pragma unroll
@@ -461,7 +477,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       }
     }
     if (m16 < (a.fold ? 1 : G))
-      *reinterpret_cast<float4*>(slog + m16 * sh.rows + (row - begin)) = make_float4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<float4*>(slog + (n * (a.fold ? 1 : G) + m16) * sh.rows + (row - begin)) = make_float4(o[0], o[1], o[2], o[3]);
   };
   // a probability in two 16-bit parts: this lane's part of four of them
   auto split_p = [&](auto* ty, const float (&p)[4], uint32_t* out) {
@@ -473,7 +489,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
 
   auto compute = [&](int t, Kv8Tile& x, float* sstage) {
     float ks[2][4], vs[2][4];
-    bool whole = t >= begin && t + 32 <= main_end;
+    bool whole = t >= begin && t + TR <= main_end;
     if (MODE == kGather) {
       // every lane has the scale of one row: the wave's 256 bytes of LDS hand the rows' four to their lane row
       const bool okl = x.ok != 0;
@@ -520,7 +536,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       }
     }
     float p[2][4];
-    float top = -INFINITY;
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       f32x4_t S = {0.f, 0.f, 0.f, 0.f};
@@ -531,13 +547,13 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       for (int f = 0; f < 2; ++f) {
         const uint4 x0 = make_uint4(decode_pair<0>(F{}, (const T*)nullptr, lo[2 * f]), decode_pair<1>(F{}, (const T*)nullptr, lo[2 * f]),
                                     decode_pair<0>(F{}, (const T*)nullptr, lo[2 * f + 1]), decode_pair<1>(F{}, (const T*)nullptr, lo[2 * f + 1]));
-        S = mfma16((const T*)nullptr, x0, qf[f], S);
+        S = mfma16((const T*)nullptr, x0, qf[NH == 1 ? 0 : s][f], S);
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
         const uint4 x1 = make_uint4(decode_pair<0>(F{}, (const T*)nullptr, up[2 * f]), decode_pair<1>(F{}, (const T*)nullptr, up[2 * f]),
                                     decode_pair<0>(F{}, (const T*)nullptr, up[2 * f + 1]), decode_pair<1>(F{}, (const T*)nullptr, up[2 * f + 1]));
-        S = mfma16((const T*)nullptr, x1, qf[2 + f], S);
+        S = mfma16((const T*)nullptr, x1, qf[NH == 1 ? 0 : s][2 + f], S);
       }
       float v[4];
 #pragma unroll
@@ -545,30 +561,37 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = t + 16 * s + 4 * j + i;
+          const int r = t + (NH == 1 ? 16 * s : 0) + 4 * j + i;
           const bool in = r >= begin && r < main_end &&
                           (MODE == kContiguous || ((x.ok >> (MODE == kPaged ? s : 16 * s + 4 * j + i)) & 1));
           v[i] = in ? v[i] : -INFINITY;
           vs[s][i] = in ? vs[s][i] : 0.f;
         }
       }
-      if (scored && t + 16 * s < main_end) stage_logits(t + 16 * s + 4 * j, v);
+      const int row0 = t + (NH == 1 ? 16 * s : 0);
+      if (scored && row0 < main_end) stage_logits(NH == 1 ? 0 : s, row0 + 4 * j, v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         p[s][i] = v[i] * kLog2e;
-        top = fmaxf(top, p[s][i]);
+        top[s] = fmaxf(top[s], p[s][i]);
       }
     }
-    raise_max(top);
-    const float neg = m == -INFINITY ? 0.f : -m;
+    if (NH == 1) {
+      raise_max(0, fmaxf(top[0], top[1]));
+    } else {
+#pragma unroll
+      for (int s = 0; s < NH; ++s) raise_max(s, top[s]);
+    }
     uint32_t pa[4];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
+      const int n = NH == 1 ? 0 : s;
+      const float neg = m[n] == -INFINITY ? 0.f : -m[n];
       float w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e = __builtin_amdgcn_exp2f(p[s][i] + neg);
-        l += e;
+        l[n] += e;
         w[i] = e * vs[s][i];
       }
       split_p((const BF16*)nullptr, w, pa + 2 * s);
@@ -599,46 +622,54 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
                                     decode_pair<0>(F{}, bf, u23));
         const uint4 e1 = make_uint4(decode_pair<1>(F{}, bf, l01), decode_pair<1>(F{}, bf, l23), decode_pair<1>(F{}, bf, u01),
                                     decode_pair<1>(F{}, bf, u23));
-        acc[4 * d + 2 * h] = mfma16(bf, pf, e0, acc[4 * d + 2 * h]);
-        acc[4 * d + 2 * h + 1] = mfma16(bf, pf, e1, acc[4 * d + 2 * h + 1]);
+        const int e = 4 * d + 2 * h;
+        if (NH == 1) {
+          acc[0][e] = mfma16(bf, pf, e0, acc[0][e]);
+          acc[0][e + 1] = mfma16(bf, pf, e1, acc[0][e + 1]);
+        } else {
+          acc[0][e] = mfma16k16(pf.x, pf.y, e0.x, e0.y, acc[0][e]);
+          acc[0][e + 1] = mfma16k16(pf.x, pf.y, e1.x, e1.y, acc[0][e + 1]);
+          acc[NH - 1][e] = mfma16k16(pf.z, pf.w, e0.z, e0.w, acc[NH - 1][e]);
+          acc[NH - 1][e + 1] = mfma16k16(pf.z, pf.w, e1.z, e1.w, acc[NH - 1][e + 1]);
+        }
       }
     }
   };
 
   float* sstage = lds + a.lds_scales + 64 * wave;
   {
-    int t = (begin & ~31) + 32 * wave;
+    int t = (begin & ~(TR - 1)) + TR * wave;
     if (t < main_end) {
-      const int t_last = t + ((last - t) >> 7 << 7);
+      const int t_last = t + (last - t) / kStep * kStep;
       Kv8Rows r0, r1;
       Kv8Tile x0, x1;
       rows_of(t, r0);
       if (MODE == kGather) {
-        for (; t <= t_last; t += 128) {
+        for (; t <= t_last; t += kStep) {
           load(t, r0, x0);
-          rows_of(min(t + 128, t_last), r0);
+          rows_of(min(t + kStep, t_last), r0);
           compute(t, x0, sstage);
         }
       } else if (t == t_last) {
         load(t, r0, x0);
         compute(t, x0, sstage);
       } else {
-        rows_of(t + 128, r1);
+        rows_of(t + kStep, r1);
         load(t, r0, x0);
-        while (true) {  // tile t + 128 in flight while t is consumed; past the last one nothing is fetched.  The loads stay
+        while (true) {  // tile t + kStep in flight while t is consumed; past the last one nothing is fetched.  The loads stay
           __builtin_amdgcn_sched_barrier(0);  // where they are: among the arithmetic they would wait for its data.
-          load(t + 128, r1, x1);
-          rows_of(t + 256, r0);
+          load(t + kStep, r1, x1);
+          rows_of(t + 2 * kStep, r0);
           __builtin_amdgcn_sched_barrier(0);
           compute(t, x0, sstage);
-          t += 128;
+          t += kStep;
           if (t > t_last) break;
           __builtin_amdgcn_sched_barrier(0);
-          load(t + 128, r0, x0);
-          rows_of(t + 256, r1);
+          load(t + kStep, r0, x0);
+          rows_of(t + 2 * kStep, r1);
           __builtin_amdgcn_sched_barrier(0);
           compute(t, x1, sstage);
-          t += 128;
+          t += kStep;
           if (t > t_last) break;
         }
       }
@@ -650,11 +681,13 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     const int lo = max(begin, closed);
     const int64_t lts = a.late_token_stride;
     const int64_t lbase = (int64_t)b * a.late_batch_stride + (int64_t)g * a.late_head_stride;
-    const T* lk = reinterpret_cast<const T*>(a.late[0]) + lbase;
-    const T* lv = reinterpret_cast<const T*>(a.late[1]) + lbase;
     const T* ty = nullptr;
     for (int t = lo + 16 * wave; t < end; t += 64) {
       const int top_row = end - 1 - closed;  // rows counted from the first late one
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+      const T* lk = reinterpret_cast<const T*>(a.late[0]) + lbase + n * a.late_head_stride;
+      const T* lv = reinterpret_cast<const T*>(a.late[1]) + lbase + n * a.late_head_stride;
       const T* kp = lk + (int64_t)min(t - closed + m16, top_row) * lts + 16 * j;
       const uint4 kf[4] = {*reinterpret_cast<const uint4*>(kp), *reinterpret_cast<const uint4*>(kp + 8),
                            *reinterpret_cast<const uint4*>(kp + 64), *reinterpret_cast<const uint4*>(kp + 72)};
@@ -664,22 +697,22 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
         vf[i] = *reinterpret_cast<const uint4*>(lv + (int64_t)min(t - closed + 4 * j + i, top_row) * lts + 16 * m8 + 8 * hi8);
       f32x4_t S = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int f = 0; f < 4; ++f) S = mfma16(ty, kf[f], qf[f], S);
+      for (int f = 0; f < 4; ++f) S = mfma16(ty, kf[f], qf[n][f], S);
       float v[4], p[4], top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = t + 4 * j + i < end ? S[i] * a.scale : -INFINITY;
-      if (scored) stage_logits(t + 4 * j, v);
+      if (scored) stage_logits(n, t + 4 * j, v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         p[i] = v[i] * kLog2e;
         top = fmaxf(top, p[i]);
       }
-      raise_max(top);
-      const float neg = m == -INFINITY ? 0.f : -m;
+      raise_max(n, top);
+      const float neg = m[n] == -INFINITY ? 0.f : -m[n];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         p[i] = __builtin_amdgcn_exp2f(p[i] + neg);
-        l += p[i];
+        l[n] += p[i];
       }
       uint32_t pa[2];
       split_p(ty, p, pa);
@@ -688,10 +721,11 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       const uint32_t r2[4] = {vf[2].x, vf[2].y, vf[2].z, vf[2].w}, r3[4] = {vf[3].x, vf[3].y, vf[3].z, vf[3].w};
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        acc[2 * d] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x05040100u),
-                                               __builtin_amdgcn_perm(r3[d], r2[d], 0x05040100u), 0, 0), acc[2 * d]);
-        acc[2 * d + 1] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x07060302u),
-                                                   __builtin_amdgcn_perm(r3[d], r2[d], 0x07060302u), 0, 0), acc[2 * d + 1]);
+        acc[n][2 * d] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x05040100u),
+                                               __builtin_amdgcn_perm(r3[d], r2[d], 0x05040100u), 0, 0), acc[n][2 * d]);
+        acc[n][2 * d + 1] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x07060302u),
+                                                   __builtin_amdgcn_perm(r3[d], r2[d], 0x07060302u), 0, 0), acc[n][2 * d + 1]);
+      }
       }
     }
   }
@@ -700,7 +734,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   if (scored) {
     __syncthreads();
     const int nh = a.fold ? 1 : G;
-    for (int h = 0; h < nh; ++h) {
+    for (int h = 0; h < NH * nh; ++h) {
       float* dst = a.logits + (int64_t)(b * a.logit_heads + g * nh + h) * a.logits_stride + begin;
       const float* src = slog + h * sh.rows;
       for (int r = 4 * threadIdx.x; r < end - begin; r += 1024) {
@@ -718,43 +752,48 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   }
 
   // ---- the four waves meet
-  float* sm = lds;                   // [4][8] running maximum
-  float* sl = lds + 4 * kMaxGroup;   // [4][8] sum of exponentials
-  float* so = lds + 8 * kMaxGroup;   // [4][G][128]
-  l = rows_sum(l);
-  if (lane < kMaxGroup) {
-    sm[wave * kMaxGroup + lane] = m;
-    sl[wave * kMaxGroup + lane] = l;
-  }
+  constexpr int kCell = NH * kMaxGroup;
+  float* sm = lds;              // [4][NH][8] running maximum
+  float* sl = lds + 4 * kCell;  // [4][NH][8] sum of exponentials
+  float* so = lds + 8 * kCell;  // [4][NH G][128]
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[e][i]), __float_as_uint(acc[e][i]), false, false);
-      acc[e][i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  for (int n = 0; n < NH; ++n) {
+    l[n] = rows_sum(l[n]);
+    if (lane < kMaxGroup) {
+      sm[wave * kCell + n * kMaxGroup + lane] = m[n];
+      sl[wave * kCell + n * kMaxGroup + lane] = l[n];
     }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int h = 4 * j + i;
-    if (j < 2 && h < G) {
-      float4* dst = reinterpret_cast<float4*>(so + (wave * G + h) * kD + 16 * m8 + 8 * hi8);
-      dst[0] = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
-      dst[1] = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[n][e][i]), __float_as_uint(acc[n][e][i]), false, false);
+        acc[n][e][i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = 4 * j + i;
+      if (j < 2 && h < G) {
+        float4* dst = reinterpret_cast<float4*>(so + ((wave * NH + n) * G + h) * kD + 16 * m8 + 8 * hi8);
+        dst[0] = make_float4(acc[n][0][i], acc[n][1][i], acc[n][2][i], acc[n][3][i]);
+        dst[1] = make_float4(acc[n][4][i], acc[n][5][i], acc[n][6][i], acc[n][7][i]);
+      }
     }
   }
   __syncthreads();
-  for (int o = threadIdx.x; o < G * kD; o += 256) {
-    const int h = o / kD, d = o % kD;
+  for (int o = threadIdx.x; o < NH * G * kD; o += 256) {
+    const int h = o / kD, d = o % kD;  // q head of the workgroup's NH G
+    const int cell = NH == 1 ? h : h < G ? h : kMaxGroup + h - G;
     float M = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) M = fmaxf(M, sm[x * kMaxGroup + h]);
+    for (int x = 0; x < 4; ++x) M = fmaxf(M, sm[x * kCell + cell]);
     const float Ms = M == -INFINITY ? 0.f : M;
     float den = 0.f, num = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const float f = __builtin_amdgcn_exp2f(sm[x * kMaxGroup + h] - Ms);
-      den = fmaf(sl[x * kMaxGroup + h], f, den);
-      num = fmaf(so[(x * G + h) * kD + d], f, num);
+      const float f = __builtin_amdgcn_exp2f(sm[x * kCell + cell] - Ms);
+      den = fmaf(sl[x * kCell + cell], f, den);
+      num = fmaf(so[(x * NH * G + h) * kD + d], f, num);
     }
     // den 0: no row took part (a NaN among the logits leaves NaN)
     if (a.direct) {
@@ -899,81 +938,86 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
 // ---------------------------------------------------------------- host side
 static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// How many shares to cut the rows into: one round of workgroups, of which the chip holds two per CU (their registers allow
-// two waves per SIMD), three of the gather mode.  In a batch every request ends in a share cut short, so long shares are
-// cut in three (sixteen requests of 8K..32K tokens: 136 us in one round, 124 / 121 / 122 / 127 / 136 in 2 / 3 / 4 / 6 / 8);
-// short ones are not: a workgroup's first microseconds move nothing.  A scored share stages its logits in LDS, up to 32 KB.
-static void kv8_cut(bool gather, int batch, int hkv, int group, int64_t rows, int max_score, bool folded, int* target, int* most, int* items) {
-  *target = std::max(1, 256 * (gather ? kGatherResident : 2) / hkv);  // shares of one round
-  *most = max_score > 0 ? 32768 / 4 / (folded ? 1 : group) / 64 * 64 : 8192;
-  const int64_t all = std::max<int64_t>(rows, 1) * batch;
-  const bool fine = !gather && batch > 1;
-  const int64_t n = std::min((all + kLeastRows - 1) / kLeastRows,
-                             std::max<int64_t>((fine ? 3 : 1) * (int64_t)*target + 1, (all + *most - 1) / *most));
-  *items = (int)std::min<int64_t>(n + (int64_t)batch * (max_score > 0 ? 2 : 1), 1 << 30);
+// How a call is run, from its sizes and layout alone.
+struct Kv8Plan {
+  bool direct, pair;
+  int target, most, least, items;
+  bool fine;
+};
+
+// direct: a share per request, and no second launch: where requests are short, and longer ones where there are many, the
+// rows a wave then takes one after the other cost less than the join and the round trip through memory.  Measured (bf16,
+// int8, eight kv heads; one launch against two, us): 1 x 333 rows 7.6 / 8.0, 1 x 512 8.2 / 7.8, 16 x 1024 13.6 / 17.0,
+// 64 x 1536 37.8 / 54.3; through an index 1 x 256 7.3 / 8.3, 1 x 333 9.9 / 8.8, 16 x 512 12.9 / 13.1, 64 x 1536 42.1 / 61.1.
+//
+// Else one round of workgroups, of which the chip holds two per CU (their registers allow two waves per SIMD), three of
+// the gather mode.  In a batch every request ends in a share cut short, so long shares are cut in three (sixteen
+// requests of 8K..32K tokens: 136 us in one round, 124 / 121 / 122 / 127 / 136 in 2 / 3 / 4 / 6 / 8); short ones are not: a
+// workgroup's first microseconds move nothing.  A scored share stages its logits in LDS, up to 32 KB.
+static Kv8Plan kv8_plan(bool gather, bool paged, int batch, int hkv, int group, int64_t rows, int max_score, bool folded) {
+  Kv8Plan p{};
+  const int64_t wgs = (int64_t)batch * hkv, all = std::max<int64_t>(rows, 1) * batch;
+  p.direct = max_score == 0 && rows <= std::min<int64_t>(2048, gather ? std::max<int64_t>(256, 4 * wgs) : std::max<int64_t>(384, 8 * wgs));
+  p.pair = paged && !gather && hkv % 2 == 0 && !p.direct;
+  const int nh = p.pair ? 2 : 1;
+  p.least = 128 / nh;  // one tile per wave
+  p.target = std::max(1, 256 * (gather ? kGatherResident : 2) * nh / hkv);  // shares of one round
+  p.most = max_score > 0 ? 32768 / 4 / (nh * (folded ? 1 : group)) / 64 * 64 : 8192;
+  p.fine = !gather && batch > 1;
+  const int64_t n = std::min((all + p.least - 1) / p.least, std::max<int64_t>((p.fine ? 3 : 1) * (int64_t)p.target + 1, (all + p.most - 1) / p.most));
+  p.items = p.direct ? batch : (int)std::min<int64_t>(n + (int64_t)batch * (max_score > 0 ? 2 : 1), 1 << 30);
+  return p;
 }
 
 // Carves the partial results; the bytes they take.  `folded` saves logits, never adds.
-// A share per request, and no second launch: where requests are short, and longer ones where there are many, the rows a
-// wave then takes one after the other cost less than the join and the round trip through memory.  Measured (bf16, int8,
-// eight kv heads; one launch against two, us): 1 x 333 rows 7.6 / 8.0, 1 x 512 8.2 / 7.8, 16 x 1024 13.6 / 17.0,
-// 64 x 1536 37.8 / 54.3; through an index 1 x 256 7.3 / 8.3, 1 x 333 9.9 / 8.8, 16 x 512 12.9 / 13.1, 64 x 1536 42.1 / 61.1.
-static bool kv8_direct(bool gather, int batch, int hkv, int64_t rows, int max_score) {
-  const int64_t heads = (int64_t)batch * hkv;
-  return max_score == 0 && rows <= std::min<int64_t>(2048, gather ? std::max<int64_t>(256, 4 * heads) : std::max<int64_t>(384, 8 * heads));
-}
-
-static size_t kv8_workspace(bool gather, int batch, int hq, int hkv, int64_t rows, int max_score, bool folded, Kv8Attn* a, char* p) {
-  int target, most, items;
-  if (kv8_direct(gather, batch, hkv, rows, max_score)) {
-    if (a) {
-      a->batch = batch;
-      a->direct = 1;
-    }
-    return 0;
+static size_t kv8_workspace(const Kv8Plan& p, int batch, int hq, int hkv, int max_score, bool folded, Kv8Attn* a, char* ws) {
+  if (a) {
+    a->batch = batch;
+    a->direct = p.direct;
+    a->pair = p.pair;
+    a->fine = p.fine ? 1024 / (p.pair ? 2 : 1) : 0;
+    a->items = p.items;
+    a->most_rows = p.most;
+    a->least_rows = p.least;
+    a->inv_target = 1.f / (float)std::max(p.target - batch / 2, (p.target + 1) / 2);
+    a->inv_fine = 1.f / (float)std::max(3 * p.target - batch / 2, p.target);
   }
-  kv8_cut(gather, batch, hkv, hq / hkv, rows, max_score, folded, &target, &most, &items);
-  const size_t o = align256((size_t)items * hq * kD * 4), l = align256((size_t)items * hq * 4);
+  if (p.direct) return 0;
+  const size_t o = align256((size_t)p.items * hq * kD * 4), l = align256((size_t)p.items * hq * 4);
   const size_t stride = ((size_t)max_score + 63) / 64 * 64;
   const int heads = folded ? hkv : hq;
   const size_t g = max_score > 0 ? align256((size_t)batch * heads * stride * 4) : 0;
   if (a) {
-    p = (char*)align256((size_t)p);
-    a->batch = batch;
-    a->inv_target = 1.f / (float)std::max(target - batch / 2, (target + 1) / 2);
-    a->inv_fine = 1.f / (float)std::max(3 * target - batch / 2, target);
-    a->most_rows = most;
-    a->items = items;
-    a->fine = !gather && batch > 1;
-    a->part_o = (float*)p;
-    a->part_lse = (float*)(p + o);
-    a->logits = max_score > 0 ? (float*)(p + o + l) : nullptr;
+    ws = (char*)align256((size_t)ws);
+    a->part_o = (float*)ws;
+    a->part_lse = (float*)(ws + o);
+    a->logits = max_score > 0 ? (float*)(ws + o + l) : nullptr;
     a->logits_stride = (int64_t)stride;
     a->logit_heads = heads;
   }
   return o + l + g + 256;
 }
 
-template <typename T, typename F, int MODE, bool LOGITS>
+template <typename T, typename F, int MODE, bool LOGITS, int NH>
 static int launch_split(Kv8Attn& a, int batch, hipStream_t stream) {
-  size_t floats = 8 * kMaxGroup + (size_t)4 * a.group * kD;
-  if (LOGITS) floats = std::max(floats, (size_t)(a.fold ? 1 : a.group) * a.most_rows);
+  size_t floats = NH * (8 * kMaxGroup + (size_t)4 * a.group * kD);
+  if (LOGITS) floats = std::max(floats, (size_t)NH * (a.fold ? 1 : a.group) * a.most_rows);
   a.lds_scales = (int)floats;
   if (MODE == kGather) floats += 256;
-  if (a.direct) a.items = a.batch;
-  hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS>), dim3((a.items + 7) / 8 * 8 * a.c.num_kv_heads), dim3(256), floats * 4, stream, a);
+  hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS, NH>), dim3((a.items + 7) / 8 * 8 * (a.c.num_kv_heads / NH)), dim3(256), floats * 4, stream, a);
   return OKV_OK;
 }
 
 template <typename T, typename F>
 static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
   const bool paged = a.c.page_table != nullptr, scored = a.max_score_len > 0;
-  if (a.idx) launch_split<T, F, kGather, false>(a, batch, stream);
-  else if (paged && scored) launch_split<T, F, kPaged, true>(a, batch, stream);
-  else if (paged) launch_split<T, F, kPaged, false>(a, batch, stream);
-  else if (scored) launch_split<T, F, kContiguous, true>(a, batch, stream);
-  else launch_split<T, F, kContiguous, false>(a, batch, stream);
-  // blocks of 512 scores put more CUs to pulling the logits, but each works out the normalisers anew
+  if (a.idx) launch_split<T, F, kGather, false, 1>(a, batch, stream);
+  else if (paged && scored && a.pair) launch_split<T, F, kPaged, true, 2>(a, batch, stream);
+  else if (paged && scored) launch_split<T, F, kPaged, true, 1>(a, batch, stream);
+  else if (paged && a.pair) launch_split<T, F, kPaged, false, 2>(a, batch, stream);
+  else if (paged) launch_split<T, F, kPaged, false, 1>(a, batch, stream);
+  else if (scored) launch_split<T, F, kContiguous, true, 1>(a, batch, stream);
+  else launch_split<T, F, kContiguous, false, 1>(a, batch, stream);
   if (a.direct) {
     OKV_HIP_CHECK(hipGetLastError());
     return OKV_OK;
@@ -999,10 +1043,11 @@ static int kv8_attend(Kv8Attn& a, int64_t rows, int batch, void* ws, size_t ws_b
   OKV_REQUIRE(a.hq <= kMaxHeads, OKV_ERR_UNSUPPORTED, "%d q heads not supported (at most %d)", a.hq, kMaxHeads);
   OKV_REQUIRE(batch <= 65535, OKV_ERR_UNSUPPORTED, "batch %d not supported", batch);
   OKV_REQUIRE(rows * batch < (1ll << 31), OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
-  OKV_REQUIRE(ws != nullptr || kv8_direct(a.idx != nullptr, batch, hkv, rows, a.max_score_len), OKV_ERR_INVALID, "workspace pointer is NULL");
   const bool folded = a.max_score_len > 0 && a.normalise == OKV_NORM_RAW;
   if (folded) a.fold = a.head_reduce == OKV_REDUCE_MAX ? 1 : 2;
-  const size_t need = kv8_workspace(a.idx != nullptr, batch, a.hq, hkv, rows, a.max_score_len, folded, &a, (char*)ws);
+  const Kv8Plan p = kv8_plan(a.idx != nullptr, a.c.page_table != nullptr, batch, hkv, a.group, rows, a.max_score_len, folded);
+  const size_t need = kv8_workspace(p, batch, a.hq, hkv, a.max_score_len, folded, &a, (char*)ws);
+  OKV_REQUIRE(ws != nullptr || need == 0, OKV_ERR_INVALID, "workspace pointer is NULL");
   OKV_REQUIRE(ws_bytes >= need, OKV_ERR_WORKSPACE, "workspace too small: have %zu, need %zu", ws_bytes, need);
   OKV_REQUIRE((int64_t)(a.items + 7) * hkv < (1ll << 31), OKV_ERR_UNSUPPORTED, "%d requests of up to %lld rows", batch, (long long)rows);
   if (a.c.dtype == OKV_BF16)
@@ -1016,14 +1061,14 @@ using namespace okv;
 
 extern "C" {
 
-int okv_kv8_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t max_rows,
-                            int32_t max_score_len, size_t* out_bytes) {
-  OKV_REQUIRE(out_bytes != nullptr, OKV_ERR_INVALID, "NULL argument");
-  OKV_REQUIRE(batch >= 1 && num_kv_heads >= 1 && num_q_heads >= num_kv_heads && max_rows >= 0 && max_score_len >= 0,
-              OKV_ERR_INVALID, "bad batch, head counts or lengths");
-  // whichever way the rows are found
-  *out_bytes = std::max(kv8_workspace(false, batch, num_q_heads, num_kv_heads, max_rows, max_score_len, false, nullptr, nullptr),
-                        kv8_workspace(true, batch, num_q_heads, num_kv_heads, max_rows, max_score_len, false, nullptr, nullptr));
+int okv_kv8_workspace_bytes(const okv_kv8_cache_t* cache, int32_t num_q_heads, int32_t batch, int32_t max_rows,
+                            int32_t max_score_len, int32_t indexed, size_t* out_bytes) {
+  OKV_REQUIRE(cache != nullptr && out_bytes != nullptr, OKV_ERR_INVALID, "NULL argument");
+  const int hkv = cache->num_kv_heads;
+  OKV_REQUIRE(batch >= 1 && hkv >= 1 && num_q_heads >= hkv && max_rows >= 0 && max_score_len >= 0, OKV_ERR_INVALID,
+              "bad batch, head counts or lengths");
+  const Kv8Plan p = kv8_plan(indexed != 0, cache->page_table != nullptr, batch, hkv, num_q_heads / hkv, max_rows, max_score_len, false);
+  *out_bytes = kv8_workspace(p, batch, num_q_heads, hkv, max_score_len, false, nullptr, nullptr);
   return OKV_OK;
 }
 

@@ -616,6 +616,7 @@ class KV8:
                 c.open_batch_stride, c.open_head_stride, c.open_token_stride = open_k.stride()[:3]
             self._c[dt] = c
         self._ref = {dt: C.byref(c) for dt, c in self._c.items()}
+        self._ws_bytes = {}  # scratch of a call, by its sizes
         # an expanded cache (one prompt shared by several requests) can be attended to, not written
         self._writable = not any(_overlaps(t) for t in (k, k_scale, open_k) if t is not None)
 
@@ -660,11 +661,16 @@ class KV8:
         return c
 
 
-@functools.lru_cache(maxsize=4096)
-def _kv8_workspace_bytes(device_index: int, batch: int, hq: int, hkv: int, rows: int, score_len: int) -> int:
-    out = C.c_size_t(0)
-    check(lib().okv_kv8_workspace_bytes(batch, hq, hkv, rows, score_len, C.byref(out)))
-    return out.value
+def _kv8_workspace_bytes(cache: KV8, hq: int, rows: int, score_len: int, indexed: bool) -> int:
+    n = cache._ws_bytes.get((hq, rows, score_len, indexed))
+    if n is None:
+        out = C.c_size_t(0)
+        check(lib().okv_kv8_workspace_bytes(next(iter(cache._ref.values())), hq, cache.bsz, rows, score_len, int(indexed),
+                                            C.byref(out)))
+        if len(cache._ws_bytes) >= 4096:  # lengths that grow by one per call
+            cache._ws_bytes.clear()
+        n = cache._ws_bytes[(hq, rows, score_len, indexed)] = out.value
+    return n
 
 
 def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor] = 0,
@@ -713,7 +719,7 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
     pass, and with `select_k` the ascending indices of the largest ones, as topk gives them.  A request
     without rows gets zeros.  okv_kv8_dense_attn."""
     q, c = _kv8_query(q, cache)
-    hq, hkv, dev, bsz = q.shape[1], cache.num_kv_heads, cache.device, cache.bsz
+    hq, dev, bsz = q.shape[1], cache.device, cache.bsz
     if seq_len is None:
         seq_len = cache.capacity
     if select_k is not None and selector is None:
@@ -730,7 +736,7 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
         elif scores.shape != (bsz, slen) or scores.dtype != torch.float32 or scores.stride(1) != 1 or scores.device != dev:
             raise ValueError("scores_out must be (bsz, score_len) float32 with contiguous rows, on the cache's GPU")
         sp, ss, sl = scores.data_ptr(), scores.stride(0), _dev_i32(score_lens, bsz, dev, "score_lens")
-    nbytes = _kv8_workspace_bytes(dev.index, bsz, hq, hkv, seq_len, slen)
+    nbytes = _kv8_workspace_bytes(cache, hq, seq_len, slen, False)
     ws = _scratch(dev, nbytes) if nbytes else None
     _launch(dev, lib().okv_kv8_dense_attn, q.data_ptr(), hq, c, _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz,
             scale if scale is not None else _SCALE128, out.data_ptr(), sl, slen, red, norm, sp, ss,
@@ -789,7 +795,7 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
         raise ValueError("tail_len without a tail")
     tail_len = tail_len or 0
     out = torch.empty_like(q)
-    nbytes = _kv8_workspace_bytes(dev.index, bsz, hq, hkv, sel_len + tail_len, 0)
+    nbytes = _kv8_workspace_bytes(cache, hq, sel_len + tail_len, 0, idx is not None)
     ws = _scratch(dev, nbytes) if nbytes else None
     _launch(dev, lib().okv_kv8_sparse_attn, q.data_ptr(), hq, c, ip, istride, int(slots is not None),
             _dev_i32(sel_lens, bsz, dev, "sel_lens"), sel_len, tkp, tvp, tts, ths, tbs,

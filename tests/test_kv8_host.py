@@ -96,10 +96,14 @@ def test_attention_refusals():
     assert sparse(cache(), n=500, stride=500, nbytes=256) == WORKSPACE
     gap = dict(page_table=PTR, page_size=64, page_table_stride=4, num_pages=9, page_stride=65 * 128 * 8, token_stride=1024)
     assert sparse(cache(**gap), slots=1) == INVALID
-    n = C.c_size_t(0)
-    assert _lib.lib().okv_kv8_workspace_bytes(0, 32, 8, 10, 0, C.byref(n)) == INVALID
-    assert _lib.lib().okv_kv8_workspace_bytes(1, 4, 8, 10, 0, C.byref(n)) == INVALID
-    assert _lib.lib().okv_kv8_workspace_bytes(1, 32, 8, 10, 0, None) == INVALID
+    n, c = C.c_size_t(0), cache()
+    size = _lib.lib().okv_kv8_workspace_bytes
+    assert size(C.byref(c), 32, 0, 10, 0, 0, C.byref(n)) == INVALID
+    assert size(C.byref(c), 4, 1, 10, 0, 0, C.byref(n)) == INVALID
+    assert size(C.byref(c), 32, 1, -1, 0, 0, C.byref(n)) == INVALID
+    assert size(C.byref(c), 32, 1, 10, 0, 0, None) == INVALID
+    assert size(None, 32, 1, 10, 0, 0, C.byref(n)) == INVALID
+    assert size(C.byref(c), 32, 1, 100000, 0, 0, C.byref(n)) == 0 and n.value > 0
 
 
 def test_page_refusals():
