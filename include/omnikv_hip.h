@@ -425,7 +425,8 @@ typedef struct okv_kv8_cache {
  * new_k + b*k_batch_stride + r*k_token_stride + g*k_head_stride + d, of V likewise (strides in elements,
  * multiples of 8, 16-byte aligned).  starts (device int32[batch]) or start for every request;
  * new_lens (device int32[batch]) or max_new for every request.  close = 1 quantises a short last
- * block too (over its own rows; the rows behind it are left as they were): with close, or without
+ * block too (over its own rows; the rows behind it and the open buffers are left as they were, so that calls which take
+ * a request's last rows from an open buffer read a short closed block through a descriptor without one): with close, or without
  * open buffers, starts must be NULL and start a multiple of block_tokens, and without open buffers
  * close must be 1 or every request must end at a block's border (max_new a multiple, new_lens NULL).
  * A request whose rows would not fit (start < 0, or start + new_len beyond its room) is left as it was.

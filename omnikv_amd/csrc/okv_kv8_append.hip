@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   if (n == 0 || start < 0 || (int64_t)start + n > kv8_room(c)) return;
   const int end = start + n;
   const int first = start / B, blk = first + blockIdx.x;
-  if (blk * B >= end) return;
+  if (blk > (end - 1) / B) return;  // (blk * B may pass 2^31 behind the last block)
   const T* src = reinterpret_cast<const T*>(a.rows[is_v]) + (int64_t)b * a.batch_stride[is_v] + (int64_t)g * a.head_stride[is_v];
   const int64_t row_stride = a.token_stride[is_v];
   T* open = reinterpret_cast<T*>(is_v ? c.open_v : c.open_k);

@@ -1042,7 +1042,8 @@ static int kv8_attend(Kv8Attn& a, int64_t rows, int batch, void* ws, size_t ws_b
   OKV_REQUIRE(a.group <= kMaxGroup, OKV_ERR_UNSUPPORTED, "GQA group size %d not supported (1 to %d)", a.group, kMaxGroup);
   OKV_REQUIRE(a.hq <= kMaxHeads, OKV_ERR_UNSUPPORTED, "%d q heads not supported (at most %d)", a.hq, kMaxHeads);
   OKV_REQUIRE(batch <= 65535, OKV_ERR_UNSUPPORTED, "batch %d not supported", batch);
-  OKV_REQUIRE(rows * batch < (1ll << 31), OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
+  // (row numbers run past the last row by up to two steps of a workgroup, and stay in 32 bits)
+  OKV_REQUIRE(rows * batch <= (1ll << 31) - 65536, OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
   const bool folded = a.max_score_len > 0 && a.normalise == OKV_NORM_RAW;
   if (folded) a.fold = a.head_reduce == OKV_REDUCE_MAX ? 1 : 2;
   const Kv8Plan p = kv8_plan(a.idx != nullptr, a.c.page_table != nullptr, batch, hkv, a.group, rows, a.max_score_len, folded);

@@ -678,7 +678,8 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, t
     """Appends k, v (bsz, Hkv, n, 128; any strides, contiguous last dimension) behind the first `start` rows of each
     request: an int, or an int32 GPU tensor (bsz,) of the requests' lengths.  new_lens (bsz,) int32: rows per request,
     at most n.  Blocks that fill become codes, the other rows wait in the open buffers; close=True quantises a
-    short last block as well (start then an int at a block's border).  A request whose rows would not
+    short last block as well (start then an int at a block's border) and leaves the open buffers alone: such rows are
+    read by an index, or through a KV8 of the same tensors without open buffers.  A request whose rows would not
     fit is left as it was.  okv_kv8_append."""
     c = cache._struct(k.dtype)
     if k.dim() != 4 or v.dim() != 4 or k.shape[0] != cache.bsz or k.shape[1] != cache.num_kv_heads or k.shape[3] != 128:
@@ -694,6 +695,8 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, t
     if n == 0:
         return
     on_dev = isinstance(start, torch.Tensor)
+    if not on_dev and not 0 <= start <= cache.capacity:
+        raise ValueError(f"invalid start {start}: the cache has room for {cache.capacity} tokens")
     starts = _dev_i32(start, cache.bsz, cache.device, "start") if on_dev else None
     _launch(cache.device, lib().okv_kv8_append, c, k.data_ptr(), kt, kg, kb, v.data_ptr(), vt, vg, vb, starts,
             0 if on_dev else int(start), _dev_i32(new_lens, cache.bsz, cache.device, "new_lens"), n, int(close), cache.bsz)
@@ -722,6 +725,8 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
     hq, dev, bsz = q.shape[1], cache.device, cache.bsz
     if seq_len is None:
         seq_len = cache.capacity
+    elif seq_len > cache.capacity:
+        raise ValueError(f"invalid seq_len {seq_len}: the cache has room for {cache.capacity} tokens")
     if select_k is not None and selector is None:
         raise ValueError("select_k needs a selector")
     out = torch.empty_like(q)
@@ -730,12 +735,14 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
         norm_s, red_s = SELECTOR_MODES[selector]
         red, norm = _REDUCE[red_s], _NORM[norm_s]
         slen = seq_len if score_len is None else score_len
+        if not 0 <= slen <= seq_len:
+            raise ValueError(f"score_len {slen} must lie in [0, seq_len]")
         scores = scores_out
         if scores is None:
             scores = torch.empty((bsz, slen), dtype=torch.float32, device=dev)
         elif scores.shape != (bsz, slen) or scores.dtype != torch.float32 or scores.stride(1) != 1 or scores.device != dev:
             raise ValueError("scores_out must be (bsz, score_len) float32 with contiguous rows, on the cache's GPU")
-        sp, ss, sl = scores.data_ptr(), scores.stride(0), _dev_i32(score_lens, bsz, dev, "score_lens")
+        sp, ss, sl = scores.data_ptr(), scores.stride(0) if bsz > 1 else max(slen, scores.stride(0)), _dev_i32(score_lens, bsz, dev, "score_lens")
     nbytes = _kv8_workspace_bytes(cache, hq, seq_len, slen, False)
     ws = _scratch(dev, nbytes) if nbytes else None
     _launch(dev, lib().okv_kv8_dense_attn, q.data_ptr(), hq, c, _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz,
@@ -776,6 +783,8 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
             raise ValueError("idx rows must not overlap")
     elif sel_len is None:
         sel_len = cache.capacity
+    elif sel_len > cache.capacity:
+        raise ValueError(f"invalid sel_len {sel_len}: the cache has room for {cache.capacity} tokens")
     tkp = tvp = None
     tts = ths = tbs = 0
     if tail_k is not None:
@@ -811,6 +820,8 @@ def kv8_read(cache: KV8, dtype: torch.dtype, idx: Optional[torch.Tensor] = None,
     c, dev, bsz = cache._struct(dtype), cache.device, cache.bsz
     if seq_len is None:
         seq_len = cache.capacity
+    elif seq_len > cache.capacity:
+        raise ValueError(f"invalid seq_len {seq_len}: the cache has room for {cache.capacity} tokens")
     n = seq_len
     if idx is not None:
         if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != bsz or not idx.is_contiguous() or idx.device != dev:

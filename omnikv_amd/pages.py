@@ -37,19 +37,20 @@ class PagePool:
 
     def add(self, *arrays: torch.Tensor) -> None:
         """Arrays (num_pages, ...) whose pages move with the pool's (the pools of a PagedKV)."""
-        self._arrays.extend(arrays)
-        self._buffers = ops.PageBuffers(self._arrays)
-        if self._buffers.num_pages != self.refs.numel() or self._buffers.device != self.table.device:
+        both = ops.PageBuffers(self._arrays + list(arrays))
+        if both.num_pages != self.refs.numel() or both.device != self.table.device:
             raise ValueError(f"arrays must hold {self.refs.numel()} pages on {self.table.device}")
+        self._arrays, self._buffers = both.tensors, both
 
     def add_cache(self, cache: ops.KV8) -> None:
         """A paged 8-bit cache that goes through this pool's table: codes, scales, and its open buffers for fork."""
-        if cache.page_table is None or cache.page_table.data_ptr() != self.table.data_ptr() or cache.page_size != self.page_size:
+        if (cache.page_table is None or cache.page_table.data_ptr() != self.table.data_ptr()
+                or cache.page_table.shape != self.table.shape or cache.page_size != self.page_size):
             raise ValueError("the cache must be paged through this pool's table")
+        rows = ops.PageBuffers(self._open + [cache.open_k, cache.open_v]) if cache.open_k is not None else self._rows
         self.add(cache.k, cache.v, cache.k_scale, cache.v_scale)
-        if cache.open_k is not None:
-            self._open += [cache.open_k, cache.open_v]
-            self._rows = ops.PageBuffers(self._open)
+        if rows is not None:
+            self._open, self._rows = rows.tensors, rows
 
     def _numbers(self, x: Numbers) -> torch.Tensor:
         return x if isinstance(x, torch.Tensor) else torch.tensor(list(x), dtype=torch.int32, device=self.table.device)

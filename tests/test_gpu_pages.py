@@ -253,3 +253,19 @@ def test_pool_of_an_8_bit_cache_in_a_replayed_graph():
     assert int((pool.refs > 0).sum()) == int(pool.used) and not pool.refs[int(pool.used):].any()
     attend()
     assert pool.status() == (0, 0)
+
+
+def test_a_refused_array_leaves_the_pool_as_it_was():
+    pool = PagePool(2, 4, 8, 16, DEV)
+    pool.add(torch.zeros((8, 4), device=DEV))
+    for bad in (torch.zeros((9, 4), device=DEV), torch.zeros((8, 8), device=DEV)[:, :4], torch.zeros((8, 4))):
+        with pytest.raises(ValueError):
+            pool.add(bad)
+    part = ops.KV8.empty_paged(pool.table[:1], 8, 16, 2)  # the table's first row alone
+    other = ops.KV8.empty_paged(pool.table.clone(), 8, 16, 2)
+    for cache in (part, other):
+        with pytest.raises(ValueError):
+            pool.add_cache(cache)
+    pool.extend([0], [20])
+    pool.fork([0], [1])
+    assert pool.status() == (0, 0) and pool.table.tolist() == [[0, 1, -1, -1], [0, 2, -1, -1]]
