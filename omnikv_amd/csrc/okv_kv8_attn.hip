@@ -1,8 +1,12 @@
 // Decode attention over the 8-bit K/V cache: okv_kv8_dense_attn, okv_kv8_sparse_attn.
 //
-// A launch of splits (each workgroup a range of one request's rows for one kv head: running maximum,
-// sum and output of a softmax over its rows), then one launch that joins the splits and finishes the
-// filter layer's scores.
+// out = sum_t p_t v_t, p_t = exp(s q.k_t - m) / sum exp(...), with k_t and v_t codes times a scale per block: the K scale
+// multiplies the logit, the V scale the probability, and the codes themselves go through the matrix cores as they are
+// (every code of either format is exact in 16 bits).
+//
+// A launch of splits (each workgroup a share of one request's rows for one kv head or two: running maximum,
+// sum and output of a softmax over its rows), then one launch that joins the shares and finishes the
+// filter layer's scores.  Short requests take one launch (kv8_plan).
 #include <math.h>
 #include <string.h>
 
@@ -267,7 +271,15 @@ struct Kv8Rows {
   int k[4], v[4], s;   // gather: index entries
 };
 
-// grid (Hkv, splits, batch), four waves that take 32-row tiles in turn.
+// A workgroup per share and kv head (or pair of them), four waves that take 32-row tiles in turn.
+//
+// Bound by the codes' bytes: every row is read once, in whole 128-byte lines, a tile in flight while the one before is
+// consumed.  One launch, eight kv heads: 450001 tokens of int8 (922 MB) 143 us = 6.4 TB/s, 131073 of e4m3 (269 MB) 44 us = 6.1,
+// with scores 52 (16.8 MB of logits are written besides), sixteen requests of 8K..32K tokens in a pool of 16-token pages (608 MB) 114 us =
+// 5.3.  With the arithmetic replaced by xors the same loads take as long (142, 51 with scores, 118).  Through an index, a
+// wave has one or two tiles and the round trips (length, index, rows, write) bound it: 8781 rows of 131072 11.1 us, 9.6 for the
+// loads alone; 19854 rows of sixteen requests 17.8.  Row loads are non-temporal: 149 against 167 us at 450001 tokens, and as
+// much better through an index (23.2 against 24.5) unless the rows lie in the last-level cache already.
 //
 // q.K^T: the tile's codes become 16-bit elements (exact) and are the A operand of v_mfma_f32_16x16x32: lane 16j + m
 // holds row m, elements 16j .. +16 and 64 + 16j .. +16.  Loading that directly would touch 16 rows x 64 bytes per
@@ -279,10 +291,11 @@ struct Kv8Rows {
 // eight elements, turned by byte permutes as they are decoded.
 // Scales of K are applied to the fp32 logits.  One running maximum per q head and wave; the waves meet in LDS.
 //
-// NH 2 (paged, an even number of kv heads): a wave takes sixteen rows of two neighbouring heads instead of 32 rows of one;
-// what is said of the upper sixteen rows then holds for the second head.  A pool stores a token's heads next to each other,
-// and 128-byte pieces a token's row apart reach memory less well than 256-byte ones: 288000 tokens of one request
-// 122.3 -> 113.2 us, sixteen of 18000 each 121.1 -> 117.6.  Through an index it made no difference (22.1, 22.6).
+// NH 2 (paged, an even number of kv heads, a token's heads next to each other): a wave takes sixteen rows of two neighbouring
+// heads instead of 32 rows of one; what is said of the upper sixteen rows then holds for the second head.
+// 128-byte pieces a token's row apart reach memory less well than 256-byte ones: 288000 tokens of one request
+// 122.3 -> 113.2 us, sixteen of 18000 each 121.1 -> 117.6; one descriptor for both heads, scales read by plain loads 119.5 -> 117.9
+// (sixteen of 8K..32K).  Through an index it made no difference (22.1, 22.6).
 template <typename T, typename F, int MODE, bool LOGITS, int NH>
 __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv8_split(Kv8Attn a) {
   extern __shared__ float lds[];
@@ -340,8 +353,9 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   uint32_t koff[4], voff[4];  // of the lane's rows in a tile
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    koff[i] = (uint32_t)(8 * (MODE == kPaged ? i & 1 : i) + m8) * ts + kcol;
-    voff[i] = (uint32_t)((MODE == kPaged ? 0 : 16 * (i >> 1)) + 4 * j + 2 * (i & 1) + hi8) * ts + vcol;
+    const uint32_t second = NH == 2 && i >= 2 ? (uint32_t)c.head_stride : 0;  // the pair's other head
+    koff[i] = (uint32_t)(8 * (MODE == kPaged ? i & 1 : i) + m8) * ts + kcol + second;
+    voff[i] = (uint32_t)((MODE == kPaged ? 0 : 16 * (i >> 1)) + 4 * j + 2 * (i & 1) + hi8) * ts + vcol + second;
   }
   const int last = main_end - 1;
   const int32_t* table = c.page_table + (int64_t)b * c.page_table_stride;
@@ -381,25 +395,28 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
       }
       x.ok = 3;
     } else if (MODE == kPaged) {
+      // sixteen rows lie in one page: those behind the end are in it too, and a scale is always there to be read
       x.ok = 0;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int u = t + (NH == 1 ? 16 * s : 0), n = min(16, main_end - u), page = r.page[NH == 1 ? s : 0];
+      for (int s = 0; s < 2 / NH; ++s) {
+        const int u = t + 16 * s, n = min(16, main_end - u), page = r.page[s];
         const bool in = (uint32_t)page < (uint32_t)c.num_pages;
         const int64_t p = in ? page : 0;
         const int slot = slot_of(u);
-        const int64_t base = p * c.page_stride + (int64_t)slot * ts + (NH == 1 ? 0 : s * c.head_stride);
-        const uint32_t bytes = in && n > 0 ? (uint32_t)(n - 1) * ts + kD : 0;
+        const int64_t base = p * c.page_stride + (int64_t)slot * ts;
+        const uint32_t bytes = in && n > 0 ? (uint32_t)(n - 1) * ts + kD + (NH == 2 ? (uint32_t)c.head_stride : 0) : 0;
         const __amdgpu_buffer_rsrc_t kr = as_buffer(kb + base, bytes), vr = as_buffer(vb + base, bytes);
-        x.k[2 * s] = buffer16(kr, koff[2 * s]);
-        x.k[2 * s + 1] = buffer16(kr, koff[2 * s + 1]);
-        x.v[2 * s] = buffer16(vr, voff[2 * s]);
-        x.v[2 * s + 1] = buffer16(vr, voff[2 * s + 1]);
-        const int64_t so = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride +
-                           (NH == 1 ? 0 : s * c.scale_head_stride);
-        x.ks[s] = buffer4(as_buffer(ksb + so, bytes ? 4 : 0), 0);
-        x.vs[s] = buffer4(as_buffer(vsb + so, bytes ? 4 : 0), 0);
-        x.ok |= in ? 1u << s : 0u;
+#pragma unroll
+        for (int i = 2 * s; i < 2 * s + 2 * NH; ++i) x.k[i] = buffer16(kr, koff[i]);
+#pragma unroll
+        for (int i = 2 * s; i < 2 * s + 2 * NH; ++i) x.v[i] = buffer16(vr, voff[i]);
+        const int64_t so = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          x.ks[s + h] = ksb[so + h * c.scale_head_stride];
+          x.vs[s + h] = vsb[so + h * c.scale_head_stride];
+          x.ok |= in ? 1u << (s + h) : 0u;
+        }
       }
     } else {
       // an entry outside the request's room is read as row 0 and takes no part
@@ -806,9 +823,13 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   }
 }
 
-// Blocks [0, Hq) of a request join the splits of one q head: 32 float4 columns x 8 split lanes, eight splits of a lane
-// in flight.  The other blocks finish 256 TPT scores each and work out the heads' normalisers themselves from the splits'
-// partial log-sum-exps (a few KB), so that no block waits for another.
+// out = sum_s 2^(lse_s - m) out_s / sum_s 2^(lse_s - m) over the shares s of a request.  Blocks [0, Hq) of a request do that for
+// one q head: 32 float4 columns x 8 share lanes, eight shares of a lane in flight (one column per thread and one share at a
+// time took 26 us; sixteen in flight -0.15 us for one request, +0.85 for sixteen).  The other blocks
+// finish 256 TPT scores each and work out the heads' normalisers themselves from the shares' partial
+// log-sum-exps (a few KB), so that no block waits for another.  Bound by the launch and two round trips: 64 shares of 32 heads
+// 4.4 us, with 131072 scores of 32 logits each (16.8 MB) 6.0.  Two scores to a thread where blocks of 512 are few enough to be on
+// the chip at once, else four.
 template <typename T, int TPT>
 __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
   const int b = blockIdx.y, tid = threadIdx.x;
@@ -954,11 +975,13 @@ struct Kv8Plan {
 // the gather mode.  In a batch every request ends in a share cut short, so long shares are cut in three (sixteen
 // requests of 8K..32K tokens: 136 us in one round, 124 / 121 / 122 / 127 / 136 in 2 / 3 / 4 / 6 / 8); short ones are not: a
 // workgroup's first microseconds move nothing.  A scored share stages its logits in LDS, up to 32 KB.
-static Kv8Plan kv8_plan(bool gather, bool paged, int batch, int hkv, int group, int64_t rows, int max_score, bool folded) {
+static Kv8Plan kv8_plan(const okv_kv8_cache_t& c, bool gather, int batch, int group, int64_t rows, int max_score, bool folded) {
   Kv8Plan p{};
+  const int hkv = c.num_kv_heads;
   const int64_t wgs = (int64_t)batch * hkv, all = std::max<int64_t>(rows, 1) * batch;
   p.direct = max_score == 0 && rows <= std::min<int64_t>(2048, gather ? std::max<int64_t>(256, 4 * wgs) : std::max<int64_t>(384, 8 * wgs));
-  p.pair = paged && !gather && hkv % 2 == 0 && !p.direct;
+  // (a token's heads in order within its row: rows behind the end then lie behind the second head's last one)
+  p.pair = c.page_table && !gather && hkv % 2 == 0 && !p.direct && c.head_stride >= kD && c.head_stride + kD <= c.token_stride;
   const int nh = p.pair ? 2 : 1;
   p.least = 128 / nh;  // one tile per wave
   p.target = std::max(1, 256 * (gather ? kGatherResident : 2) * nh / hkv);  // shares of one round
@@ -1046,7 +1069,7 @@ static int kv8_attend(Kv8Attn& a, int64_t rows, int batch, void* ws, size_t ws_b
   OKV_REQUIRE(rows * batch <= (1ll << 31) - 65536, OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
   const bool folded = a.max_score_len > 0 && a.normalise == OKV_NORM_RAW;
   if (folded) a.fold = a.head_reduce == OKV_REDUCE_MAX ? 1 : 2;
-  const Kv8Plan p = kv8_plan(a.idx != nullptr, a.c.page_table != nullptr, batch, hkv, a.group, rows, a.max_score_len, folded);
+  const Kv8Plan p = kv8_plan(a.c, a.idx != nullptr, batch, a.group, rows, a.max_score_len, folded);
   const size_t need = kv8_workspace(p, batch, a.hq, hkv, a.max_score_len, folded, &a, (char*)ws);
   OKV_REQUIRE(ws != nullptr || need == 0, OKV_ERR_INVALID, "workspace pointer is NULL");
   OKV_REQUIRE(ws_bytes >= need, OKV_ERR_WORKSPACE, "workspace too small: have %zu, need %zu", ws_bytes, need);
@@ -1068,7 +1091,7 @@ int okv_kv8_workspace_bytes(const okv_kv8_cache_t* cache, int32_t num_q_heads, i
   const int hkv = cache->num_kv_heads;
   OKV_REQUIRE(batch >= 1 && hkv >= 1 && num_q_heads >= hkv && max_rows >= 0 && max_score_len >= 0, OKV_ERR_INVALID,
               "bad batch, head counts or lengths");
-  const Kv8Plan p = kv8_plan(indexed != 0, cache->page_table != nullptr, batch, hkv, num_q_heads / hkv, max_rows, max_score_len, false);
+  const Kv8Plan p = kv8_plan(*cache, indexed != 0, batch, num_q_heads / hkv, max_rows, max_score_len, false);
   *out_bytes = kv8_workspace(p, batch, num_q_heads, hkv, max_score_len, false, nullptr, nullptr);
   return OKV_OK;
 }

@@ -28,7 +28,11 @@ def main():
                              "empty", "gather", "copy",
                              "offload_memcpy", "offload_zero_copy", "offload_incremental", "h2d", "window", "window_loop", "window_fused", "window_then_dense",
                              "paged_dense", "paged_fused", "paged_fused_select", "paged_score", "paged_topk", "paged_sparse", "paged_sparse_slots",
-                             "paged_sparse_floor"])
+                             "paged_sparse_floor",
+                             "kv8_append", "kv8_read", "kv8_dense", "kv8_fused", "kv8_sparse", "paged_kv8_dense", "paged_kv8_fused",
+                             "paged_kv8_sparse_slots", "pages_fork", "pages_compact"])
+    ap.add_argument("--kv-format", default="e4m3", choices=sorted(ops.KV8_FORMATS), help="codes of the *kv8* ops")
+    ap.add_argument("--kv-block", type=int, default=64, help="tokens per scale of the *kv8* ops (paged: at most the page)")
     ap.add_argument("--batch", type=int, default=16, help="requests of the paged_* ops (ragged lengths 8192..32768)")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--pages-in-order", action="store_true", help="paged_* ops: identity page table instead of shuffled")
@@ -65,6 +69,8 @@ def main():
     dev = torch.device("cuda:0")
     if args.op.startswith("paged_"):
         return paged(args, dev)
+    if args.op.startswith("pages_"):
+        return pages(args, dev)
     dtype = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[args.dtype]
     es = 4 if dtype == torch.float32 else 2
     n, tail, nl = args.ctx, args.tail, args.layers
@@ -96,6 +102,11 @@ def main():
     dst = torch.empty_like(ks[0]) if args.op == "copy" else None
     qw = [torch.randn((1, HQ, args.window, D), generator=gen, device=dev).to(dtype) for _ in range(nl)] \
         if args.op.startswith("window") else None
+    kv8 = []
+    if args.op.startswith("kv8_"):
+        for l in range(nl):
+            kv8.append(ops.KV8.empty(1, HKV, n + tail, args.kv_format, args.kv_block, None, dev))
+            ops.kv8_append(kv8[l], ks[l], vs[l], close=True)
     off = None
     if args.op.startswith("offload") or args.op == "h2d":
         # one offloaded layer group: `nl` layers whose prompt K/V live in pinned host memory
@@ -181,6 +192,16 @@ def main():
         if args.op == "sparse_packed":
             return ops.sparse_attn(qs[l], packed[l][0], packed[l][1],
                                    tail_k=ks[l][:, :, n:], tail_v=vs[l][:, :, n:])
+        if args.op == "kv8_append":
+            return ops.kv8_append(kv8[l], ks[l], vs[l], close=True)
+        if args.op == "kv8_read":
+            return ops.kv8_read(kv8[l], dtype, seq_len=n + tail)
+        if args.op == "kv8_dense":
+            return ops.kv8_dense_attn(qs[l], kv8[l], seq_len=n + tail)
+        if args.op == "kv8_fused":
+            return ops.kv8_dense_attn(qs[l], kv8[l], seq_len=n + tail, selector=args.selector, score_len=n)
+        if args.op == "kv8_sparse":
+            return ops.kv8_sparse_attn(qs[l], kv8[l], idx=idx, tail_k=ks[l][:, :, n:], tail_v=vs[l][:, :, n:])
         if args.op == "gather":
             return ops.gather_rows(ks[l][:, :, :n], idx)
         if args.op == "copy":
@@ -195,7 +216,13 @@ def main():
             return None
 
     row = HKV * D * es
+    row8 = HKV * (D + 4.0 / args.kv_block)  # codes and their share of a scale
     algo = {
+        "kv8_append": 2.0 * (n + tail) * (row + row8),
+        "kv8_read": 2.0 * (n + tail) * (row + row8),
+        "kv8_dense": 2.0 * (n + tail) * row8,
+        "kv8_fused": 2.0 * (n + tail) * row8 + 4.0 * n,
+        "kv8_sparse": 2.0 * k_sel * row8 + 2.0 * tail * row + 4.0 * k_sel,
         "dense": 2.0 * (n + tail) * row,
         "fused": 2.0 * (n + tail) * row + 4.0 * n,
         "fused_select": 2.0 * (n + tail) * row + 4.0 * n + 4.0 * k_sel,
@@ -230,7 +257,7 @@ def main():
     e1.synchronize()
     us = e0.elapsed_time(e1) * 1e3 / args.reps
     res = {"op": args.op, "ctx": n, "selected": k_sel, "tail": tail, "dtype": args.dtype,
-           "layout": args.layout, "us_per_call": us, "algorithmic_bytes": algo,
+           "layout": args.layout, **({"kv_format": args.kv_format, "kv_block": args.kv_block} if kv8 else {}), "us_per_call": us, "algorithmic_bytes": algo,
            "algorithmic_GBps": algo / us / 1e3 if algo else None, "frac_of_8TBps": algo / us / 1e3 / 8000.0}
     if args.op == "sparse_timeline":
         res["timeline_ns"] = sparse_timeline()
@@ -303,6 +330,14 @@ def paged(args, dev):
         pk = torch.empty((total, args.page_size, HKV, D), dtype=dtype, device=dev).normal_(generator=gen)
         pv = torch.empty((total, args.page_size, HKV, D), dtype=dtype, device=dev).normal_(generator=gen)
         pools.append(ops.PagedKV(pk, pv, table.to(dev), args.page_size))
+    block = min(args.kv_block, args.page_size)
+    if args.op.startswith("paged_kv8"):
+        lens32 = lens.to(dev).to(torch.int32)
+        for l, pool in enumerate(pools):  # the same rows in 8 bits, request by request through the same table
+            c = ops.KV8.empty_paged(pool.page_table, total, args.page_size, HKV, args.kv_format, block, dtype)
+            new = torch.empty((args.batch, HKV, int(lens.max()), D), dtype=dtype, device=dev).normal_(generator=gen)
+            ops.kv8_append(c, new, new, 0, lens32)
+            pools[l] = c
     if args.contiguous:
         dense_ = lambda q, kv, **kw: ops.dense_attn(q, kv[0], kv[1], **kw)
         sparse_ = lambda q, kv, **kw: ops.sparse_attn(q, kv[0], kv[1], **kw)
@@ -312,6 +347,8 @@ def paged(args, dev):
     qs = [torch.randn((args.batch, HQ, 1, D), generator=gen, device=dev).to(dtype) for _ in range(nl)]
     lens_d = lens.to(dev)
     nmax = int(lens.max())
+    if args.op.startswith("paged_kv8"):
+        dense_, sparse_ = ops.kv8_dense_attn, ops.kv8_sparse_attn
     k_per = torch.tensor([max(1, int(args.ratio * int(n))) for n in lens], dtype=torch.int32)
     kmax, k_per_d = int(k_per.max()), k_per.to(dev)
     _, scores = dense_(qs[0], pools[0], seq_len=nmax, seq_lens=lens_d, selector=args.selector, score_len=nmax,
@@ -319,7 +356,7 @@ def paged(args, dev):
     idx = torch.zeros((args.batch, kmax), dtype=torch.int32, device=dev)
     ops.topk(scores, kmax, seq_lens=lens_d, k_per_seg=k_per_d, out=idx)
 
-    slots = pools[0].slot_index(idx) if args.op in ("paged_sparse_slots", "paged_sparse_floor") else None
+    slots = pools[0].slot_index(idx) if args.op in ("paged_sparse_slots", "paged_kv8_sparse_slots", "paged_sparse_floor") else None
     floor = None
     if args.op == "paged_sparse_floor":
         # the load-only counterpart of paged_sparse_slots: same grid, slot lookups, loads and bytes, no arithmetic
@@ -335,9 +372,9 @@ def paged(args, dev):
 
     def call(i):
         l = i % nl
-        if args.op == "paged_dense":
+        if args.op in ("paged_dense", "paged_kv8_dense"):
             return dense_(qs[l], pools[l], seq_len=nmax, seq_lens=lens_d)
-        if args.op == "paged_fused":
+        if args.op in ("paged_fused", "paged_kv8_fused"):
             return dense_(qs[l], pools[l], seq_len=nmax, seq_lens=lens_d, selector=args.selector,
                                   score_len=nmax, score_lens=lens_d)
         if args.op == "paged_fused_select":
@@ -352,13 +389,14 @@ def paged(args, dev):
             return check(lib().okv_diag_gather_floor(pools[l].pool_k.data_ptr(), pools[l].pool_v.data_ptr(), C.byref(lay),
                                                      slots.data_ptr(), slots.stride(0), k_per_d.data_ptr(), kmax, args.batch,
                                                      rows, 4, sink.data_ptr(), torch.cuda.current_stream().cuda_stream))
-        if args.op == "paged_sparse_slots":
-            return ops.sparse_attn(qs[l], pools[l], slots=slots, sel_len=kmax, sel_lens=k_per_d)
+        if args.op in ("paged_sparse_slots", "paged_kv8_sparse_slots"):
+            return sparse_(qs[l], pools[l], slots=slots, sel_len=kmax, sel_lens=k_per_d)
         return sparse_(qs[l], pools[l], idx=idx, sel_len=kmax, sel_lens=k_per_d)
 
     tokens, sel = int(lens.sum()), int(k_per.sum())
-    row = HKV * D * es
-    algo = {"paged_dense": 2.0 * tokens * row, "paged_fused": 2.0 * tokens * row + 4.0 * tokens,
+    row = HKV * D * es if not args.op.startswith("paged_kv8") else HKV * (D + 4.0 / block)
+    algo = {"paged_kv8_dense": 2.0 * tokens * row, "paged_kv8_fused": 2.0 * tokens * row + 4.0 * tokens,
+            "paged_kv8_sparse_slots": 2.0 * sel * row + 4.0 * sel, "paged_dense": 2.0 * tokens * row, "paged_fused": 2.0 * tokens * row + 4.0 * tokens,
             "paged_fused_select": 2.0 * tokens * row + 4.0 * tokens + 4.0 * sel,
             "paged_score": 1.0 * tokens * row + 4.0 * tokens, "paged_topk": 4.0 * tokens + 4.0 * sel,
             "paged_sparse": 2.0 * sel * row + 4.0 * sel, "paged_sparse_slots": 2.0 * sel * row + 4.0 * sel,
@@ -385,6 +423,57 @@ def paged(args, dev):
         torch.cuda.synchronize()
         res["copy_bytes_each_way"] = csrc.numel() * es
     print(json.dumps(res))
+
+
+def pages(args, dev):
+    """Page operations over `--layers` layers of an 8-bit pool (K, V and their scales): `--batch` sequences end, are forked
+    from `--batch` others of ragged length and grow; or a third of 4096 scattered pages is compacted."""
+    page, nl = args.page_size, args.layers
+    block = min(args.kv_block, page)
+    gen = torch.Generator().manual_seed(3)
+    if args.op == "pages_compact":
+        num, width = 4096, 64
+        used = torch.randperm(num, generator=gen)[: num // 3].to(torch.int32)
+        seqs = -(-used.numel() // width)
+        flat = torch.full((seqs * width,), -1, dtype=torch.int32)
+        flat[: used.numel()] = used
+        table, refs = flat.view(seqs, width).to(dev), torch.zeros(num, dtype=torch.int32)
+        refs[used.long()] = 1
+        refs, moved = refs.to(dev), int((used >= used.numel()).sum())
+    else:
+        lens = torch.randint(1, 4096, (args.batch,), generator=gen, dtype=torch.int32)
+        width = 4096 // page + 2
+        num = int((-(-lens // page)).sum()) + 3 * args.batch
+        pool_table = torch.full((2 * args.batch, width), -1, dtype=torch.int32, device=dev)
+        pool_lens, refs = torch.zeros(2 * args.batch, dtype=torch.int32, device=dev), torch.zeros(num, dtype=torch.int32, device=dev)
+        parents = torch.arange(args.batch, dtype=torch.int32, device=dev)
+        ops.pages_extend(pool_table, pool_lens, refs, parents, lens.to(dev), page)
+        children, grow = parents + args.batch, torch.full((args.batch,), page, dtype=torch.int32, device=dev)
+        moved = int((lens % page != 0).sum())
+    arrays = [torch.zeros((num, page, HKV, D), dtype=torch.uint8, device=dev) for _ in range(2 * nl)]
+    arrays += [torch.zeros((num, page // block, HKV), device=dev) for _ in range(2 * nl)]
+    bufs = ops.PageBuffers(arrays)
+
+    def call():
+        if args.op == "pages_compact":  # (into new arrays: every call finds the same pages)
+            return ops.pages_compact(table, refs, bufs)
+        ops.pages_free(pool_table, pool_lens, refs, children, page)
+        ops.pages_fork(pool_table, pool_lens, refs, parents, children, page, bufs)
+        ops.pages_extend(pool_table, pool_lens, refs, children, grow, page)
+
+    for _ in range(args.warmup):
+        call()
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    for _ in range(args.reps):
+        call()
+    e1.record()
+    e1.synchronize()
+    us = e0.elapsed_time(e1) * 1e3 / args.reps
+    algo = 2.0 * moved * 2 * nl * page * HKV * (D + 4.0 / block)  # read and written
+    print(json.dumps({"op": args.op, "layers": nl, "page_size": page, "pages_copied": moved, "us_per_call": us,
+                      "algorithmic_bytes": algo, "algorithmic_GBps": algo / us / 1e3, "frac_of_8TBps": algo / us / 1e3 / 8000.0}))
 
 
 if __name__ == "__main__":

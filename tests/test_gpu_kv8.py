@@ -466,6 +466,39 @@ def test_long_cache_offsets_pass_32_bits():
     check_attention(ops.kv8_sparse_attn(q.to(DEV), cache, idx=idx), q, kk, vv, 128 ** -0.5, BF)
 
 
+@pytest.mark.parametrize("layout", ["head by head", "every other head", "token padded"])
+def test_pages_in_other_layouts(layout):
+    """Pools whose heads of a token do not lie back to back; rows behind the end hold codes that decode to NaN."""
+    g = torch.Generator().manual_seed(37)
+    pages, page, hkv, lens = 24, 32, 4, [333, 17, 250]
+    if layout == "head by head":
+        k, v = (torch.full((pages, hkv, page, 128), 0x7F, dtype=torch.uint8, device=DEV).transpose(1, 2) for _ in "kv")
+    elif layout == "every other head":
+        k, v = (torch.full((pages, page, 2 * hkv, 128), 0x7F, dtype=torch.uint8, device=DEV)[:, :, ::2] for _ in "kv")
+    else:
+        k, v = (torch.full((pages, page, hkv + 1, 128), 0x7F, dtype=torch.uint8, device=DEV)[:, :, :hkv] for _ in "kv")
+    s = torch.full((2, pages, page // 16, hkv), float("nan"), device=DEV)
+    order, table = torch.randperm(pages, generator=g).to(torch.int32).tolist(), torch.full((3, 11), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        for i in range(-(-n // page)):
+            table[b, i] = order.pop()
+    table = table.to(DEV)
+    cache = ops.KV8(k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn), s[0], s[1], 16, page_table=table)
+    x, y = rows(g, 3, hkv, 333), rows(g, 3, hkv, 333)
+    for b, n in enumerate(lens):
+        one = ops.KV8(cache.k, cache.v, s[0], s[1], 16, page_table=table[b: b + 1])
+        ops.kv8_append(one, x[b: b + 1, :, :n].to(DEV), y[b: b + 1, :, :n].to(DEV), 0, close=True)
+    q = rows(g, 3, 4 * hkv)
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    ks, vs = ([held(z[b, :, :n], "e4m3", 16, False) for b, n in enumerate(lens)] for z in (x, y))
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache, seq_len=340, seq_lens=t), q, ks, vs, 128 ** -0.5, BF)
+    out, raw = ops.kv8_dense_attn(q.to(DEV), cache, seq_len=340, seq_lens=t, selector="last", score_len=340, score_lens=t)
+    check_attention(out, q, ks, vs, 128 ** -0.5, BF)
+    for b, n in enumerate(lens):
+        _, z, _, _, mass = ref.attention(q[b], ks[b], vs[b], 128 ** -0.5)
+        assert bool(((raw[b, :n].cpu().double() - z.amax(0)).abs() <= ref.logit_error(mass).amax(0)).all())
+
+
 def test_append_at_the_last_token_numbers():
     """A page table of almost 2^31 tokens whose last page alone lies in the pool: block numbers behind the end do not wrap."""
     g = torch.Generator().manual_seed(34)
