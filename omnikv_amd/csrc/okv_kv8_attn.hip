@@ -253,9 +253,6 @@ __device__ __forceinline__ uint4 buffer16(__amdgpu_buffer_rsrc_t r, uint32_t off
   const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 2);  // 2: non-temporal
   return make_uint4(v.x, v.y, v.z, v.w);
 }
-__device__ __forceinline__ float buffer4(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
-  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0));
-}
 
 enum { kContiguous = 0, kPaged = 1, kGather = 2 };
 
@@ -388,10 +385,10 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
 #pragma unroll
       for (int i = 0; i < 4; ++i) x.v[i] = buffer16(vr, voff[i]);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {  // the same four bytes for every lane
-        const int64_t so = (int64_t)((t + 16 * s) >> a.block_shift) * c.scale_block_stride;
-        x.ks[s] = buffer4(as_buffer(ksb + so, n > 16 * s ? 4 : 0), 0);
-        x.vs[s] = buffer4(as_buffer(vsb + so, n > 16 * s ? 4 : 0), 0);
+      for (int s = 0; s < 2; ++s) {  // the same four bytes for every lane; behind the end the last row's, unused
+        const int64_t so = (int64_t)(min(t + 16 * s, last) >> a.block_shift) * c.scale_block_stride;
+        x.ks[s] = ksb[so];
+        x.vs[s] = vsb[so];
       }
       x.ok = 3;
     } else if (MODE == kPaged) {
