@@ -254,6 +254,14 @@ __device__ __forceinline__ uint4 buffer16(__amdgpu_buffer_rsrc_t r, uint32_t off
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// What is read at the same address by the whole wave and written by nobody meanwhile, as a scalar load: among the vector
+// loads, which come back in order, it would have to wait for the rows asked for before it (sixteen requests of 8K..32K tokens
+// in a pool, with scores: 154.6 -> 143.5 us; 131073 tokens with scores 57.7 -> 57.3).
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 enum { kContiguous = 0, kPaged = 1, kGather = 2 };
 
 // A wave's 32 rows as lane l = 16j + m holds them: load i has K row 8i + (m & 7), chunk j + 4(m >> 3) of sixteen bytes, and
@@ -365,7 +373,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   auto rows_of = [&](int t, Kv8Rows& r) {
     if (MODE == kPaged) {
 #pragma unroll
-      for (int s = 0; s < 2 / NH; ++s) r.page[s] = table[page_of(min(t + 16 * s, last))];
+      for (int s = 0; s < 2 / NH; ++s) r.page[s] = scalar_load(table + page_of(min(t + 16 * s, last)));
     } else if (MODE == kGather) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -387,8 +395,8 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
 #pragma unroll
       for (int s = 0; s < 2; ++s) {  // the same four bytes for every lane; behind the end the last row's, unused
         const int64_t so = (int64_t)(min(t + 16 * s, last) >> a.block_shift) * c.scale_block_stride;
-        x.ks[s] = ksb[so];
-        x.vs[s] = vsb[so];
+        x.ks[s] = scalar_load(ksb + so);
+        x.vs[s] = scalar_load(vsb + so);
       }
       x.ok = 3;
     } else if (MODE == kPaged) {
@@ -410,8 +418,8 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
         const int64_t so = p * c.scale_page_stride + (int64_t)(slot >> a.block_shift) * c.scale_block_stride;
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
-          x.ks[s + h] = ksb[so + h * c.scale_head_stride];
-          x.vs[s + h] = vsb[so + h * c.scale_head_stride];
+          x.ks[s + h] = scalar_load(ksb + so + h * c.scale_head_stride);
+          x.vs[s + h] = scalar_load(vsb + so + h * c.scale_head_stride);
           x.ok |= in ? 1u << (s + h) : 0u;
         }
       }
