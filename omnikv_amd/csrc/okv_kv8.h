@@ -43,6 +43,15 @@ __device__ __forceinline__ void decode4(I8, uint32_t x, float* o) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = (float)(int8_t)(x >> (8 * i));
 }
+// two fp32 -> one dword of two 16-bit elements, the first in the low half
+__device__ __forceinline__ uint32_t pack_pair(const BF16*, float a, float b) {
+  const f32x2_t x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
+}
+__device__ __forceinline__ uint32_t pack_pair(const F16*, float a, float b) {
+  const f32x2_t x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_t));
+}
 // ---- fp32 within the format's range -> code, ties to even
 __device__ __forceinline__ uint32_t encode4(E4M3, const float* v) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);

@@ -54,16 +54,26 @@ struct AppendArgs {
   int32_t start, max_new, close;
 };
 
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+template <typename T> constexpr uint32_t kInfBits = 0x7f80;  // of bfloat16
+template <> constexpr uint32_t kInfBits<F16> = 0x7c00;
+__device__ __forceinline__ float magnitude(const BF16*, uint32_t bits) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ float magnitude(const F16*, uint32_t bits) {
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+
 // scale = max(amax / qmax, 2^-126), code = nearest(x * fl32(1 / scale)).  One workgroup per (touched block, kv head, request, K
 // or V): 16 lanes hold a row (eight elements each), sixteen rows per trip, the whole block in registers between
 // the two passes (maximum, then codes), so that each element is read once and written once.  Bound by that: 131073 tokens of
-// eight heads, bf16 to e4m3 in blocks of 64 (805 MB), 149..171 us = 4.7..5.4 TB/s, what a large copy reaches; one token
-// for each of sixteen requests 3.4 us, a launch.
+// eight heads, bf16 to e4m3 in blocks of 64 (805 MB), 132 us = 6.1 TB/s; one token for each of sixteen requests a
+// launch.  Rows come in and codes go out non-temporal (147 us without, 145 and 138 with one of the two); 152 before
+// the maximum was taken over bit patterns and the rows a block does not have were left out.
 // The workgroup of the first touched block also moves the rows of the block that stays open: it has read the old
 // open rows by then, and nobody else touches the request's open buffer.
 template <typename T, typename F>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
-  __shared__ float s_max[4];
+  __shared__ uint32_t s_max[4];
   const okv_kv8_cache_t& c = a.c;
   const int B = c.block_tokens;
   const int g = blockIdx.y, b = blockIdx.z >> 1, is_v = blockIdx.z & 1;
@@ -83,50 +93,53 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   if (whole) {
     constexpr int P = kMaxBlockTokens / 16;
     uint4 x[P];
-    float amax = 0.f;
-    bool bad = false;
+    // magnitudes order as the 16-bit patterns without the sign, infinities and NaNs above all numbers: the maximum needs
+    // no conversion and no test of each element
+    u16x2_t top = {0, 0};
 #pragma unroll
     for (int p = 0; p < P; ++p) {
+      if (16 * p >= B) break;
       const int r = 16 * p + row, t = blk * B + r;
       x[p] = make_uint4(0, 0, 0, 0);
-      if (r < B && t < end) {
+      if (t < end) {
         const T* q = t >= start ? src + (int64_t)(t - start) * row_stride : open + (int64_t)r * c.open_token_stride;
-        x[p] = *reinterpret_cast<const uint4*>(q + 8 * col);
-      }
-      float v[8];
-      cvt8((const T*)nullptr, x[p], v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        amax = fmaxf(amax, fabsf(v[i]));
-        bad = bad || !(fabsf(v[i]) < INFINITY);
+        x[p] = load_stream16(q + 8 * col);
       }
     }
-    if (bad) amax = INFINITY;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    if ((tid & 63) == 0) s_max[tid >> 6] = amax;
+    for (int p = 0; p < P; ++p) {
+      if (16 * p >= B) break;
+      for (const uint32_t w : {x[p].x, x[p].y, x[p].z, x[p].w})
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w & 0x7fff7fffu));
+    }
+    uint32_t m = top.x > top.y ? top.x : top.y;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    if ((tid & 63) == 0) s_max[tid >> 6] = m;
     __syncthreads();
-    amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    const bool poison = amax == INFINITY;
+    m = __builtin_amdgcn_readfirstlane(max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
+    const bool poison = m >= kInfBits<T>;
+    const float amax = magnitude((const T*)nullptr, m);
     const float scale = poison ? NAN : fmaxf(amax / qmax_of(F{}), kMinScale);
-    const float inv = poison ? 0.f : 1.f / scale;
+    const float inv = 1.f / scale;
     int64_t ro, so;
     if (kv8_locate(c, b, blk * B, &ro, &so)) {
       uint8_t* dst = reinterpret_cast<uint8_t*>(is_v ? c.v_codes : c.k_codes) + ro + (int64_t)g * c.head_stride;
       if (tid == 0) (is_v ? c.v_scale : c.k_scale)[so + (int64_t)g * c.scale_head_stride] = scale;
 #pragma unroll
       for (int p = 0; p < P; ++p) {
+        if (16 * p >= B) break;
         const int r = 16 * p + row;
-        if (r >= B || blk * B + r >= end) continue;
-        float v[8];
-        cvt8((const T*)nullptr, x[p], v);
+        if (blk * B + r >= end) continue;
+        uint2 codes = make_uint2(0, 0);
+        if (!poison) {
+          float v[8];
+          cvt8((const T*)nullptr, x[p], v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] *= inv;
-          v[i] = poison ? 0.f : fminf(fmaxf(v[i], -qmax_of(F{})), qmax_of(F{}));
+          for (int i = 0; i < 8; ++i) v[i] = __builtin_amdgcn_fmed3f(v[i] * inv, -qmax_of(F{}), qmax_of(F{}));
+          codes = make_uint2(encode4(F{}, v), encode4(F{}, v + 4));
         }
-        *reinterpret_cast<uint2*>(dst + (int64_t)r * c.token_stride + 8 * col) =
-            make_uint2(encode4(F{}, v), encode4(F{}, v + 4));
+        __builtin_nontemporal_store(u32x2_t{codes.x, codes.y}, reinterpret_cast<u32x2_t*>(dst + (int64_t)r * c.token_stride + 8 * col));
       }
     }
   }
@@ -139,9 +152,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
         *reinterpret_cast<const uint4*>(src + (int64_t)(t - start) * row_stride + 8 * col);
 }
 
-// value = code * scale, rounded once to 16 bits; 16 lanes per row.  Bound by the writes: 131073 tokens of eight heads (268 MB
-// read, 537 MB written) 217 us = 2.5 TB/s written, a copy's rate of writing next to reads.  Four or eight rows of a thread in flight, packed or
-// non-temporal stores changed nothing (219..222).
+// value = code * scale, rounded once to 16 bits; 16 lanes per row.  Bound by the bytes: 131073 tokens of eight heads (268 MB
+// read, 537 MB written) 178 us = 4.5 TB/s, 8001 tokens 10.9 us.  Stores of eight elements that do not stay in the caches: 201 and 13.1
+// with element-wise ones, 180 and 14.5 where the loads are non-temporal instead.  Four or eight rows of a thread in flight: no
+// difference.
 struct ReadArgs {
   okv_kv8_cache_t c;
   const int32_t* idx;
@@ -182,8 +196,9 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= s;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) store1(dst + i, v[i]);
+  const T* ty = nullptr;
+  __builtin_nontemporal_store(u32x4_t{pack_pair(ty, v[0], v[1]), pack_pair(ty, v[2], v[3]), pack_pair(ty, v[4], v[5]), pack_pair(ty, v[6], v[7])},
+                              reinterpret_cast<u32x4_t*>(dst));
 }
 
 }  // namespace okv

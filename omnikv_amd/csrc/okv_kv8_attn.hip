@@ -177,15 +177,6 @@ __device__ __forceinline__ bool find_share(const Kv8Attn& a, int item, int reque
 }
 
 // ---------------------------------------------------------------- matrix-core pieces
-// two fp32 -> one dword of two 16-bit elements, the first in the low half
-__device__ __forceinline__ uint32_t pack_pair(const BF16*, float a, float b) {
-  const f32x2_t x = {a, b};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
-}
-__device__ __forceinline__ uint32_t pack_pair(const F16*, float a, float b) {
-  const f32x2_t x = {a, b};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2_t));
-}
 __device__ __forceinline__ f32x2_t unpack_pair(const BF16*, uint32_t x) {
   return f32x2_t{__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)};
 }
