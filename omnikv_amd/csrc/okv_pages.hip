@@ -6,7 +6,7 @@
 // A plan is one workgroup, because "lowest free first" is one prefix sum over the counts and because a scan over workgroups
 // would need device-wide fences, which cost more than the scan (a plan with them took 16 us, without 3.6).  Its threads meet in LDS; what it
 // decides is read by the next launch.  It is bound by its chain of round trips to memory: 3.6 to 4.9 us for 64 forks, 4.9 to
-// compact 4096 pages, 5.2 to 7.7 for 64 sequences to grow (it writes the table's entries itself).  The pages' bytes are moved by the
+// compact 4096 pages, 5.3 for 64 sequences to grow (it writes the table's entries itself; 7.9 with a second trip through the counts).  The pages' bytes are moved by the
 // launch after it, all buffers at once.
 #include "okv_internal.h"
 
@@ -263,10 +263,12 @@ __global__ __launch_bounds__(256) void pages_fork_apply(okv_page_pool_t p, const
   if (fresh >= 0 && threadIdx.x == 0) to[full] = fresh;
 }
 
-// One thread per entry; two trips through the counts: whether there are enough free pages, then who gets which.
+// One thread per entry.  A trip through the counts finds the free pages, the first kFresh of them are kept in LDS, and if
+// there are enough a thread per page writes it into the table; a call that takes more pages goes through the counts again.
+constexpr int kFresh = 4096;
 __global__ __launch_bounds__(kPlanThreads) void pages_extend_plan(okv_page_pool_t p, const int32_t* seqs, const int32_t* more,
                                                                  int n, int32_t* status) {
-  __shared__ int s_at[kMaxEntries + 1], s_seq[kMaxEntries], s_from[kMaxEntries];
+  __shared__ int s_at[kMaxEntries + 1], s_seq[kMaxEntries], s_from[kMaxEntries], s_fresh[kFresh];
   const int i = threadIdx.x;
   int turn = 0;
   int4 refs = load_refs(p, 0);
@@ -281,34 +283,38 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_plan(okv_page_pool_
   s_seq[i] = s;
   s_from[i] = from;
   block_scan(i < n && !ok, &bad, turn);
-  for (int base = 0; base < p.num_pages && have < want; base += kTrip) {
-    const int4 r = base ? load_refs(p, base) : refs;
-    block_scan((r.x <= 0) + (r.y <= 0) + (r.z <= 0) + (r.w <= 0), &total, turn);
-    have = min(have + total, want);
-  }
+  // the k-th page taken goes to the last entry whose pages start at or before the k-th
+  auto give = [&](int k, int page) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_at[mid] <= k) lo = mid;
+      else hi = mid - 1;
+    }
+    p.table[(int64_t)s_seq[lo] * p.table_stride + s_from[lo] + (k - s_at[lo])] = page;
+    p.refs[page] = 1;
+  };
+  auto trip = [&](int base, const int4& r, int k0, auto take) {  // the number of free pages of a trip; take(k, page) of each
+    const int f[4] = {r.x <= 0, r.y <= 0, r.z <= 0, r.w <= 0};
+    int k = k0 + block_scan(f[0] + f[1] + f[2] + f[3], &total, turn);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (f[x] && k < want) take(k, base + kPerThread * i + x);
+      k += f[x];
+    }
+    return total;
+  };
+  for (int base = 0; base < p.num_pages && have < want; base += kTrip)
+    have = min(have + trip(base, base ? load_refs(p, base) : refs, have,
+                           [&](int k, int page) { if (k < kFresh) s_fresh[k] = page; }), want);
+  __syncthreads();
   if (have == want) {
     if (ok) p.lens[s] = (int)to;
-    for (int base = 0, k0 = 0; base < p.num_pages && k0 < want; base += kTrip) {
-      if (base) refs = load_refs(p, base);
-      const int f[4] = {refs.x <= 0, refs.y <= 0, refs.z <= 0, refs.w <= 0};
-      int k = k0 + block_scan(f[0] + f[1] + f[2] + f[3], &total, turn);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if (f[x] && k < want) {
-          int lo = 0, hi = n - 1;  // the last entry whose pages start at or before the k-th
-          while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s_at[mid] <= k) lo = mid;
-            else hi = mid - 1;
-          }
-          const int page = base + kPerThread * i + x;
-          p.table[(int64_t)s_seq[lo] * p.table_stride + s_from[lo] + (k - s_at[lo])] = page;
-          p.refs[page] = 1;
-        }
-        k += f[x];
-      }
-      k0 += total;
-    }
+    if (want <= kFresh)
+      for (int k = i; k < want; k += kPlanThreads) give(k, s_fresh[k]);
+    else
+      for (int base = 0, k0 = 0; base < p.num_pages && k0 < want; base += kTrip)
+        k0 += trip(base, base ? load_refs(p, base) : refs, k0, give);
   }
   if (status && i == 0) {
     status[0] = want - have;

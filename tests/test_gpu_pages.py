@@ -269,3 +269,19 @@ def test_a_refused_array_leaves_the_pool_as_it_was():
     pool.extend([0], [20])
     pool.fork([0], [1])
     assert pool.status() == (0, 0) and pool.table.tolist() == [[0, 1, -1, -1], [0, 2, -1, -1]]
+
+
+@pytest.mark.parametrize("want", [4095, 4096, 4097, 9000])
+def test_growth_by_more_pages_than_a_plan_keeps(want):
+    """Calls that take so many pages in all: one long sequence among short ones, then another of half a page more."""
+    page, r = 4, random.Random(want)
+    lens = [r.randint(0, 40) for _ in range(200)]
+    table, lt, refs, bufs, m = make(10, 210, want, 2 * want + 2200, page, lens, shapes=((1,),))
+    status = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for seqs, more in (([205, 206, 207, 208], [page * (want - 7), 1, 0, 6 * page]),
+                       ([201, 202, 203], [2 * page, page * (want - 2) - 1, -5])):
+        before = sum(refs.tolist())
+        ops.pages_extend(table, lt, refs, i32(seqs), i32(more), page, status)
+        assert status.tolist() == m.extend(seqs, more) == [0, 0]
+        assert sum(refs.tolist()) - before == want
+        same(table, lt, refs, bufs, m)
