@@ -507,12 +507,13 @@ KV8_FORMATS = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
 _SCALE128 = 1.0 / math.sqrt(128)
 _KV8_CODES = {torch.float8_e4m3fn: _lib.OKV_E4M3, torch.int8: _lib.OKV_I8}
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice  # (torch.cuda.current_device() less its check that the GPU is in use: tensors are)
 
 
 def _launch(device: torch.device, fn, *args) -> None:
     """fn(*args, current stream of `device`), with that device current: a launch goes to the current one."""
     i = device.index
-    if i != torch.cuda.current_device():
+    if i != _current_device():
         with torch.cuda.device(i):
             check(fn(*args, _raw_stream(i)))
         return
@@ -946,12 +947,12 @@ def pages_compact(table, refs, buffers, table_out: Optional[torch.Tensor] = None
     if bufs.device != dev or bufs.num_pages != refs.numel():
         raise ValueError("buffers must hold refs.numel() pages on the table's GPU")
     if table_out is None:
-        table_out = torch.empty(table.shape, dtype=torch.int32, device=dev)
+        table_out = torch.empty_like(table)
     elif table_out.shape != table.shape or table_out.dtype != torch.int32 or table_out.stride(1) != 1 or table_out.device != dev:
         raise ValueError("table_out must look like table")
     if refs_out is None:
         refs_out = torch.empty_like(refs)
-    used = torch.empty(1, dtype=torch.int32, device=dev)
+    used = refs.new_empty(1)
     ws = _pages_scratch(pool, 0, dev)
     _launch(dev, lib().okv_pages_compact, pool, table_out.data_ptr(), max(table_out.stride(0), table_out.shape[1]),
             _dev_i32(refs_out, refs.numel(), dev, "refs_out"), used.data_ptr(), bufs._c, len(bufs), ws.data_ptr(), ws.numel())
