@@ -773,15 +773,20 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
         idx = slots
     ip, istride = None, 0
     if idx is not None:
-        if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != bsz or idx.stride(1) != 1 or idx.device != dev:
+        if idx.dtype is not torch.int32 or idx.dim() != 2 or idx.device != dev:
+            raise ValueError(f"idx must be a ({bsz}, k) int32 tensor with contiguous rows on the cache's GPU")
+        (ib, width), (istride, unit) = idx.shape, idx.stride()
+        if ib != bsz or unit != 1:
             raise ValueError(f"idx must be a ({bsz}, k) int32 tensor with contiguous rows on the cache's GPU")
         if sel_len is None:
-            sel_len = idx.shape[1]
-        elif sel_len > idx.shape[1]:
+            sel_len = width
+        elif sel_len > width:
             raise ValueError("sel_len exceeds idx")
-        ip, istride = idx.data_ptr(), max(idx.stride(0), idx.shape[1])
-        if bsz > 1 and idx.stride(0) < idx.shape[1]:
-            raise ValueError("idx rows must not overlap")
+        if istride < width:
+            if bsz > 1:
+                raise ValueError("idx rows must not overlap")
+            istride = width
+        ip = idx.data_ptr()
     elif sel_len is None:
         sel_len = cache.capacity
     elif sel_len > cache.capacity:
@@ -790,17 +795,19 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
     tts = ths = tbs = 0
     if tail_k is not None:
         shape, strides = tail_k.shape, tail_k.stride()
-        if (tail_k.dim() != 4 or tail_v is None or shape != tail_v.shape or strides != tail_v.stride()
-                or strides[3] != 1 or shape[0] != bsz or shape[1] != hkv or shape[3] != 128):
+        if len(strides) != 4 or tail_v is None or shape != tail_v.shape or strides != tail_v.stride():
             raise ValueError("tail_k / tail_v must be (bsz, Hkv, T, 128), same strides, contiguous last dimension")
-        if tail_k.dtype is not q.dtype or tail_v.dtype is not q.dtype or tail_k.device != dev or tail_v.device != dev:
+        (tb, th, rows, td), (tbs, ths, tts, unit) = shape, strides
+        if tb != bsz or th != hkv or td != 128 or unit != 1:
+            raise ValueError("tail_k / tail_v must be (bsz, Hkv, T, 128), same strides, contiguous last dimension")
+        dt = q.dtype
+        if tail_k.dtype is not dt or tail_v.dtype is not dt or tail_k.device != dev or tail_v.device != dev:
             raise ValueError("tail and q differ in dtype or GPU")
         if tail_len is None:
-            tail_len = shape[2]
-        elif tail_len > shape[2]:
+            tail_len = rows
+        elif tail_len > rows:
             raise ValueError("tail_len exceeds the tail")
         tkp, tvp = tail_k.data_ptr(), tail_v.data_ptr()
-        tbs, ths, tts, _ = strides
     elif tail_len:
         raise ValueError("tail_len without a tail")
     tail_len = tail_len or 0
