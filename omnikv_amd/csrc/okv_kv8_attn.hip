@@ -49,7 +49,7 @@ struct Kv8Attn {
   int32_t least_rows;
   int32_t pair;       // two kv heads to a wave (NH 2)
   int32_t fine;       // shares of a batch longer than this are cut in three; 0: not
-  int32_t direct;     // one share per request, which writes the output itself: no second launch
+  int32_t direct;     // waves per workgroup where one share per request writes the output itself, without a second launch; 0: not
   int32_t fold;         // raw scores: the q heads of a kv head are folded by the split (1 max, 2 sum): one logits row per kv head
   int32_t logit_heads;  // rows of `logits` per request
   int32_t lds_scales;   // floats before the scale staging of the gather mode
@@ -119,9 +119,10 @@ __device__ __forceinline__ void request_lens(const Kv8Attn& a, int b, int* main_
 }
 
 // The share `item` (false: there is none), or with item < 0 the shares of request `request`.
+template <bool DIRECT>
 __device__ __forceinline__ bool find_share(const Kv8Attn& a, int item, int request, Share* s) {
   const int lane = threadIdx.x & 63;
-  if (a.direct) {
+  if (DIRECT) {
     const int b = item;
     if (b >= a.batch) return false;
     request_lens(a, b, &s->main_len, &s->L, &s->A);
@@ -292,10 +293,10 @@ struct Kv8Rows {
 // 128-byte pieces a token's row apart reach memory less well than 256-byte ones: 288000 tokens of one request
 // 122.3 -> 113.2 us, sixteen of 18000 each 121.1 -> 117.6; one descriptor for both heads, scales read by plain loads 119.5 -> 117.9
 // (sixteen of 8K..32K).  Through an index it made no difference (22.1, 22.6).
-template <typename T, typename F, int MODE, bool LOGITS, int NH>
-__global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv8_split(Kv8Attn a) {
+template <typename T, typename F, int MODE, bool LOGITS, int NH, bool DIRECT, int W>
+__global__ __launch_bounds__(64 * W, MODE == kGather && W == 4 ? kGatherResident : 2) void kv8_split(Kv8Attn a) {
   extern __shared__ float lds[];
-  constexpr int TR = 32 / NH, kStep = 4 * TR;  // rows of a tile, and between a wave's tiles
+  constexpr int TR = 32 / NH, kStep = W * TR;  // rows of a tile, and between a wave's tiles
   const okv_kv8_cache_t& c = a.c;
   if constexpr (MODE != kPaged) {  // one batch of scalar loads instead of a round trip before each first use (the paged mode's
     // page descriptors leave too few scalar registers for that: 131 against 121 us)
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
   // stored head by head next to each other (pools) are fetched together
   const int turn = blockIdx.x >> 3, groups = c.num_kv_heads / NH, g = turn % groups * NH;
   Share sh;
-  if (!find_share(a, (int)((turn / groups) * 8 + (blockIdx.x & 7)), 0, &sh)) return;
+  if (!find_share<DIRECT>(a, (int)((turn / groups) * 8 + (blockIdx.x & 7)), 0, &sh)) return;
   const int b = sh.b, main_len = sh.main_len, L = sh.L, A = LOGITS ? sh.A : 0;
   int begin, end;
   {
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     begin = sh.index < nA ? sh.index * sh.rows : A + (sh.index - nA) * sh.rows;
     end = min(begin + sh.rows, sh.index < nA ? A : L);
   }
-  if (begin >= end && !a.direct) return;  // (a request without rows gets its zeros below)
+  if (begin >= end && !DIRECT) return;  // (a request without rows gets its zeros below)
   // rows [0, closed) are codes, the rest 16-bit rows: the open block, or the tail
   const int closed = a.sparse || !c.open_k ? main_len : main_len >> a.block_shift << a.block_shift;
   const int main_end = min(end, closed);
@@ -695,7 +696,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     const int64_t lts = a.late_token_stride;
     const int64_t lbase = (int64_t)b * a.late_batch_stride + (int64_t)g * a.late_head_stride;
     const T* ty = nullptr;
-    for (int t = lo + 16 * wave; t < end; t += 64) {
+    for (int t = lo + 16 * wave; t < end; t += 16 * W) {
       const int top_row = end - 1 - closed;  // rows counted from the first late one
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
@@ -750,7 +751,7 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     for (int h = 0; h < NH * nh; ++h) {
       float* dst = a.logits + (int64_t)(b * a.logit_heads + g * nh + h) * a.logits_stride + begin;
       const float* src = slog + h * sh.rows;
-      for (int r = 4 * threadIdx.x; r < end - begin; r += 1024) {
+      for (int r = 4 * threadIdx.x; r < end - begin; r += 256 * W) {
         const float4 v = *reinterpret_cast<const float4*>(src + r);
         if (begin + r + 3 < end) {
           *reinterpret_cast<float4*>(dst + r) = v;
@@ -766,9 +767,9 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
 
   // ---- the four waves meet
   constexpr int kCell = NH * kMaxGroup;
-  float* sm = lds;              // [4][NH][8] running maximum
-  float* sl = lds + 4 * kCell;  // [4][NH][8] sum of exponentials
-  float* so = lds + 8 * kCell;  // [4][NH G][128]
+  float* sm = lds;                  // [W][NH][8] running maximum
+  float* sl = lds + W * kCell;      // [W][NH][8] sum of exponentials
+  float* so = lds + 2 * W * kCell;  // [W][NH G][128]
 #pragma unroll
   for (int n = 0; n < NH; ++n) {
     l[n] = rows_sum(l[n]);
@@ -794,22 +795,22 @@ __global__ __launch_bounds__(256, MODE == kGather ? kGatherResident : 2) void kv
     }
   }
   __syncthreads();
-  for (int o = threadIdx.x; o < NH * G * kD; o += 256) {
+  for (int o = threadIdx.x; o < NH * G * kD; o += 64 * W) {
     const int h = o / kD, d = o % kD;  // q head of the workgroup's NH G
     const int cell = NH == 1 ? h : h < G ? h : kMaxGroup + h - G;
     float M = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) M = fmaxf(M, sm[x * kCell + cell]);
+    for (int x = 0; x < W; ++x) M = fmaxf(M, sm[x * kCell + cell]);
     const float Ms = M == -INFINITY ? 0.f : M;
     float den = 0.f, num = 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 0; x < W; ++x) {
       const float f = __builtin_amdgcn_exp2f(sm[x * kCell + cell] - Ms);
       den = fmaf(sl[x * kCell + cell], f, den);
       num = fmaf(so[(x * NH * G + h) * kD + d], f, num);
     }
     // den 0: no row took part (a NaN among the logits leaves NaN)
-    if (a.direct) {
+    if (DIRECT) {
       store1(reinterpret_cast<T*>(a.out) + (int64_t)(b * a.hq + g * G + h) * kD + d, den == 0.f ? 0.f : num / den);
       continue;
     }
@@ -830,7 +831,7 @@ template <typename T, int TPT>
 __global__ __launch_bounds__(256) void kv8_join(Kv8Attn a) {
   const int b = blockIdx.y, tid = threadIdx.x;
   Share sh;
-  find_share(a, -1, b, &sh);
+  find_share<false>(a, -1, b, &sh);
   const int A = sh.A;
   constexpr int U = 8;
   if ((int)blockIdx.x < a.hq) {
@@ -957,15 +958,19 @@ static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How a call is run, from its sizes and layout alone.
 struct Kv8Plan {
-  bool direct, pair;
+  int direct;  // waves of a workgroup, or 0
+  bool pair;
   int target, most, least, items;
   bool fine;
 };
 
 // direct: a share per request, and no second launch: where requests are short, and longer ones where there are many, the
-// rows a wave then takes one after the other cost less than the join and the round trip through memory.  Measured (bf16,
-// int8, eight kv heads; one launch against two, us): 1 x 333 rows 7.6 / 8.0, 1 x 512 8.2 / 7.8, 16 x 1024 13.6 / 17.0,
-// 64 x 1536 37.8 / 54.3; through an index 1 x 256 7.3 / 8.3, 1 x 333 9.9 / 8.8, 16 x 512 12.9 / 13.1, 64 x 1536 42.1 / 61.1.
+// rows a wave then takes one after the other cost less than the join and the round trip through memory.  Eight waves to a
+// workgroup as long as every workgroup has a CU of its own, else four.  Measured (bf16, int8, eight kv heads; one launch against
+// two, us): contiguous 1 x 333 rows 6.5 / 7.4, 1 x 512 7.7 / 7.2, 4 x 512 7.8 / 8.3, 4 x 768 9.5 / 8.3, 16 x 1024 11.8 / 15.0,
+// 64 x 1536 32.4 / 44.2; through an index 1 x 333 6.9 / 7.9, 1 x 512 8.2 / 8.1, 8 x 512 8.9 / 9.3, 8 x 768 11.9 / 10.9,
+// 16 x 768 13.0 / 14.0, 16 x 1536 20.2 / 19.4, 64 x 1536 38.0 / 44.3.  Four waves: 1 x 333 7.1; eight at 64 x 512 16.5 for 12.6.
+// Requests of unequal lengths gain less, since the longest decides: hence no more than 2048.
 //
 // Else one round of workgroups, of which the chip holds two per CU (their registers allow two waves per SIMD), three of
 // the gather mode.  In a batch every request ends in a share cut short, so long shares are cut in three (sixteen
@@ -975,7 +980,8 @@ static Kv8Plan kv8_plan(const okv_kv8_cache_t& c, bool gather, int batch, int gr
   Kv8Plan p{};
   const int hkv = c.num_kv_heads;
   const int64_t wgs = (int64_t)batch * hkv, all = std::max<int64_t>(rows, 1) * batch;
-  p.direct = max_score == 0 && rows <= std::min<int64_t>(2048, gather ? std::max<int64_t>(256, 4 * wgs) : std::max<int64_t>(384, 8 * wgs));
+  if (max_score == 0 && rows <= std::min<int64_t>(2048, std::max<int64_t>(512, (gather ? 6 : 8) * wgs)))
+    p.direct = wgs <= 256 ? 8 : 4;
   // (a token's heads in order within its row: rows behind the end then lie behind the second head's last one)
   p.pair = c.page_table && !gather && hkv % 2 == 0 && !p.direct && c.head_stride >= kD && c.head_stride + kD <= c.token_stride;
   const int nh = p.pair ? 2 : 1;
@@ -1017,19 +1023,32 @@ static size_t kv8_workspace(const Kv8Plan& p, int batch, int hq, int hkv, int ma
   return o + l + g + 256;
 }
 
-template <typename T, typename F, int MODE, bool LOGITS, int NH>
+template <typename T, typename F, int MODE, bool LOGITS, int NH, bool DIRECT = false, int W = 4>
 static int launch_split(Kv8Attn& a, int batch, hipStream_t stream) {
-  size_t floats = NH * (8 * kMaxGroup + (size_t)4 * a.group * kD);
+  size_t floats = NH * (2 * W * kMaxGroup + (size_t)W * a.group * kD);
   if (LOGITS) floats = std::max(floats, (size_t)NH * (a.fold ? 1 : a.group) * a.most_rows);
   a.lds_scales = (int)floats;
-  if (MODE == kGather) floats += 256;
-  hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS, NH>), dim3((a.items + 7) / 8 * 8 * (a.c.num_kv_heads / NH)), dim3(256), floats * 4, stream, a);
+  if (MODE == kGather) floats += 64 * W;
+  hipLaunchKernelGGL((kv8_split<T, F, MODE, LOGITS, NH, DIRECT, W>), dim3((a.items + 7) / 8 * 8 * (a.c.num_kv_heads / NH)), dim3(64 * W), floats * 4, stream, a);
   return OKV_OK;
+}
+
+template <typename T, typename F, int W>
+static void launch_direct(Kv8Attn& a, int batch, hipStream_t stream) {
+  if (a.idx) launch_split<T, F, kGather, false, 1, true, W>(a, batch, stream);
+  else if (a.c.page_table) launch_split<T, F, kPaged, false, 1, true, W>(a, batch, stream);
+  else launch_split<T, F, kContiguous, false, 1, true, W>(a, batch, stream);
 }
 
 template <typename T, typename F>
 static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
   const bool paged = a.c.page_table != nullptr, scored = a.max_score_len > 0;
+  if (a.direct) {
+    if (a.direct == 8) launch_direct<T, F, 8>(a, batch, stream);
+    else launch_direct<T, F, 4>(a, batch, stream);
+    OKV_HIP_CHECK(hipGetLastError());
+    return OKV_OK;
+  }
   if (a.idx) launch_split<T, F, kGather, false, 1>(a, batch, stream);
   else if (paged && scored && a.pair) launch_split<T, F, kPaged, true, 2>(a, batch, stream);
   else if (paged && scored) launch_split<T, F, kPaged, true, 1>(a, batch, stream);
@@ -1037,10 +1056,6 @@ static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
   else if (paged) launch_split<T, F, kPaged, false, 1>(a, batch, stream);
   else if (scored) launch_split<T, F, kContiguous, true, 1>(a, batch, stream);
   else launch_split<T, F, kContiguous, false, 1>(a, batch, stream);
-  if (a.direct) {
-    OKV_HIP_CHECK(hipGetLastError());
-    return OKV_OK;
-  }
   const int64_t shares = a.items / a.batch;
   const int tokens = shares * ((a.max_score_len + 511) / 512) <= 65536 ? 512 : 1024;
   const dim3 grid(a.hq + (a.max_score_len + tokens - 1) / tokens, batch);

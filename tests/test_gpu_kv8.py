@@ -311,6 +311,28 @@ def test_batch_of_many_ragged_requests(page):
     check_attention(got, q, [k[:, :n:3] for k, n in zip(ks, closed)], [v[:, :n:3] for v, n in zip(vs, closed)], 128 ** -0.5, BF)
 
 
+@pytest.mark.parametrize("bsz, hkv, most", [(1, 8, 512), (3, 2, 513), (70, 4, 500), (70, 4, 2047), (33, 8, 130)])
+@pytest.mark.parametrize("page", [0, 48])
+def test_short_requests_in_one_launch(bsz, hkv, most, page):
+    """Around the sizes where a request is one share, few and many of them, one of no rows, one of a single open row."""
+    g = torch.Generator().manual_seed(27)
+    lens = [int(x) for x in torch.randint(2, most + 1, (bsz,), generator=g)]
+    lens[0] = most
+    if bsz > 2:
+        lens[1], lens[2] = 0, 1
+    cache, ks, vs = make(g, "int8", HF, 16, page, lens, hkv)
+    q = rows(g, bsz, 2 * hkv, dtype=HF)
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=t, seq_len=most), q, ks, vs, 128 ** -0.5, HF)
+    closed = [n // 16 * 16 for n in lens]
+    idx = torch.arange(0, most, dtype=torch.int32, device=DEV).flip(0).expand(bsz, -1).contiguous()
+    idx[idx >= torch.tensor(closed, device=DEV)[:, None]] = -1  # padding in front of the request's own rows
+    tk, tv = rows(g, bsz, hkv, 3, dtype=HF), rows(g, bsz, hkv, 3, dtype=HF)
+    got = ops.kv8_sparse_attn(q.to(DEV), cache, idx=idx, tail_k=tk.to(DEV), tail_v=tv.to(DEV))
+    check_attention(got, q, [torch.cat([k[:, :n].flip(1), x.double()], 1) for k, n, x in zip(ks, closed, tk)],
+                    [torch.cat([v[:, :n].flip(1), x.double()], 1) for v, n, x in zip(vs, closed, tv)], 128 ** -0.5, HF)
+
+
 def test_a_shared_prompt_can_be_read_by_several_requests_and_not_written():
     g = torch.Generator().manual_seed(26)
     one, ks, vs = make(g, "e4m3", BF, 32, 0, [600], 2, open_rows=False)
