@@ -563,7 +563,7 @@ class KV8:
             raise ValueError("codes must be torch.float8_e4m3fn or torch.int8, K and V alike")
         if k.dim() != 4 or k.shape[-1] != 128 or k.stride(-1) != 1 or v.shape != k.shape or v.stride() != k.stride():
             raise ValueError("K and V codes must be 4-d with 128 contiguous elements last, same shape and strides")
-        if any(s % 16 for s in k.stride()[:3]):
+        if any(s % 16 and n > 1 for s, n in zip(k.stride()[:3], k.shape)):
             raise ValueError("code strides must be multiples of 16")
         if block not in (16, 32, 64, 128):
             raise ValueError("block must be 16, 32, 64 or 128 tokens")
@@ -595,7 +595,7 @@ class KV8:
         self.page_size = tokens if paged else 0
         self.capacity = page_table.shape[1] * tokens if paged else tokens  # tokens a request has room for
         self.dtype = open_k.dtype if open_k is not None else None
-        st, ss = k.stride(), k_scale.stride()
+        st, ss = [s if n > 1 or s % 16 == 0 else 0 for s, n in zip(k.stride(), k.shape)], k_scale.stride()
         self._c = {}
         for dt in (torch.bfloat16, torch.float16):
             if self.dtype not in (None, dt):
@@ -683,18 +683,27 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, t
     read by an index, or through a KV8 of the same tensors without open buffers.  A request whose rows would not
     fit is left as it was.  okv_kv8_append."""
     c = cache._struct(k.dtype)
-    if k.dim() != 4 or v.dim() != 4 or k.shape[0] != cache.bsz or k.shape[1] != cache.num_kv_heads or k.shape[3] != 128:
+    shape, dev = k.shape, cache.device
+    if len(shape) != 4:
         raise ValueError(f"new rows must be ({cache.bsz}, {cache.num_kv_heads}, n, 128)")
-    (kb, kg, kt, k1), (vb, vg, vt, v1) = k.stride(), v.stride()
-    if v.shape != k.shape or v.dtype is not k.dtype or k1 != 1 or v1 != 1:
+    b, h, n, d = shape
+    if b != cache.bsz or h != cache.num_kv_heads or d != 128:
+        raise ValueError(f"new rows must be ({cache.bsz}, {cache.num_kv_heads}, n, 128)")
+    if v.shape != shape or v.dtype is not k.dtype:
         raise ValueError("new K and V must share shape and dtype, with a contiguous last dimension")
-    if k.device != cache.device or v.device != cache.device:
+    (kb, kg, kt, k1), (vb, vg, vt, v1) = k.stride(), v.stride()
+    if k1 != 1 or v1 != 1:
+        raise ValueError("new K and V must share shape and dtype, with a contiguous last dimension")
+    if k.device != dev or v.device != dev:
         raise ValueError("new rows and cache must be on one GPU")
     if not cache._writable:
         raise ValueError("rows of this cache share memory: it can be read only")
-    n = k.shape[2]
     if n == 0:
         return
+    if b == 1:  # (whatever a view left as the stride of a single entry)
+        kb = vb = 0
+    if n == 1:
+        kt = vt = 0
     on_dev = isinstance(start, torch.Tensor)
     if not on_dev and not 0 <= start <= cache.capacity:
         raise ValueError(f"invalid start {start}: the cache has room for {cache.capacity} tokens")
@@ -800,6 +809,10 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
         (tb, th, rows, td), (tbs, ths, tts, unit) = shape, strides
         if tb != bsz or th != hkv or td != 128 or unit != 1:
             raise ValueError("tail_k / tail_v must be (bsz, Hkv, T, 128), same strides, contiguous last dimension")
+        if tb == 1:
+            tbs = 0
+        if rows == 1:
+            tts = 0
         dt = q.dtype
         if tail_k.dtype is not dt or tail_v.dtype is not dt or tail_k.device != dev or tail_v.device != dev:
             raise ValueError("tail and q differ in dtype or GPU")

@@ -558,6 +558,22 @@ def test_a_closed_short_block_is_read_without_the_open_buffers():
                     [held(y[0], "e4m3", 64, False)], 128 ** -0.5, BF)
 
 
+def test_single_entries_in_views_of_any_stride():
+    """One request, one row: the strides of these dimensions say nothing."""
+    g = torch.Generator().manual_seed(38)
+    odd = lambda x: x.to(DEV).as_strided(x.shape, (131, 128, 3, 1))  # x: (1, heads, 1, 128)
+    buf = torch.zeros(2 * 64 * 128, dtype=torch.uint8, device=DEV).view(torch.int8)
+    codes = [buf.clone().as_strided((1, 2, 64, 128), (7, 64 * 128, 128, 1)) for _ in "kv"]
+    s = torch.zeros((2, 1, 2, 4), device=DEV)
+    cache = ops.KV8(codes[0], codes[1], s[0], s[1], 16)
+    x, y, q = rows(g, 1, 2, 1), rows(g, 1, 2, 1), rows(g, 1, 8)
+    ops.kv8_append(cache, odd(x), odd(y), 0, close=True)
+    k, v = held(x[0], "int8", 16, False), held(y[0], "int8", 16, False)
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache, seq_len=1), q, [k], [v], 128 ** -0.5, BF)
+    out = ops.kv8_sparse_attn(q.to(DEV), cache, sel_len=1, tail_k=odd(y), tail_v=odd(x))
+    check_attention(out, q, [torch.cat([k, y[0].double()], 1)], [torch.cat([v, x[0].double()], 1)], 128 ** -0.5, BF)
+
+
 def test_scores_into_a_row_of_a_larger_tensor():
     """One request: the row's stride says nothing, whatever a view left there."""
     g = torch.Generator().manual_seed(36)
