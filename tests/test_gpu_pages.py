@@ -285,3 +285,48 @@ def test_growth_by_more_pages_than_a_plan_keeps(want):
         assert status.tolist() == m.extend(seqs, more) == [0, 0]
         assert sum(refs.tolist()) - before == want
         same(table, lt, refs, bufs, m)
+
+
+def test_pool_of_16_bit_pages_forks_grows_and_compacts():
+    """PagePool under ops.PagedKV: attention through the table after every step is that of each sequence's own rows."""
+    g = torch.Generator().manual_seed(11)
+    seqs, width, pages, page, hkv = 5, 8, 40, 16, 2
+    pool = PagePool(seqs, width, pages, page, DEV)
+    pk, pv = (torch.zeros((pages, page, hkv, 128), dtype=torch.bfloat16, device=DEV) for _ in "kv")
+    pool.add(pk, pv)
+    kv = ops.PagedKV(pk, pv, pool.table, page)
+    own = [[torch.zeros(hkv, 0, 128), torch.zeros(hkv, 0, 128)] for _ in range(seqs)]
+
+    def write(s, n):  # n more rows of sequence s, through the table
+        for t, mine in ((pk, 0), (pv, 1)):
+            x = torch.randn(hkv, n, 128, generator=g).to(torch.bfloat16)
+            at = torch.arange(own[s][mine].shape[1], own[s][mine].shape[1] + n, device=DEV)
+            t[pool.table[s, at // page].long(), at % page] = x.transpose(0, 1).to(DEV)
+            own[s][mine] = torch.cat([own[s][mine], x.float()], 1)
+
+    def check(live):
+        q = torch.randn(seqs, 2 * hkv, 128, generator=g).to(torch.bfloat16)
+        out = ops.dense_attn(q.to(DEV), kv, seq_len=width * page, seq_lens=pool.lens)
+        for s in live:
+            k, v = (x.double() for x in own[s])
+            assert int(pool.lens[s]) == k.shape[1]
+            p = torch.softmax(torch.einsum("hgd,hnd->hgn", q[s].double().view(hkv, 2, 128), k) * 128 ** -0.5, -1)
+            want = torch.einsum("hgn,hnd->hgd", p, v).reshape(2 * hkv, 128)
+            assert float((out[s].cpu().double() - want).abs().max()) < 2e-2  # (the bar of 16-bit attention in these tests)
+
+    pool.extend([0, 1], [37, 64])
+    write(0, 37), write(1, 64)
+    check([0, 1])
+    pool.fork([0, 0, 1], [2, 3, 4])
+    for c, p in ((2, 0), (3, 0), (4, 1)):
+        own[c] = [x.clone() for x in own[p]]
+    check(range(5))
+    pool.extend(list(range(5)), [3, 20, 5, 0, 17])
+    for s, n in enumerate([3, 20, 5, 0, 17]):
+        write(s, n)
+    check(range(5))
+    pool.free([1, 3])
+    pool.compact()
+    assert int(pool.used) == int((pool.refs > 0).sum()) and bool((pool.refs[int(pool.used):] == 0).all())
+    check([0, 2, 4])
+    assert pool.status() == (0, 0)
