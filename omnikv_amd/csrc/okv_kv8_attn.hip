@@ -268,7 +268,7 @@ struct Kv8Rows {
   int k[4], v[4], s;   // gather: index entries
 };
 
-// A workgroup per share and kv head (or pair of them), four waves that take 32-row tiles in turn.
+// A workgroup per share and kv head (or pair of them), W waves that take 32-row tiles in turn.
 //
 // Bound by the codes' bytes: every row is read once, in whole 128-byte lines, a tile in flight while the one before is
 // consumed.  One launch, eight kv heads: 450001 tokens of int8 (922 MB) 143 us = 6.4 TB/s, 131073 of e4m3 (269 MB) 44 us = 6.1,
