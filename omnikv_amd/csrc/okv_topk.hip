@@ -121,8 +121,9 @@ __global__ __launch_bounds__(kThreads) void topk_select(const float* __restrict_
   __shared__ TopkShared sh;
   const int b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = seq_lens ? seq_lens[b] : max_seq_len;
-  int k = k_per_seg ? k_per_seg[b] : max_k;
+  // what the device says is held to what the call made room for
+  const int n = seq_lens ? min(seq_lens[b], max_seq_len) : max_seq_len;
+  int k = k_per_seg ? min(k_per_seg[b], max_k) : max_k;
   if (k > n) k = n;
   if (k <= 0) return;
   const float* s = scores + (int64_t)b * score_stride;

@@ -193,11 +193,12 @@ __device__ __forceinline__ void wave_find_bin(const uint32_t* hist, uint32_t wan
   want_in = __shfl(fw, src);
 }
 
+// what the device says is held to what the call made room for
 __device__ __forceinline__ int req_len(const int32_t* seq_lens, int max_seq_len, int b) {
-  return seq_lens ? seq_lens[b] : max_seq_len;
+  return seq_lens ? min(seq_lens[b], max_seq_len) : max_seq_len;
 }
 __device__ __forceinline__ int req_k(const int32_t* k_per_seg, int max_k, int b, int n) {
-  int k = k_per_seg ? k_per_seg[b] : max_k;
+  const int k = k_per_seg ? min(k_per_seg[b], max_k) : max_k;
   return k < n ? k : n;
 }
 

@@ -95,6 +95,22 @@ def test_topk_ragged_batch():
         assert (out[b, kb:] == -7).all()  # untouched beyond k_b
 
 
+@pytest.mark.parametrize("n", [900, 20000])
+def test_topk_lengths_and_counts_beyond_the_call_count_as_its_bounds(n):
+    """Device lengths past the scores' rows and counts past the output's: as the bounds themselves; negative ones: none."""
+    g = torch.Generator().manual_seed(12)
+    k = 70
+    s = torch.randn((4, n + 64), generator=g)
+    s[:, n:] = 1e9  # behind the rows, larger than all of theirs
+    lens = torch.tensor([n + 50, (1 << 31) - 1, n, -3], dtype=torch.int32, device=DEV)
+    ks = torch.tensor([k, k + 9, (1 << 31) - 1, k], dtype=torch.int32, device=DEV)
+    out = torch.full((5, k + 20), -7, dtype=torch.int32, device=DEV)
+    ops.topk(s.to(DEV)[:, :n], k, seq_lens=lens, k_per_seg=ks, out=out[:4, :k])
+    want = orc.select_topk_stable(s[:3, :n], k).to(torch.int32)
+    assert torch.equal(out[:3, :k].cpu(), want)
+    assert bool((out[3:] == -7).all()) and bool((out[:, k:] == -7).all())
+
+
 # ---------------------------------------------------------------- scoring
 def _inputs(n, dtype, layout):
     q, k, v = synth.filter_layer_inputs(n)
