@@ -729,8 +729,8 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
                    idx_out: Optional[torch.Tensor] = None):
     """dense_attn over an 8-bit cache: q (bsz, Hq, 128) attends to the first seq_len rows (seq_lens: per request, on
     the GPU) -> (bsz, Hq, 128); with `selector` also the filter layer's scores of the first score_len rows, from the same
-    pass, and with `select_k` the ascending indices of the largest ones, as topk gives them.  A request
-    without rows gets zeros.  okv_kv8_dense_attn."""
+    pass, and with `select_k` the ascending indices of the largest ones, as topk gives them: of a request's own rows alone,
+    -1 (in idx_out: what was there) behind the last of them.  A request without rows gets zeros.  okv_kv8_dense_attn."""
     q, c = _kv8_query(q, cache)
     hq, dev, bsz = q.shape[1], cache.device, cache.bsz
     if seq_len is None:
@@ -763,7 +763,12 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
     if select_k is None:
         return out, scores
     with torch.cuda.device(dev):
-        return out, scores, topk(scores, select_k, score_lens, k_per_seg, out=idx_out)
+        # only a request's own rows have scores: its length bounds the ranking too (topk itself holds lengths to slen)
+        if seq_lens is None or score_lens is seq_lens:
+            ranked = score_lens
+        else:
+            ranked = seq_lens if score_lens is None else torch.minimum(seq_lens.view(-1), score_lens.view(-1))
+        return out, scores, topk(scores, select_k, ranked, k_per_seg, out=idx_out)
 
 
 def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = None, sel_len: Optional[int] = None,

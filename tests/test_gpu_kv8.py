@@ -246,6 +246,28 @@ def test_dense_select_equals_topk_of_its_scores():
     assert torch.equal(out, ops.kv8_dense_attn(q, cache, seq_lens=t, seq_len=900, selector="last")[0])
 
 
+@pytest.mark.parametrize("lens", [[900, 500, 30, 0], [20000, 150, 15000, 16384]])
+def test_dense_select_ranks_the_requests_own_rows_alone(lens):
+    """Ragged lengths without score_lens, with larger ones, and with smaller and larger ones: what a request has no rows
+    for is never selected, whatever the buffer of the scores held."""
+    g = torch.Generator().manual_seed(14)
+    cache, _, _ = make(g, "int8", BF, 16, 0, lens, 1)
+    q, n, k = rows(g, 4, 4).to(DEV), max(lens), 60
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for wanted in (None, t, t + 100, torch.tensor([n, 40, n, 40], dtype=torch.int32, device=DEV)):
+        buf = torch.full((4, n), 1e9, device=DEV)
+        out, scores, idx = ops.kv8_dense_attn(q, cache, seq_lens=t, seq_len=n, selector="last", score_len=n, score_lens=wanted,
+                                              scores_out=buf, select_k=k)
+        scored = t if wanted is None else torch.minimum(t, wanted)
+        assert idx.shape == (4, k) and bool((scores.cpu() == 1e9).sum(1).eq(n - scored.cpu()).all())
+        for b, m in enumerate(scored.tolist()):
+            want = torch.full((k,), -1, dtype=torch.int32)
+            if m:
+                top = torch.sort(scores[b, :m].cpu(), descending=True, stable=True)[1][:k].sort()[0]
+                want[: top.numel()] = top.to(torch.int32)
+            assert torch.equal(idx[b].cpu(), want), (b, m)
+
+
 SPARSE = [
     # fmt, dtype, block, page, hkv, group, lengths, selected rows, tails
     ("e4m3", BF, 64, 0, 2, 4, [300], [1], [0]),
