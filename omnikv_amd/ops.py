@@ -753,6 +753,11 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
         elif scores.shape != (bsz, slen) or scores.dtype != torch.float32 or scores.stride(1) != 1 or scores.device != dev:
             raise ValueError("scores_out must be (bsz, score_len) float32 with contiguous rows, on the cache's GPU")
         sp, ss, sl = scores.data_ptr(), scores.stride(0) if bsz > 1 else max(slen, scores.stride(0)), _dev_i32(score_lens, bsz, dev, "score_lens")
+    if select_k is not None and idx_out is not None:
+        kk = min(select_k, slen)
+        if (idx_out.shape != (bsz, kk) or idx_out.dtype != torch.int32 or idx_out.stride(1) != 1 or idx_out.device != dev
+                or (bsz > 1 and idx_out.stride(0) < kk)):
+            raise ValueError("idx_out must be (bsz, min(select_k, score_len)) int32 with contiguous rows, on the cache's GPU")
     nbytes = _kv8_workspace_bytes(cache, hq, seq_len, slen, False)
     ws = _scratch(dev, nbytes) if nbytes else None
     _launch(dev, lib().okv_kv8_dense_attn, q.data_ptr(), hq, c, _dev_i32(seq_lens, bsz, dev, "seq_lens"), seq_len, bsz,

@@ -158,3 +158,25 @@ def test_python_front_end_refuses_cpu_tensors_and_shapes():
         ops.PageBuffers([torch.zeros((4, 16))])
     with pytest.raises(ValueError, match="table"):
         ops.pages_free(torch.zeros((2, 4), dtype=torch.int32), torch.zeros(2), torch.zeros(4), torch.zeros(1), 16)
+
+
+def cpu_cache(bsz=2, hkv=2, cap=1024):
+    """A handle whose tensors are on the CPU: every check of a front end runs before anything is launched."""
+    c = ops.KV8.__new__(ops.KV8)
+    c.device, c.bsz, c.num_kv_heads, c.capacity, c.block, c.page_table = torch.device("cpu"), bsz, hkv, cap, 64, None
+    c._c = {torch.bfloat16: cache(num_kv_heads=hkv, capacity=cap)}
+    c._ref = {dt: C.byref(x) for dt, x in c._c.items()}
+    c._ws_bytes, c._writable = {}, True
+    return c
+
+
+def test_select_refuses_an_output_that_does_not_fit():
+    c, q = cpu_cache(), torch.zeros((2, 8, 128), dtype=torch.bfloat16)
+    good = torch.zeros((2, 20), dtype=torch.int32)
+    for out in (good.long(), good.float(), good[:1], good[:, :19], torch.zeros((2, 21), dtype=torch.int32), good[0],
+                torch.zeros((20, 2), dtype=torch.int32).t(), torch.zeros((2, 40), dtype=torch.int32)[:, ::2],
+                good[:1].expand(2, 20), torch.zeros((2, 20), dtype=torch.int32, device="meta")):
+        with pytest.raises(ValueError, match="idx_out"):
+            ops.kv8_dense_attn(q, c, seq_len=500, selector="last", score_len=400, select_k=20, idx_out=out)
+    with pytest.raises(ValueError, match="idx_out"):  # no more entries than there are scores
+        ops.kv8_dense_attn(q, c, seq_len=500, selector="last", score_len=10, select_k=20, idx_out=good)
