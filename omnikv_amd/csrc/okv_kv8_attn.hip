@@ -1065,19 +1065,25 @@ static int launch_kv8(Kv8Attn& a, int batch, hipStream_t stream) {
   return OKV_OK;
 }
 
+// What a plan is made for: without these bounds its divisions mean nothing (a group above 128 leaves a scored share no rows).
+static int check_sizes(int hq, int hkv, int64_t rows, int batch) {
+  OKV_REQUIRE(hq >= hkv && hq % hkv == 0, OKV_ERR_INVALID, "bad head counts q=%d kv=%d", hq, hkv);
+  OKV_REQUIRE(hq / hkv <= kMaxGroup, OKV_ERR_UNSUPPORTED, "GQA group size %d not supported (1 to %d)", hq / hkv, kMaxGroup);
+  OKV_REQUIRE(hq <= kMaxHeads, OKV_ERR_UNSUPPORTED, "%d q heads not supported (at most %d)", hq, kMaxHeads);
+  OKV_REQUIRE(batch <= 65535, OKV_ERR_UNSUPPORTED, "batch %d not supported", batch);
+  // (row numbers run past the last row by up to two steps of a workgroup, and stay in 32 bits)
+  OKV_REQUIRE(rows * batch <= (1ll << 31) - 65536, OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
+  return OKV_OK;
+}
+
 static int kv8_attend(Kv8Attn& a, int64_t rows, int batch, void* ws, size_t ws_bytes, hipStream_t stream) {
   const int hkv = a.c.num_kv_heads;
   OKV_REQUIRE(a.q && a.out, OKV_ERR_INVALID, "q or out is NULL");
   OKV_REQUIRE(((uintptr_t)a.q & 15) == 0, OKV_ERR_INVALID, "q must be 16-byte aligned");
-  OKV_REQUIRE(a.hq >= hkv && a.hq % hkv == 0, OKV_ERR_INVALID, "bad head counts q=%d kv=%d", a.hq, hkv);
+  if (int rc = check_sizes(a.hq, hkv, rows, batch)) return rc;
   a.group = a.hq / hkv;
   a.block_shift = __builtin_ctz(a.c.block_tokens);
   a.page_shift = a.c.page_table && (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz(a.c.page_size) : -1;
-  OKV_REQUIRE(a.group <= kMaxGroup, OKV_ERR_UNSUPPORTED, "GQA group size %d not supported (1 to %d)", a.group, kMaxGroup);
-  OKV_REQUIRE(a.hq <= kMaxHeads, OKV_ERR_UNSUPPORTED, "%d q heads not supported (at most %d)", a.hq, kMaxHeads);
-  OKV_REQUIRE(batch <= 65535, OKV_ERR_UNSUPPORTED, "batch %d not supported", batch);
-  // (row numbers run past the last row by up to two steps of a workgroup, and stay in 32 bits)
-  OKV_REQUIRE(rows * batch <= (1ll << 31) - 65536, OKV_ERR_UNSUPPORTED, "%lld rows not supported", (long long)rows * batch);
   const bool folded = a.max_score_len > 0 && a.normalise == OKV_NORM_RAW;
   if (folded) a.fold = a.head_reduce == OKV_REDUCE_MAX ? 1 : 2;
   const Kv8Plan p = kv8_plan(a.c, a.idx != nullptr, batch, a.group, rows, a.max_score_len, folded);
@@ -1102,6 +1108,7 @@ int okv_kv8_workspace_bytes(const okv_kv8_cache_t* cache, int32_t num_q_heads, i
   const int hkv = cache->num_kv_heads;
   OKV_REQUIRE(batch >= 1 && hkv >= 1 && num_q_heads >= hkv && max_rows >= 0 && max_score_len >= 0, OKV_ERR_INVALID,
               "bad batch, head counts or lengths");
+  if (int rc = check_sizes(num_q_heads, hkv, max_rows, batch)) return rc;
   const Kv8Plan p = kv8_plan(*cache, indexed != 0, batch, num_q_heads / hkv, max_rows, max_score_len, false);
   *out_bytes = kv8_workspace(p, batch, num_q_heads, hkv, max_score_len, false, nullptr, nullptr);
   return OKV_OK;

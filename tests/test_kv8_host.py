@@ -180,3 +180,31 @@ def test_select_refuses_an_output_that_does_not_fit():
             ops.kv8_dense_attn(q, c, seq_len=500, selector="last", score_len=400, select_k=20, idx_out=out)
     with pytest.raises(ValueError, match="idx_out"):  # no more entries than there are scores
         ops.kv8_dense_attn(q, c, seq_len=500, selector="last", score_len=10, select_k=20, idx_out=good)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("hkv, group, code", [(1, 9, UNSUPPORTED), (2, 72, UNSUPPORTED), (1, 129, UNSUPPORTED), (1, 256, UNSUPPORTED),
+                                              (8, 1000, UNSUPPORTED), (64, 8, UNSUPPORTED)])
+def test_scratch_of_unsupported_heads_is_refused_as_the_call_is(paged, hkv, group, code):
+    c = cache(num_kv_heads=hkv, token_stride=128 * hkv, head_stride=128)
+    if paged:
+        for k, v in dict(page_table=PTR, page_size=64, page_table_stride=16, num_pages=20, page_stride=64 * 128 * hkv).items():
+            setattr(c, k, v)
+    n = C.c_size_t(0)
+    for rows, score_len in ((1000, 500), (1000, 0), (100, 0)):
+        assert _lib.lib().okv_kv8_workspace_bytes(C.byref(c), hkv * group, 1, rows, score_len, 0, C.byref(n)) == code
+    assert dense(c, hq=hkv * group, n=1000, scores=PTR, score_len=500) == code
+
+
+def test_scratch_of_other_bad_sizes_is_refused():
+    size, c, n = _lib.lib().okv_kv8_workspace_bytes, cache(), C.c_size_t(0)
+    assert size(C.byref(c), 31, 1, 1000, 500, 0, C.byref(n)) == INVALID
+    assert size(C.byref(c), 32, 65536, 10, 0, 0, C.byref(n)) == UNSUPPORTED
+    assert size(C.byref(c), 32, 3, 1 << 30, 0, 0, C.byref(n)) == UNSUPPORTED
+    assert size(C.byref(c), 32, 1, (1 << 31) - 65536, 500, 0, C.byref(n)) == 0
+
+
+def test_selecting_with_unsupported_heads_raises():
+    c = cpu_cache(bsz=1, hkv=1)
+    with pytest.raises(Exception, match="GQA group size 200"):
+        ops.kv8_dense_attn(torch.zeros((1, 200, 128), dtype=torch.bfloat16), c, seq_len=1000, selector="last", select_k=5)
