@@ -438,7 +438,7 @@ int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, int64_t k_to
                    int32_t close, int32_t batch, okv_stream_t stream);
 
 /* Scratch of the two attention calls over `cache`: max_rows is max_seq_len, or max_sel_len + max_tail_len;
- * max_score_len 0 without scores; indexed 1 for a sparse call with an index.  0 bytes: ws may be NULL.  Head counts and sizes
+ * max_score_len 0 without scores; indexed 1 for a sparse call with an index (one of no entries may be NULL).  0 bytes: ws may be NULL.  Head counts and sizes
  * that the calls refuse are refused here. */
 int okv_kv8_workspace_bytes(const okv_kv8_cache_t* cache, int32_t num_q_heads, int32_t batch, int32_t max_rows,
                             int32_t max_score_len, int32_t indexed, size_t* out_bytes);

@@ -1109,8 +1109,13 @@ int okv_kv8_workspace_bytes(const okv_kv8_cache_t* cache, int32_t num_q_heads, i
   OKV_REQUIRE(batch >= 1 && hkv >= 1 && num_q_heads >= hkv && max_rows >= 0 && max_score_len >= 0, OKV_ERR_INVALID,
               "bad batch, head counts or lengths");
   if (int rc = check_sizes(num_q_heads, hkv, max_rows, batch)) return rc;
-  const Kv8Plan p = kv8_plan(*cache, indexed != 0, batch, num_q_heads / hkv, max_rows, max_score_len, false);
-  *out_bytes = kv8_workspace(p, batch, num_q_heads, hkv, max_score_len, false, nullptr, nullptr);
+  // an index without entries may come as NULL: a call planned as one without an index
+  size_t bytes = 0;
+  for (int gather = 0; gather <= (indexed != 0); ++gather) {
+    const Kv8Plan p = kv8_plan(*cache, gather != 0, batch, num_q_heads / hkv, max_rows, max_score_len, false);
+    bytes = std::max(bytes, kv8_workspace(p, batch, num_q_heads, hkv, max_score_len, false, nullptr, nullptr));
+  }
+  *out_bytes = bytes;
   return OKV_OK;
 }
 
@@ -1166,7 +1171,7 @@ int okv_kv8_sparse_attn(const void* q, int32_t num_q_heads, const okv_kv8_cache_
   else OKV_REQUIRE(max_sel_len <= kv8_room(*cache), OKV_ERR_INVALID, "max_sel_len %d exceeds the cache's %lld tokens",
                    max_sel_len, (long long)kv8_room(*cache));
   if (slots)
-    OKV_REQUIRE(idx && cache->page_table && cache->page_stride == cache->page_size * cache->token_stride &&
+    OKV_REQUIRE((idx || max_sel_len == 0) && cache->page_table && cache->page_stride == cache->page_size * cache->token_stride &&
                     cache->scale_page_stride == cache->page_size / cache->block_tokens * cache->scale_block_stride,
                 OKV_ERR_INVALID, "slots need an index and a pool whose pages lie back to back");
   if (max_tail_len > 0)

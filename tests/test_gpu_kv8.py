@@ -379,6 +379,24 @@ def test_sparse_without_an_index_and_with_a_tail_alone():
     check_attention(out, q, tk[:, :, :4].double(), tv[:, :, :4].double(), 128 ** -0.5, BF)
 
 
+@pytest.mark.parametrize("bsz", [1, 2, 5])
+@pytest.mark.parametrize("page", [0, 32])
+@pytest.mark.parametrize("tail", [1, 600, 2500])
+def test_an_empty_selection_leaves_the_tail(bsz, page, tail):
+    """An index without entries, contiguous, paged and by slots: the same as no selected rows at all."""
+    g = torch.Generator().manual_seed(28)
+    cache, _, _ = make(g, "int8", BF, 16, page, [80] * bsz, 2, open_rows=False)
+    q, tk, tv = rows(g, bsz, 8), rows(g, bsz, 2, tail), rows(g, bsz, 2, tail)
+    none = torch.empty((bsz, 0), dtype=torch.int32, device=DEV)
+    kw = dict(tail_k=tk.to(DEV), tail_v=tv.to(DEV))
+    for how in [dict(idx=none)] + ([dict(slots=none), dict(slots=cache.slot_index(none))] if page else []):
+        check_attention(ops.kv8_sparse_attn(q.to(DEV), cache, **how, **kw), q, tk.double(), tv.double(), 128 ** -0.5, BF)
+    some = torch.full((bsz, 4), 3, dtype=torch.int32, device=DEV)
+    check_attention(ops.kv8_sparse_attn(q.to(DEV), cache, idx=some, sel_len=0, **kw), q, tk.double(), tv.double(), 128 ** -0.5, BF)
+    with pytest.raises(Exception, match="no rows"):
+        ops.kv8_sparse_attn(q.to(DEV), cache, idx=none)
+
+
 def test_pages_outside_the_pool_take_no_part():
     g = torch.Generator().manual_seed(23)
     cache, ks, vs = make(g, "e4m3", BF, 16, 32, [200, 90], 2)

@@ -208,3 +208,17 @@ def test_selecting_with_unsupported_heads_raises():
     c = cpu_cache(bsz=1, hkv=1)
     with pytest.raises(Exception, match="GQA group size 200"):
         ops.kv8_dense_attn(torch.zeros((1, 200, 128), dtype=torch.bfloat16), c, seq_len=1000, selector="last", select_k=5)
+
+
+def test_scratch_of_an_indexed_call_is_enough_for_an_empty_index():
+    """An array without entries has no address: such a call runs as one without an index."""
+    n, size = [C.c_size_t(0), C.c_size_t(0)], _lib.lib().okv_kv8_workspace_bytes
+    for hkv in (1, 2, 8):
+        for page in (0, 64):
+            c = cache(num_kv_heads=hkv, token_stride=128 * hkv, head_stride=128, page_table=PTR if page else None, page_size=page,
+                      page_table_stride=16, num_pages=20, page_stride=64 * 128 * hkv)
+            for batch in (1, 2, 3, 17):
+                for rows in (1, 512, 600, 1400, 2049, 30000):
+                    for indexed in (0, 1):
+                        assert size(C.byref(c), 4 * hkv, batch, rows, 0, indexed, C.byref(n[indexed])) == 0
+                    assert n[1].value >= n[0].value, (hkv, page, batch, rows)
