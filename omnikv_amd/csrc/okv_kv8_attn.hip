@@ -207,6 +207,20 @@ __device__ __forceinline__ f32x4_t mfma16k16(uint32_t a0, uint32_t a1, uint32_t 
                                                    __builtin_bit_cast(s16x4_t, make_uint2(b0, b1)), c, 0, 0, 0);
 }
 
+// Four 16-bit elements of V as the B operand next to probabilities in bf16: bfloat16's as they are, float16's in two parts,
+// the nearest bf16 and the rest, exact together (11 bits = 8 + 3; bf16 has the range).  (Probabilities in float16, whose
+// smallest step is 2^-24, lose what is below 2^-25 of the largest.)
+template <typename T> constexpr bool kTwoParts = false;
+template <> constexpr bool kTwoParts<F16> = true;
+__device__ __forceinline__ uint4 bf16_rows(const BF16*, uint32_t a, uint32_t b) { return make_uint4(a, b, 0, 0); }
+__device__ __forceinline__ uint4 bf16_rows(const F16* f, uint32_t a, uint32_t b) {
+  const BF16* bf = nullptr;
+  const f32x2_t va = unpack_pair(f, a), vb = unpack_pair(f, b);
+  const uint32_t ha = pack_pair(bf, va.x, va.y), hb = pack_pair(bf, vb.x, vb.y);
+  const f32x2_t ua = unpack_pair(bf, ha), ub = unpack_pair(bf, hb);
+  return make_uint4(ha, hb, pack_pair(bf, va.x - ua.x, va.y - ua.y), pack_pair(bf, vb.x - ub.x, vb.y - ub.y));
+}
+
 // lanes 8..15 (MASK 0xC) or 0..7 (MASK 0x3) of every 16-lane row take `from` of the lane eight away, the others keep `own`
 template <int MASK>
 __device__ __forceinline__ uint32_t take8(uint32_t own, uint32_t from) {
@@ -493,8 +507,9 @@ __global__ __launch_bounds__(64 * W, MODE == kGather && W == 4 ? kGatherResident
     if (m16 < (a.fold ? 1 : G))
       *reinterpret_cast<float4*>(slog + (n * (a.fold ? 1 : G) + m16) * sh.rows + (row - begin)) = make_float4(o[0], o[1], o[2], o[3]);
   };
-  // a probability in two 16-bit parts: this lane's part of four of them
-  auto split_p = [&](auto* ty, const float (&p)[4], uint32_t* out) {
+  // a probability in two bf16 parts: this lane's part of four of them
+  auto split_p = [&](const float (&p)[4], uint32_t* out) {
+    const BF16* ty = nullptr;
     const uint32_t h0 = pack_pair(ty, p[0], p[1]), h1 = pack_pair(ty, p[2], p[3]);
     const f32x2_t u0 = unpack_pair(ty, h0), u1 = unpack_pair(ty, h1);
     out[0] = hi8 ? pack_pair(ty, p[0] - u0.x, p[1] - u0.y) : h0;
@@ -608,7 +623,7 @@ __global__ __launch_bounds__(64 * W, MODE == kGather && W == 4 ? kGatherResident
         l[n] += e;
         w[i] = e * vs[s][i];
       }
-      split_p((const BF16*)nullptr, w, pa + 2 * s);
+      split_p(w, pa + 2 * s);
     }
     const uint4 pf = make_uint4(pa[0], pa[1], pa[2], pa[3]);
     // lane m keeps eight elements of its lane row's four rows of either sixteen
@@ -696,6 +711,7 @@ __global__ __launch_bounds__(64 * W, MODE == kGather && W == 4 ? kGatherResident
     const int64_t lts = a.late_token_stride;
     const int64_t lbase = (int64_t)b * a.late_batch_stride + (int64_t)g * a.late_head_stride;
     const T* ty = nullptr;
+    const BF16* bf = nullptr;
     for (int t = lo + 16 * wave; t < end; t += 16 * W) {
       const int top_row = end - 1 - closed;  // rows counted from the first late one
 #pragma unroll
@@ -729,16 +745,19 @@ __global__ __launch_bounds__(64 * W, MODE == kGather && W == 4 ? kGatherResident
         l[n] += p[i];
       }
       uint32_t pa[2];
-      split_p(ty, p, pa);
-      const uint4 pf = make_uint4(pa[0], pa[1], 0, 0);  // the upper four of the contraction's eight rows: none
+      split_p(p, pa);
+      // the contraction's upper four rows are the same ones again, with what bf16 leaves of float16's V (bf16's: nothing)
+      const uint4 pf = kTwoParts<T> ? make_uint4(pa[0], pa[1], pa[0], pa[1]) : make_uint4(pa[0], pa[1], 0, 0);
       const uint32_t r0[4] = {vf[0].x, vf[0].y, vf[0].z, vf[0].w}, r1[4] = {vf[1].x, vf[1].y, vf[1].z, vf[1].w};
       const uint32_t r2[4] = {vf[2].x, vf[2].y, vf[2].z, vf[2].w}, r3[4] = {vf[3].x, vf[3].y, vf[3].z, vf[3].w};
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        acc[n][2 * d] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x05040100u),
-                                               __builtin_amdgcn_perm(r3[d], r2[d], 0x05040100u), 0, 0), acc[n][2 * d]);
-        acc[n][2 * d + 1] = mfma16(ty, pf, make_uint4(__builtin_amdgcn_perm(r1[d], r0[d], 0x07060302u),
-                                                   __builtin_amdgcn_perm(r3[d], r2[d], 0x07060302u), 0, 0), acc[n][2 * d + 1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t sel = h ? 0x07060302u : 0x05040100u;
+          const uint4 e = bf16_rows(ty, __builtin_amdgcn_perm(r1[d], r0[d], sel), __builtin_amdgcn_perm(r3[d], r2[d], sel));
+          acc[n][2 * d + h] = mfma16(bf, pf, e, acc[n][2 * d + h]);
+        }
       }
       }
     }

@@ -653,3 +653,28 @@ def test_front_end_refusals():
                 lambda: ops.kv8_append(cache, q[:, :2, None], q[:, :2, None], 5, close=True)):
         with pytest.raises(Exception, match="invalid"):
             bad()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("top", [12.0, 18.0, 24.0])
+def test_small_probabilities_of_16_bit_rows_keep_their_bits(dtype, top):
+    """An 8-bit block takes almost all the weight and has V = 0: what is left of the output are the 16-bit rows, with
+    probabilities around exp(-top), down to 2^-37: below half the smallest float16."""
+    g = torch.Generator().manual_seed(39)
+    k, v = torch.zeros(1, 1, 31, 128), torch.rand(1, 1, 31, 128, generator=g) * 4e4
+    k[:, :, :16] = top * 128 ** -0.5
+    v[:, :, :16] = 0
+    k[:, :, 16:] = torch.randn(1, 1, 15, 128, generator=g) * 0.05
+    k, v = k.to(dtype), v.to(dtype)
+    cache = ops.KV8.empty(1, 1, 64, "int8", 16, dtype, DEV)
+    ops.kv8_append(cache, k.to(DEV), v.to(DEV), 0)
+    q = (1 + 0.1 * torch.randn(1, 4, 128, generator=g)).to(dtype)
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache, seq_len=31), q, [held(k[0], "int8", 16, True)],
+                    [held(v[0], "int8", 16, True)], 128 ** -0.5, dtype)
+    closed = [held(x[0, :, :16], "int8", 16, True) for x in (k, v)]
+    tk = (torch.randn(1, 1, 700, 128, generator=g) * 0.05).to(dtype)
+    tv = (torch.rand(1, 1, 700, 128, generator=g) * 4e4).to(dtype)
+    idx = torch.arange(16, dtype=torch.int32, device=DEV)[None]
+    out = ops.kv8_sparse_attn(q.to(DEV), cache, idx=idx, tail_k=tk.to(DEV), tail_v=tv.to(DEV))
+    check_attention(out, q, [torch.cat([closed[0], tk[0].double()], 1)], [torch.cat([closed[1], tv[0].double()], 1)],
+                    128 ** -0.5, dtype)
