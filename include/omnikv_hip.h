@@ -488,7 +488,7 @@ int okv_kv8_read(const okv_kv8_cache_t* cache, const int32_t* idx, int64_t idx_s
  * `buffers`: for every layer's K, V and scales one array of num_pages pages, page p at base +
  * p*page_bytes (base and page_bytes multiples of 4; of 16 for speed), listed in HOST memory.  Pages
  * are handed out lowest first, in the order of the call's entries, so results are reproducible.  Fork and extend
- * take at most 1024 entries in one call.
+ * take at most 1024 entries in one call; sequences, pages and entries are at most 2^30 each.
  *
  * status (device int32[2], may be NULL): [0] pages the pool was short of -- then the call changed
  * nothing --, [1] entries that were refused and skipped.  Entries refused: sequence numbers

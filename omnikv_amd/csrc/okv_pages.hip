@@ -17,6 +17,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kMaxEntries = kPlanThreads;  // entries of a call: one per thread of the plan
 constexpr int kPerThread = 4;              // pages of a plan's trip through the counts, per thread
 constexpr int kTrip = kPlanThreads * kPerThread;
+constexpr int kMost = 1 << 30;  // pages, sequences, pages of a sequence, entries: what is counted runs a step past the last, in 32 bits
 
 struct BufferList {
   okv_page_buffer_t b[kBuffersPerLaunch];
@@ -419,6 +420,8 @@ static int check_pool(const okv_page_pool_t* p, const char* what, bool lens) {
               "%s: num_seqs %d, max_pages %d, num_pages %d, page_size %d", what, p->num_seqs, p->max_pages, p->num_pages,
               p->page_size);
   OKV_REQUIRE(p->table_stride >= p->max_pages, OKV_ERR_INVALID, "%s: table_stride < max_pages", what);
+  OKV_REQUIRE(p->num_seqs <= kMost && p->max_pages <= kMost && p->num_pages <= kMost, OKV_ERR_UNSUPPORTED,
+              "%s: num_seqs %d, max_pages %d, num_pages %d (at most 2^30 each)", what, p->num_seqs, p->max_pages, p->num_pages);
   return OKV_OK;
 }
 static int check_buffers(const okv_page_buffer_t* b, int n, const char* what) {
@@ -450,6 +453,8 @@ extern "C" {
 int okv_pages_workspace_bytes(const okv_page_pool_t* pool, int32_t n, size_t* out_bytes) {
   OKV_REQUIRE(pool != nullptr && out_bytes != nullptr && n >= 0 && pool->num_seqs >= 1 && pool->num_pages >= 1, OKV_ERR_INVALID,
               "bad argument");
+  OKV_REQUIRE(pool->num_seqs <= kMost && pool->num_pages <= kMost && n <= kMost, OKV_ERR_UNSUPPORTED,
+              "okv_pages_workspace_bytes: %d sequences, %d pages, %d entries (at most 2^30 each)", pool->num_seqs, pool->num_pages, n);
   *out_bytes = pages_ws_bytes(pool, n);
   return OKV_OK;
 }
@@ -458,6 +463,7 @@ int okv_pages_free(const okv_page_pool_t* pool, const int32_t* seqs, int32_t n, 
   int rc = check_pool(pool, "okv_pages_free", true);
   if (rc) return rc;
   OKV_REQUIRE(n >= 1 && seqs, OKV_ERR_INVALID, "okv_pages_free: n >= 1 entries");
+  OKV_REQUIRE(n <= kMost, OKV_ERR_UNSUPPORTED, "okv_pages_free: %d entries in one call (at most 2^30)", n);
   hipLaunchKernelGGL(pages_free_kernel, dim3(n), dim3(256), 0, (hipStream_t)stream, *pool, seqs, n, status);
   OKV_HIP_CHECK(hipGetLastError());
   return OKV_OK;
@@ -504,6 +510,8 @@ int okv_pages_copy(const okv_page_buffer_t* host_buffers, int32_t num_buffers, i
   int rc = check_buffers(host_buffers, num_buffers, "okv_pages_copy");
   if (rc) return rc;
   OKV_REQUIRE(n >= 0 && num_pages >= 1 && (n == 0 || (src && dst)), OKV_ERR_INVALID, "okv_pages_copy: bad lists");
+  OKV_REQUIRE(n <= kMost && num_pages <= kMost, OKV_ERR_UNSUPPORTED, "okv_pages_copy: %d entries, %d pages (at most 2^30 each)", n,
+              num_pages);
   if (n == 0) return OKV_OK;
   for (int lo = 0; lo < num_buffers; lo += kBuffersPerLaunch) {
     const int m = num_buffers - lo < kBuffersPerLaunch ? num_buffers - lo : kBuffersPerLaunch;

@@ -866,6 +866,9 @@ def kv8_read(cache: KV8, dtype: torch.dtype, idx: Optional[torch.Tensor] = None,
 
 
 # ---------------------------------------------------------------- pages of a cache
+_MOST = 1 << 30  # pages, sequences, entries of a call (a larger number would be cut to 32 bits on its way)
+
+
 class PageBuffers:
     """The arrays whose pages move together (every layer's K, V and scales): contiguous tensors
     (num_pages, ...) on one GPU, their page a multiple of 4 bytes.  Listed once, used by every call."""
@@ -875,6 +878,8 @@ class PageBuffers:
         if not self.tensors:
             raise ValueError("no buffers")
         self.device, self.num_pages = self.tensors[0].device, self.tensors[0].shape[0]
+        if self.num_pages > _MOST:
+            raise ValueError("more than 2^30 pages")
         self._c = (_lib.PageBuffer * len(self.tensors))()
         for t, b in zip(self.tensors, self._c):
             if not t.is_cuda or t.device != self.device or not t.is_contiguous() or t.shape[0] != self.num_pages:
@@ -892,6 +897,8 @@ def _buffers(buffers) -> PageBuffers:
 def _page_pool(table, lens, refs, page_size):
     rows, width = table.shape
     stride, unit = table.stride()
+    if max(rows, width, refs.numel()) > _MOST:
+        raise ValueError("more than 2^30 sequences or pages")
     if table.dtype is not torch.int32 or unit != 1 or not table.is_cuda:
         raise ValueError("table must be a (num_seqs, max_pages) int32 GPU tensor with contiguous rows")
     if stride < width:
@@ -904,8 +911,8 @@ def _page_pool(table, lens, refs, page_size):
 
 
 def _entries(t, n, device, name):
-    if t.dim() != 1 or n < 1:
-        raise ValueError(f"{name} must be a list of at least one entry")
+    if t.dim() != 1 or not 1 <= n <= _MOST:
+        raise ValueError(f"{name} must be a list of at least one entry (and at most 2^30)")
     return _dev_i32(t, n, device, name)
 
 

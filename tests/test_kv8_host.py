@@ -222,3 +222,29 @@ def test_scratch_of_an_indexed_call_is_enough_for_an_empty_index():
                     for indexed in (0, 1):
                         assert size(C.byref(c), 4 * hkv, batch, rows, 0, indexed, C.byref(n[indexed])) == 0
                     assert n[1].value >= n[0].value, (hkv, page, batch, rows)
+
+
+def test_pools_and_lists_beyond_what_the_plans_count_are_refused():
+    """Page, sequence and entry numbers run past the last one by a step of a workgroup, and stay in 32 bits."""
+    l, most = _lib.lib(), (1 << 31) - 1
+    buf = (_lib.PageBuffer * 1)(_lib.PageBuffer(PTR, 4096))
+    big, n = 1 << 50, C.c_size_t(0)
+    for field in ("num_pages", "max_pages", "num_seqs"):
+        pool = _lib.PagePool(PTR, PTR, PTR, 1 << 32, 4, 8, 100, 16)
+        setattr(pool, field, most)
+        assert l.okv_pages_free(C.byref(pool), PTR, 1, None, None) == UNSUPPORTED
+        assert l.okv_pages_fork(C.byref(pool), PTR, PTR, 1, buf, 1, None, 0, None, PTR, big, None) == UNSUPPORTED
+        assert l.okv_pages_extend(C.byref(pool), PTR, PTR, 1, None, None) == UNSUPPORTED
+        assert l.okv_pages_compact(C.byref(pool), PTR, 1 << 32, PTR, None, buf, 1, PTR, big, None) == UNSUPPORTED
+        if field != "max_pages":
+            assert l.okv_pages_workspace_bytes(C.byref(pool), 3, C.byref(n)) == UNSUPPORTED
+    ok = _lib.PagePool(PTR, PTR, PTR, 8, 4, 8, 100, 16)
+    assert l.okv_pages_workspace_bytes(C.byref(ok), most, C.byref(n)) == UNSUPPORTED
+    assert l.okv_pages_free(C.byref(ok), PTR, most, None, None) == UNSUPPORTED
+    assert l.okv_pages_copy(buf, 1, 100, PTR, PTR, None, most, None) == UNSUPPORTED
+    assert l.okv_pages_copy(buf, 1, most, PTR, PTR, None, 3, None) == UNSUPPORTED
+    meta = lambda *shape: torch.empty(shape, dtype=torch.int32, device="meta")  # noqa: E731
+    with pytest.raises(ValueError, match="2\\^30"):  # (2^32 + 5 would arrive as 5)
+        ops.pages_free(meta(4, 8), meta(4), meta((1 << 32) + 5), meta(1), 16)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.PageBuffers([meta((1 << 32) + 5, 4)])
