@@ -586,7 +586,7 @@ class KV8:
         if open_k is not None:
             if (tuple(open_k.shape) != (self.bsz, hkv, block, 128) or open_k.dtype not in (torch.bfloat16, torch.float16)
                     or open_v.shape != open_k.shape or open_v.dtype != open_k.dtype or open_v.stride() != open_k.stride()
-                    or open_k.stride(-1) != 1 or any(s % 8 for s in open_k.stride()[:3])):
+                    or open_k.stride(-1) != 1 or any(s % 8 and n > 1 for s, n in zip(open_k.stride()[:3], open_k.shape))):
                 raise ValueError(f"open_k / open_v must be ({self.bsz}, {hkv}, {block}, 128) in bfloat16 or float16, "
                                  "same strides (multiples of 8), contiguous last dimension")
         self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
@@ -614,7 +614,8 @@ class KV8:
                 c.scale_batch_stride, c.scale_head_stride, c.scale_block_stride = ss
             if open_k is not None:
                 c.open_k, c.open_v = open_k.data_ptr(), open_v.data_ptr()
-                c.open_batch_stride, c.open_head_stride, c.open_token_stride = open_k.stride()[:3]
+                c.open_batch_stride, c.open_head_stride, c.open_token_stride = [
+                    s if n > 1 else 0 for s, n in zip(open_k.stride()[:3], open_k.shape)]
             self._c[dt] = c
         self._ref = {dt: C.byref(c) for dt, c in self._c.items()}
         self._ws_bytes = {}  # scratch of a call, by its sizes
@@ -702,6 +703,8 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, t
         return
     if b == 1:  # (whatever a view left as the stride of a single entry)
         kb = vb = 0
+    if h == 1:
+        kg = vg = 0
     if n == 1:
         kt = vt = 0
     on_dev = isinstance(start, torch.Tensor)
@@ -821,6 +824,8 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
             raise ValueError("tail_k / tail_v must be (bsz, Hkv, T, 128), same strides, contiguous last dimension")
         if tb == 1:
             tbs = 0
+        if th == 1:
+            ths = 0
         if rows == 1:
             tts = 0
         dt = q.dtype

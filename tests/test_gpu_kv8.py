@@ -614,6 +614,22 @@ def test_single_entries_in_views_of_any_stride():
     check_attention(out, q, [torch.cat([k, y[0].double()], 1)], [torch.cat([v, x[0].double()], 1)], 128 ** -0.5, BF)
 
 
+def test_a_single_kv_head_in_views_of_any_stride():
+    """One kv head, in the new rows, the tail and the open buffers: the stride between heads says nothing."""
+    g = torch.Generator().manual_seed(40)
+    n, odd = 37, lambda x: x.to(DEV).as_strided(x.shape, (x.shape[2] * 128, 5, 128, 1))  # noqa: E731  x: (b, 1, n, 128)
+    x, y, q, tk, tv = rows(g, 2, 1, n), rows(g, 2, 1, n), rows(g, 2, 4), rows(g, 2, 1, 9), rows(g, 2, 1, 9)
+    whole = ops.KV8.empty(2, 1, 64, "int8", 16, BF, DEV)
+    cache = ops.KV8(whole.k, whole.v, whole.k_scale, whole.v_scale, 16, odd(whole.open_k), odd(whole.open_v))
+    ops.kv8_append(cache, odd(x), odd(y), 0)
+    ks, vs = [held(r, "int8", 16, True) for r in x], [held(r, "int8", 16, True) for r in y]
+    check_attention(ops.kv8_dense_attn(q.to(DEV), cache, seq_len=n), q, ks, vs, 128 ** -0.5, BF)
+    idx = torch.arange(32, dtype=torch.int32, device=DEV).expand(2, -1).contiguous()
+    out = ops.kv8_sparse_attn(q.to(DEV), cache, idx=idx, tail_k=odd(tk), tail_v=odd(tv))
+    check_attention(out, q, [torch.cat([k[:, :32], t.double()], 1) for k, t in zip(ks, tk)],
+                    [torch.cat([v[:, :32], t.double()], 1) for v, t in zip(vs, tv)], 128 ** -0.5, BF)
+
+
 def test_scores_into_a_row_of_a_larger_tensor():
     """One request: the row's stride says nothing, whatever a view left there."""
     g = torch.Generator().manual_seed(36)
