@@ -330,3 +330,38 @@ def test_pool_of_16_bit_pages_forks_grows_and_compacts():
     assert int(pool.used) == int((pool.refs > 0).sum()) and bool((pool.refs[int(pool.used):] == 0).all())
     check([0, 2, 4])
     assert pool.status() == (0, 0)
+
+
+def test_a_step_that_the_pool_refuses_leaves_the_caches_as_they_were():
+    """Appending what extend granted (the difference of the lengths), not what was asked for: a pool that is short, and an
+    entry that is refused, change neither codes nor open rows; the next step that fits goes on as if nothing had been asked."""
+    import test_gpu_kv8 as kv8
+
+    g = torch.Generator().manual_seed(12)
+    seqs, page, hkv, block, bf = 3, 32, 2, 16, torch.bfloat16
+    pool = PagePool(seqs, 4, 7, page, DEV)
+    cache = ops.KV8.empty_paged(pool.table, 7, page, hkv, "int8", block, bf)
+    pool.add_cache(cache)
+    own = [[torch.zeros(hkv, 0, 128, dtype=bf)] * 2 for _ in range(seqs)]
+
+    def step(more, granted):
+        starts = pool.lens.clone()
+        pool.extend(list(range(seqs)), more)
+        x, y = (kv8.rows(g, seqs, hkv, max(more)) for _ in "kv")
+        ops.kv8_append(cache, x.to(DEV), y.to(DEV), starts, pool.lens - starts)
+        for s, n in enumerate(granted):
+            own[s] = [torch.cat([a, t[s, :, :n]], 1) for a, t in zip(own[s], (x, y))]
+        q = kv8.rows(g, seqs, 4 * hkv)
+        out = ops.kv8_dense_attn(q.to(DEV), cache, seq_lens=pool.lens)
+        kv8.check_attention(out, q, *([kv8.held(own[s][i], "int8", block, True) for s in range(seqs)] for i in (0, 1)), 128 ** -0.5, bf)
+
+    step([45, 70, 20], [45, 70, 20])  # 2 + 3 + 1 of 7 pages
+    state = [t.clone() for t in (cache.k.view(torch.uint8), cache.k_scale, cache.open_k, cache.open_v, pool.table, pool.lens)]
+    step([30, 35, 10], [0, 0, 0])  # two more wanted, one left
+    for t, was in zip((cache.k.view(torch.uint8), cache.k_scale, cache.open_k, cache.open_v, pool.table, pool.lens), state):
+        assert torch.equal(t, was)
+    assert pool.status() == (1, 0)
+    step([100, 5, 3], [0, 5, 3])  # five pages for a sequence of at most four: that entry alone is refused
+    assert pool.status() == (0, 1)
+    step([19, 0, 30], [19, 0, 30])
+    assert pool.status() == (0, 0)
