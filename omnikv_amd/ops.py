@@ -786,7 +786,8 @@ def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = N
                     slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """sparse_attn over an 8-bit cache: rows idx (bsz, k) int32 of the codes (None: rows [0, sel_len)) followed by
     16-bit tail rows (bsz, Hkv, T, 128) in q's dtype; slots: KV8.slot_index(idx) instead of idx.  Entries outside the
-    request's room (padding, -1) take no part; open rows are not reached.  okv_kv8_sparse_attn."""
+    request's room (padding, -1) take no part.  They name rows that are codes: the place of an open row holds whatever was there before
+    (open_k / open_v themselves can be the tail).  okv_kv8_sparse_attn."""
     q, c = _kv8_query(q, cache)
     hq, hkv, dev, bsz = q.shape[1], cache.num_kv_heads, cache.device, cache.bsz
     if slots is not None:

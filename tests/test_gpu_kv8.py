@@ -694,3 +694,27 @@ def test_small_probabilities_of_16_bit_rows_keep_their_bits(dtype, top):
     out = ops.kv8_sparse_attn(q.to(DEV), cache, idx=idx, tail_k=tk.to(DEV), tail_v=tv.to(DEV))
     check_attention(out, q, [torch.cat([closed[0], tk[0].double()], 1)], [torch.cat([closed[1], tv[0].double()], 1)],
                     128 ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("page", [0, 32])
+def test_a_selection_and_the_open_rows_as_its_tail(page):
+    """A filter layer scores the rows that are codes, a sparse layer reads those it selects and its own open rows as the
+    tail: with every code selected, attention over the whole request."""
+    g = torch.Generator().manual_seed(41)
+    lens, hkv, block = [333, 31, 160, 7], 2, 16
+    (one, k1, v1), (two, k2, v2) = (make(g, "e4m3", BF, block, page, lens, hkv) for _ in range(2))
+    for codes in (one.k, one.v, two.k, two.v) if not page else ():
+        for b, n in enumerate(lens):  # behind the last full block: whatever was there before
+            codes.view(torch.uint8)[b, :, n // block * block:].fill_(0x66)
+    q, q2 = rows(g, 4, 8), rows(g, 4, 8)
+    t = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    closed = t // block * block
+    for k in (333, 20):
+        out, scores, idx = ops.kv8_dense_attn(q.to(DEV), one, seq_lens=t, seq_len=333, selector="last", score_len=333,
+                                              score_lens=closed, select_k=k)
+        check_attention(out, q, k1, v1, 128 ** -0.5, BF)
+        how = dict(slots=two.slot_index(idx)) if page else dict(idx=idx)
+        got = ops.kv8_sparse_attn(q2.to(DEV), two, tail_k=two.open_k, tail_v=two.open_v, tail_lens=t - closed, **how)
+        at = [torch.cat([i[i >= 0].long().cpu(), torch.arange(n // block * block, n)]) for i, n in zip(idx, lens)]
+        assert all(a.numel() == min(k, n // block * block) + n % block for a, n in zip(at, lens))
+        check_attention(got, q2, [x[:, a] for x, a in zip(k2, at)], [x[:, a] for x, a in zip(v2, at)], 128 ** -0.5, BF)
