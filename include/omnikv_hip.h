@@ -444,8 +444,8 @@ int okv_kv8_workspace_bytes(const okv_kv8_cache_t* cache, int32_t num_q_heads, i
                             int32_t max_score_len, int32_t indexed, size_t* out_bytes);
 
 /*
- * okv_dense_attn over an 8-bit cache: the rows [0, seq_len) of each request, those behind the last
- * full block from its open buffer, with optional filter-layer scores of the first score_len rows
+ * okv_dense_attn over an 8-bit cache: the rows [0, seq_len) of each request, seq_len the length it has, those behind
+ * that length's last full block from its open buffer, with optional filter-layer scores of the first score_len rows
  * (as okv_score defines them).  num_q_heads is num_kv_heads times a group of 1 to 8.  Lengths read
  * from the device count as clamped to [0, max_seq_len] and [0, min(max_score_len, seq_len)]; a request without rows gets
  * zeros.

@@ -305,7 +305,7 @@ struct Kv8Rows {
 // NH 2 (paged, an even number of kv heads, a token's heads next to each other): a wave takes sixteen rows of two neighbouring
 // heads instead of 32 rows of one; what is said of the upper sixteen rows then holds for the second head.
 // 128-byte pieces a token's row apart reach memory less well than 256-byte ones: 288000 tokens of one request
-// 122.3 -> 113.2 us, sixteen of 18000 each 121.1 -> 117.6; one descriptor for both heads, scales read by plain loads 119.5 -> 117.9
+// 122.3 -> 113.2 us, sixteen of 18000 each 121.1 -> 117.6; one descriptor for both heads 119.5 -> 117.9
 // (sixteen of 8K..32K).  Through an index it made no difference (22.1, 22.6).
 template <typename T, typename F, int MODE, bool LOGITS, int NH, bool DIRECT, int W>
 __global__ __launch_bounds__(64 * W, MODE == kGather && W == 4 ? kGatherResident : 2) void kv8_split(Kv8Attn a) {
@@ -784,7 +784,7 @@ __global__ __launch_bounds__(64 * W, MODE == kGather && W == 4 ? kGatherResident
     __syncthreads();
   }
 
-  // ---- the four waves meet
+  // ---- the W waves meet
   constexpr int kCell = NH * kMaxGroup;
   float* sm = lds;                  // [W][NH][8] running maximum
   float* sl = lds + W * kCell;      // [W][NH][8] sum of exponentials

@@ -677,7 +677,7 @@ def _kv8_workspace_bytes(cache: KV8, hq: int, rows: int, score_len: int, indexed
 
 def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor] = 0,
                new_lens: Optional[torch.Tensor] = None, close: bool = False) -> None:
-    """Appends k, v (bsz, Hkv, n, 128; any strides, contiguous last dimension) behind the first `start` rows of each
+    """Appends k, v (bsz, Hkv, n, 128; strides multiples of 8, contiguous last dimension) behind the first `start` rows of each
     request: an int, or an int32 GPU tensor (bsz,) of the requests' lengths.  new_lens (bsz,) int32: rows per request,
     at most n.  Blocks that fill become codes, the other rows wait in the open buffers; close=True quantises a
     short last block as well (start then an int at a block's border) and leaves the open buffers alone: such rows are
@@ -730,8 +730,10 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
                    score_lens: Optional[torch.Tensor] = None, scores_out: Optional[torch.Tensor] = None,
                    select_k: Optional[int] = None, k_per_seg: Optional[torch.Tensor] = None,
                    idx_out: Optional[torch.Tensor] = None):
-    """dense_attn over an 8-bit cache: q (bsz, Hq, 128) attends to the first seq_len rows (seq_lens: per request, on
-    the GPU) -> (bsz, Hq, 128); with `selector` also the filter layer's scores of the first score_len rows, from the same
+    """dense_attn over an 8-bit cache: q (bsz, Hq, 128) attends to the seq_len rows that each request holds (seq_lens: per
+    request, on the GPU, seq_len their bound) -> (bsz, Hq, 128).  The rows behind the last full block of that length are taken
+    from the open buffers: what is shorter than a request ends at a block's border, or goes through a KV8 of the same tensors
+    without them.  With `selector` also the filter layer's scores of the first score_len rows, from the same
     pass, and with `select_k` the ascending indices of the largest ones, as topk gives them: of a request's own rows alone,
     -1 (in idx_out: what was there) behind the last of them.  A request without rows gets zeros.  okv_kv8_dense_attn."""
     q, c = _kv8_query(q, cache)

@@ -2,8 +2,9 @@
 
 `PagePool` keeps the tensors that the page operations of `ops` work on (table, lens, refs; include/omnikv_hip.h,
 okv_page_pool_t) and the list of arrays whose pages move together: the pools of `ops.PagedKV` and the codes and scales of
-a paged `ops.KV8`, which read and write through the same `table`.  Nothing here waits for the GPU
-except `status()`; a step of page operations on tensors of sequence numbers can be captured in a HIP graph.
+a paged `ops.KV8`, which read and write through the same `table`.  Sequence numbers and token counts are int32 tensors on the
+GPU or lists of Python numbers.  With tensors nothing here waits for the GPU except `status()`, and a step of page operations
+can be captured in a HIP graph; a list is copied to the GPU first, which waits for the stream and cannot be captured.
 
 An 8-bit cache's open buffers belong to the sequences, not to the pages: `fork` copies a child's from its parent's, for
 every cache that `add_cache` named.
