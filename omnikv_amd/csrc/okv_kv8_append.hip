@@ -66,7 +66,7 @@ __device__ __forceinline__ float magnitude(const F16*, uint32_t bits) {
 // scale = max(amax / qmax, 2^-126), code = nearest(x * fl32(1 / scale)).  One workgroup per (touched block, kv head, request, K
 // or V): 16 lanes hold a row (eight elements each), sixteen rows per trip, the whole block in registers between
 // the two passes (maximum, then codes), so that each element is read once and written once.  Bound by that: 131073 tokens of
-// eight heads, bf16 to e4m3 in blocks of 64 (805 MB), 132 us = 6.1 TB/s; one token for each of sixteen requests a
+// eight heads, bf16 to e4m3 in blocks of 64 (805 MB), 134 us = 6.0 TB/s; one token for each of sixteen requests a
 // launch.  Rows come in and codes go out non-temporal (147 us without, 145 and 138 with one of the two); 152 before
 // the maximum was taken over bit patterns and the rows a block does not have were left out.
 // The workgroup of the first touched block also moves the rows of the block that stays open: it has read the old
