@@ -249,6 +249,11 @@ def dense_attn_window(q, q_window, k, v, selector: str = "uniform", seq_len: Opt
 def topk(scores: torch.Tensor, k: int, seq_lens: Optional[torch.Tensor] = None,
          k_per_seg: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(bsz, min(k, N)) int32 ascending indices of the k largest scores; okv_topk."""
+    return _topk(scores, k, seq_lens, k_per_seg, out, _workspace)
+
+
+def _topk(scores, k, seq_lens, k_per_seg, out, scratch) -> torch.Tensor:
+    """topk with its scratch from scratch(device, bytes)."""
     _require_gpu(scores, "scores")
     if scores.dtype != torch.float32 or scores.dim() != 2 or scores.stride(1) != 1:
         raise ValueError("scores must be (bsz, N) float32 with contiguous rows")
@@ -261,7 +266,7 @@ def topk(scores: torch.Tensor, k: int, seq_lens: Optional[torch.Tensor] = None,
             out = torch.full((batch, kk), -1, dtype=torch.int32, device=scores.device)
     if kk == 0:
         return out
-    ws = _workspace(scores.device, workspace_bytes(_lib.OKV_OP_TOPK, batch, 0, 0, 0, n))
+    ws = scratch(scores.device, workspace_bytes(_lib.OKV_OP_TOPK, batch, 0, 0, 0, n))
     check(lib().okv_topk(
         scores.data_ptr(), scores.stride(0), _lens(seq_lens, batch, "seq_lens"), n,
         _lens(k_per_seg, batch, "k_per_seg"), k, batch, out.data_ptr(), out.stride(0),
@@ -778,7 +783,7 @@ def kv8_dense_attn(q: torch.Tensor, cache: KV8, seq_len: Optional[int] = None, s
             ranked = score_lens
         else:
             ranked = seq_lens if score_lens is None else torch.minimum(seq_lens.view(-1), score_lens.view(-1))
-        return out, scores, topk(scores, select_k, ranked, k_per_seg, out=idx_out)
+        return out, scores, _topk(scores, select_k, ranked, k_per_seg, idx_out, _scratch)
 
 
 def kv8_sparse_attn(q: torch.Tensor, cache: KV8, idx: Optional[torch.Tensor] = None, sel_len: Optional[int] = None,

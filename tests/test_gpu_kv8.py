@@ -718,3 +718,39 @@ def test_a_selection_and_the_open_rows_as_its_tail(page):
         at = [torch.cat([i[i >= 0].long().cpu(), torch.arange(n // block * block, n)]) for i, n in zip(idx, lens)]
         assert all(a.numel() == min(k, n // block * block) + n % block for a, n in zip(at, lens))
         check_attention(got, q2, [x[:, a] for x, a in zip(k2, at)], [x[:, a] for x, a in zip(v2, at)], 128 ** -0.5, BF)
+
+
+def test_a_selection_uses_scratch_of_its_own(monkeypatch):
+    """None of the buffers that the 16-bit calls of a stream share: two captured graphs, replayed side by side, and eager
+    calls next to them select what each selects alone."""
+    g = torch.Generator().manual_seed(42)
+    n, k = 40000, 2700
+    cache, _, _ = make(g, "int8", BF, 64, 0, [n], 1)
+    qs = [rows(g, 1, 4).to(DEV) for _ in range(3)]
+
+    def call(q):
+        return ops.kv8_dense_attn(q, cache, seq_len=n, selector="last", score_len=n, select_k=k)[2]
+
+    with monkeypatch.context() as mp:
+        mp.setattr(ops, "_workspace", lambda *a: pytest.fail("shared scratch"))
+        want = [call(q) for q in qs]
+    for q, idx in zip(qs, want):
+        assert torch.equal(idx, ops.topk(ops.kv8_dense_attn(q, cache, seq_len=n, selector="last", score_len=n)[1], k))
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for q in qs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(call(q))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for idx in got:
+            idx.fill_(-1)
+        for s, graph in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = call(qs[2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got + [eager], want))
