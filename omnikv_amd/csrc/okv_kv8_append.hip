@@ -225,7 +225,7 @@ int okv_kv8_append(const okv_kv8_cache_t* cache, const void* new_k, int64_t k_to
   int rc = kv8_validate(cache, "okv_kv8_append");
   if (rc) return rc;
   const int B = cache->block_tokens;
-  OKV_REQUIRE(new_k && new_v, OKV_ERR_INVALID, "new_k or new_v is NULL");
+  OKV_REQUIRE((new_k && new_v) || max_new == 0, OKV_ERR_INVALID, "new_k or new_v is NULL");
   OKV_REQUIRE(batch >= 1 && max_new >= 0, OKV_ERR_INVALID, "bad batch or length");
   const AppendArgs a{*cache, {new_k, new_v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
                      {k_batch_stride, v_batch_stride}, starts, new_lens, start, max_new, close ? 1 : 0};
@@ -257,7 +257,7 @@ int okv_kv8_read(const okv_kv8_cache_t* cache, const int32_t* idx, int64_t idx_s
                  int64_t out_token_stride, int64_t out_head_stride, int64_t out_batch_stride, okv_stream_t stream) {
   int rc = kv8_validate(cache, "okv_kv8_read");
   if (rc) return rc;
-  OKV_REQUIRE(k_out && v_out, OKV_ERR_INVALID, "k_out or v_out is NULL");
+  OKV_REQUIRE((k_out && v_out) || max_rows == 0, OKV_ERR_INVALID, "k_out or v_out is NULL");
   OKV_REQUIRE(batch >= 1 && max_rows >= 0 && max_seq_len >= 0 && max_seq_len <= kv8_room(*cache), OKV_ERR_INVALID,
               "bad batch or length");
   if (idx) OKV_REQUIRE(idx_stride >= max_rows, OKV_ERR_INVALID, "idx_stride < max_rows");

@@ -155,3 +155,27 @@ def test_model_generates_with_an_8_bit_cache():
     got = [lm.generate_greedy(ids, 12) for lm in lms]
     assert torch.equal(got[0][0][:, :1], got[1][0][:, :1]) and torch.equal(got[0][1][0], got[1][1][0])
     assert got[1][0].shape == (1, 12) and all(bool(l.isfinite().all()) for l in got[1][1])
+
+
+def test_a_prompt_too_short_for_a_selection():
+    """A ratio that selects no row of a short prompt: the sparse layers attend to the generated tokens alone."""
+    g = torch.Generator().manual_seed(7)
+    cache, twin = (OmniKVMultiStageCache([0, 1, 4, 7], 7, 1, False, max_new_tokens=8, kv_format="int8", kv_block=16) for _ in "ab")
+    for i in range(7):
+        k, v = rows(g, 5, torch.bfloat16), rows(g, 5, torch.bfloat16)
+        for c in (cache, twin):
+            c.append(k, v, i)
+    for step in range(12):
+        cache.stage = twin.stage = "decoding"
+        for i in range(7):
+            k, v, q = rows(g, 1, torch.bfloat16), rows(g, 1, torch.bfloat16), rows(g, 1, torch.bfloat16, HQ)
+            cache.append(k, v, i)
+            if i in (1, 4):
+                out, idx = cache.attend_and_select(q, i, 0, 5, "softmax_before_last")
+                assert idx.shape == (1, 0)
+                twin.set_idx_on_gpu(idx, i)
+            else:
+                out = cache.attend(q, i)
+            kk, vv = twin.update(k, v, i)
+            assert kk.shape[2] == (step + 1 if i in (3, 6) else 5 + step + 1)
+            within(out, q, kk, vv, torch.bfloat16)

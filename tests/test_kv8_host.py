@@ -248,3 +248,13 @@ def test_pools_and_lists_beyond_what_the_plans_count_are_refused():
         ops.pages_free(meta(4, 8), meta(4), meta((1 << 32) + 5), meta(1), 16)
     with pytest.raises(ValueError, match="2\\^30"):
         ops.PageBuffers([meta((1 << 32) + 5, 4)])
+
+
+def test_calls_of_no_rows_need_no_arrays():
+    """An array without rows has no address."""
+    c, l = cache(), _lib.lib()
+    assert l.okv_kv8_read(C.byref(c), None, 0, 0, None, 10, 1, None, None, 128, 1280, 0, None) == 0
+    assert l.okv_kv8_read(C.byref(c), None, 0, 1, None, 10, 1, None, None, 128, 1280, 0, None) == INVALID
+    assert l.okv_kv8_append(C.byref(c), None, 1024, 128, 0, None, 1024, 128, 0, None, 0, None, 0, 0, 1, None) == 0
+    assert l.okv_kv8_append(C.byref(c), None, 1024, 128, 0, None, 1024, 128, 0, None, 0, None, 4, 0, 1, None) == INVALID
+    assert append(c, start=2000, n=0) == INVALID
